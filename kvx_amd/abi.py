@@ -158,6 +158,34 @@ class GatherDesc(C.Structure):
                 ("seq_lens", SeqLens), ("max_seq_len", C.c_uint32)]
 
 
+# kvx_ext.h's operators (no reference counterparts).
+
+class RopeStyle(enum.IntEnum):
+    HALF = 0
+    INTERLEAVED = 1
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("style", C.c_int), ("rot_dim", C.c_uint32),
+                ("magnitude", C.c_float), ("position_dtype", C.c_int), ("reserved", C.c_uint32),
+                ("positions", C.c_void_p), ("inv_freq", C.c_void_p), ("query", TensorDesc),
+                ("query_out", TensorDesc)]
+
+
+ATTENTION_CAUSAL = 1
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("size", C.c_uint32), ("flags", C.c_uint32), ("query", TensorDesc),
+                ("out", TensorDesc), ("lse", C.c_void_p), ("query_indptr", C.c_void_p),
+                ("query_indptr_dtype", C.c_int), ("window", C.c_uint32), ("scale", C.c_float),
+                ("softcap", C.c_float), ("max_seq_len", C.c_uint32),
+                ("max_query_len", C.c_uint32), ("block_table", BlockTable),
+                ("seq_lens", SeqLens), ("k_scale", ScaleDesc), ("v_scale", ScaleDesc),
+                ("pool_blocks", C.POINTER(PoolBlocks)), ("workspace", C.c_void_p),
+                ("workspace_size", C.c_uint64)]
+
+
 # Exported symbols and their argument lists (include/*.h).
 _P = C.POINTER
 _SIGS = {
@@ -172,6 +200,11 @@ _SIGS = {
                                      _P(ScaleDesc), C.c_void_p],
     "kvx_launch_gather_kv_pools": [_P(CacheDesc), _P(GatherDesc), _P(PoolBlocks), _P(ScaleDesc),
                                    _P(ScaleDesc), C.c_void_p],
+    "kvx_launch_rope_write_kv": [_P(CacheDesc), _P(WriteDesc), _P(RopeDesc), C.c_void_p],
+    "kvx_attention_workspace_size": [_P(CacheDesc), _P(AttentionDesc), _P(C.c_uint64)],
+    "kvx_launch_attention": [_P(CacheDesc), _P(AttentionDesc), C.c_void_p],
+    "kvx_launch_copy_blocks": [_P(_P(CacheDesc)), C.c_uint32, C.c_void_p, C.c_int, C.c_uint32,
+                               C.c_void_p],
 }
 for _t in ("f32", "f16", "bf16"):
     _SIGS[f"kvx_launch_write_kv_{_t}"] = [_P(CacheDesc), _P(WriteDesc), C.c_void_p]

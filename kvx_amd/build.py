@@ -33,7 +33,7 @@ LIB_PATH = PKG_DIR / "libkvx_amd.so"
 
 # The kernel families live in kernels_*.hip (one translation unit each, all
 # including kernels.h) so that they compile in parallel.
-SOURCES = ["abi.cpp", "launch.cpp", "dispatch.hip"] + sorted(
+SOURCES = ["abi.cpp", "launch.cpp", "operators.cpp", "dispatch.hip"] + sorted(
     p.name for p in CSRC.glob("kernels_*.hip"))
 ARCH = "gfx950"
 

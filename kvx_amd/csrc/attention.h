@@ -1,0 +1,257 @@
+// What the kernels of the attention over a paged cache share: their
+// arguments, the map from workgroups to query rows, and the map from token
+// numbers to cache rows.
+//
+// Rows.  A kv head's query rows are its `group` query heads at each new token.
+// A workgroup takes a tile of them: `tile_tokens` tokens by `tile_heads` heads
+// (the group, or a part of one wider than the tile), all of which read the
+// same keys and values.  Tiles are numbered without knowing each sequence's
+// length on the host: sequence s starts at tile begin(s) / tile_tokens + s,
+// begin(s) its first row.  That leaves every sequence room for its
+// ceil(n / tile_tokens) tiles, at most one of them unused.
+//
+// Splits.  Where the tiles alone do not fill the machine, a tile's tokens are
+// divided among `splits` workgroups.  Each writes its unnormalised sum, its
+// maximum and its sum of weights to the workspace, and
+// attention_join_kernel adds them up.
+//
+// Logits are kept in units of log2, so that a weight is one exp2.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "kernels.h"
+#include "kvx_internal.h"
+
+namespace kvx {
+namespace dev {
+
+constexpr int kRowTile = 16;  // rows of attention_rows_kernel's tile
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+struct AttentionArgs {
+  // cache and table
+  const char *k, *v;
+  const char *pool[2];
+  int64_t bytes_per_block;
+  int64_t table_count;
+  const void *table, *indptr, *lens;
+  GeomBytes gk, gv;
+  ScaleRef ks, vs;
+  int32_t pool_blocks[2];
+  int32_t format, index64, indptr64, lens64;
+  int32_t max_blocks, block_size, block_log2, num_blocks;  // block_log2 < 0: not a power of two
+  // queries; strides in bytes
+  const char *q;
+  char *out;
+  float *lse;
+  const void *qptr;
+  int64_t q_tok, q_head, o_tok, o_head;
+  int32_t qptr64;
+  int32_t seqs, tokens, heads, group, head_dim;
+  int32_t causal, window;
+  float scale_log2;  // scale * log2 e
+  float cap, cap_in; // softcap * log2 e and scale / softcap; cap 0: none
+  // tiles
+  int32_t tile_heads, head_tiles, tile_tokens, tiles;
+  int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
+  int32_t splits;
+  int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
+  float *part_o;      // [partial row, query head, split, head_dim]
+  float *part_ml;     // the same without head_dim: (maximum, sum of weights)
+  int32_t chunk_k, chunk_v;  // elements of a head that load together (rows kernel)
+};
+
+struct QueryTile {
+  int32_t seq;
+  int32_t first;   // first row of the tile in its sequence
+  int32_t count;   // tokens of the tile
+  int64_t begin;   // row number of the sequence's first row
+  int32_t rows;    // the sequence's new tokens
+  int64_t length;  // its cached tokens, as given
+  int32_t usable;  // of those, the ones the table can hold
+};
+
+__device__ __forceinline__ int64_t index_at(const void *p, bool is64, int64_t i) {
+  return is64 ? static_cast<const int64_t *>(p)[i] : (int64_t)static_cast<const int32_t *>(p)[i];
+}
+
+__device__ __forceinline__ int64_t query_begin(const AttentionArgs &a, int64_t s) {
+  const int64_t b = index_at(a.qptr, a.qptr64, s);
+  return b < 0 ? 0 : b > a.tokens ? a.tokens : b;
+}
+
+// The last s in [0, seqs) for which `before(s)`, a property that holds up to
+// some s, is true (0 where it never is): 64 pivots at a time.  Uniform over
+// the wave, all of whose lanes call.
+template <typename F>
+__device__ __forceinline__ int last_sequence(int seqs, const F &before) {
+  const int lane = (int)(threadIdx.x % kWave);
+  int lo = 0, span = seqs;
+  while (span > 1) {
+    const int step = (span + kWave - 1) / kWave;
+    const int hits = __popcll(__ballot(lane * step < span && before(lo + lane * step)));
+    const int at = hits > 0 ? hits - 1 : 0;
+    lo += at * step;
+    span = min(step, span - at * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The tile with number `tile`, or false where it has no rows or another
+// kernel takes its sequence.  Uniform over the wave, all of whose lanes call.
+__device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, QueryTile *t) {
+  if (a.qptr == nullptr) {
+    t->seq = tile;
+    t->first = 0;
+    t->count = 1;
+    t->begin = tile;
+    t->rows = 1;
+  } else {
+    const int lo = last_sequence(a.seqs, [&](int q) {
+      return query_begin(a, q) / a.tile_tokens + q <= (int64_t)tile;
+    });
+    const int64_t b = query_begin(a, lo), e = query_begin(a, lo + 1);
+    const int64_t j = tile - (b / a.tile_tokens + lo);
+    const int64_t n = e > b ? e - b : 0;
+    if (j < 0 || j * a.tile_tokens >= n || n < a.least_rows || n > a.most_rows) return false;
+    t->seq = lo;
+    t->begin = b;
+    t->rows = (int32_t)n;
+    t->first = (int32_t)j * a.tile_tokens;
+    t->count = min(a.tile_tokens, t->rows - t->first);
+  }
+  t->length = index_at(a.lens, a.lens64, t->seq);
+  int64_t hold;
+  if (a.format == KVX_BLOCK_TABLE_RAGGED) {
+    hold = index_at(a.indptr, a.indptr64, t->seq + 1) - index_at(a.indptr, a.indptr64, t->seq);
+    if (hold > 0x7FFF0000) hold = 0x7FFF0000;
+  } else {
+    hold = (int64_t)a.max_blocks * a.block_size;
+  }
+  hold = min(hold, t->length);
+  t->usable = hold < 0 ? 0 : (int32_t)hold;
+  return true;
+}
+
+// Tokens [lo, hi) that row i of the sequence attends to.
+__device__ __forceinline__ void row_range(const AttentionArgs &a, const QueryTile &t, int i,
+                                          int *lo, int *hi) {
+  *lo = 0;
+  *hi = t.usable;
+  if (!a.causal) return;
+  const int64_t pos = t.length - t.rows + i;
+  if (pos + 1 < t.usable) *hi = pos < 0 ? 0 : (int)(pos + 1);
+  if (a.window > 0 && pos - a.window + 1 > 0)
+    *lo = (int)min(pos - a.window + 1, (int64_t)t.usable);
+}
+
+// Tokens of split z of a tile that sees [lo, hi): whole steps of 64 from the
+// step that holds lo.
+__device__ __forceinline__ void split_range(int lo, int hi, int splits, int z, int *from, int *to) {
+  const int start = lo & ~63;
+  if (hi <= lo) {
+    *from = *to = start;
+    return;
+  }
+  const int steps = (hi - start + 63) >> 6;
+  const int per = (steps + splits - 1) / splits;
+  *from = min(start + z * per * 64, hi);
+  *to = min(start + (z + 1) * per * 64, hi);
+}
+
+// Where token `at` of a sequence lies: the addresses of its K and V rows (head
+// 0), or false for a token that is not there.  `block` is the physical block
+// for block-indexed scales.  `at` < the sequence's usable tokens.
+struct TokenRows {
+  const char *k, *v;
+  int32_t block;
+};
+
+__device__ __forceinline__ bool token_rows(const AttentionArgs &a, int seq, int at, TokenRows *r) {
+  int lb, off;
+  if (a.block_log2 >= 0) {
+    lb = at >> a.block_log2;
+    off = at - (lb << a.block_log2);
+  } else {
+    lb = at / a.block_size;
+    off = at - lb * a.block_size;
+  }
+  const char *kb, *vb;
+  if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
+    const uint32_t *t = static_cast<const uint32_t *>(a.table) + (int64_t)seq * 2 * a.max_blocks + lb;
+    const uint32_t ek = t[0], ev = t[a.max_blocks];
+    const char *pk = a.pool[ek >> 31], *pv = a.pool[ev >> 31];
+    const int32_t ik = (int32_t)(ek & 0x7FFFFFFFu), iv = (int32_t)(ev & 0x7FFFFFFFu);
+    if (pk == nullptr || pv == nullptr || ik >= a.pool_blocks[ek >> 31] ||
+        iv >= a.pool_blocks[ev >> 31])
+      return false;
+    kb = pk + ik * a.bytes_per_block;
+    vb = pv + iv * a.bytes_per_block;
+    r->block = 0;
+  } else {
+    int64_t i = (int64_t)seq * a.max_blocks + lb;
+    if (a.format == KVX_BLOCK_TABLE_RAGGED) {
+      i = index_at(a.indptr, a.indptr64, seq) + at;
+      if (i < 0 || i >= a.table_count) return false;
+    }
+    const int64_t b = index_at(a.table, a.index64, i);
+    if (b < 0 || b >= a.num_blocks) return false;
+    kb = a.k + b * a.gk.s_block;
+    vb = a.v + b * a.gv.s_block;
+    r->block = (int32_t)b;
+  }
+  r->k = kb + off * a.gk.s_off;
+  r->v = vb + off * a.gv.s_off;
+  return true;
+}
+
+__device__ __forceinline__ float scale_of(const ScaleRef &s, int32_t block, int32_t head) {
+  return s.p[s.indexed ? block * s.s_block + head * s.s_head : 0];
+}
+
+// x = scale * q.k (in log2 units) of a raw product.
+__device__ __forceinline__ float logit(const AttentionArgs &a, float dot) {
+  if (a.cap != 0.0f) return a.cap * tanhf(dot * a.cap_in);
+  return dot * a.scale_log2;
+}
+
+// One element of a cache or query tensor as f32.
+template <int C>
+__device__ __forceinline__ float value_at(const char *p) {
+  if constexpr (C == KVX_DTYPE_F32) return *reinterpret_cast<const float *>(p);
+  else if constexpr (C == KVX_DTYPE_BF16)
+    return bf16_to_f32(*reinterpret_cast<const uint16_t *>(p));
+  else if constexpr (C == KVX_DTYPE_F16) return (float)*reinterpret_cast<const _Float16 *>(p);
+  else return decode_pair<C == KVX_DTYPE_F8_E5M2>((int)*reinterpret_cast<const uint8_t *>(p), false)[0];
+}
+
+template <int C>
+constexpr int bytes_of_type() {
+  return C == KVX_DTYPE_F32 ? 4 : C == KVX_DTYPE_BF16 || C == KVX_DTYPE_F16 ? 2 : 1;
+}
+
+template <int IO>
+__device__ __forceinline__ void store_out(char *p, float x) {
+  if constexpr (IO == KVX_DTYPE_F32) *reinterpret_cast<float *>(p) = x;
+  else *reinterpret_cast<uint16_t *>(p) = (uint16_t)(pack_pair<IO>(f32x2{x, x}) & 0xFFFFu);
+}
+
+// Number of (row, head) among the partial results.
+__device__ __forceinline__ int64_t part_index(const AttentionArgs &a, const QueryTile &t, int i,
+                                              int head) {
+  const int64_t row = a.part_rows > 0 ? (int64_t)t.seq * a.part_rows + i : t.begin + i;
+  return row * (a.heads * a.group) + head;
+}
+
+// Other lanes of the wave see what this one wrote to LDS.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+void run_attention_rows(const AttentionArgs &a, int io, int cache, hipStream_t s);
+
+}  // namespace dev
+}  // namespace kvx

@@ -1,0 +1,212 @@
+// Host planning of the attention over a paged cache, and the kernel that
+// joins the splits of a tile.
+#include <hip/hip_runtime.h>
+
+#include "attention.h"
+#include "kvx_internal.h"
+
+namespace kvx {
+namespace dev {
+namespace {
+
+constexpr int kJoinThreads = 256;
+
+// Adds up the splits of one row and head: with M the largest maximum,
+//   out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
+// One wave has a row and head; the splits' partial sums are adjacent.
+template <int IO>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionArgs a) {
+  const int lane = (int)(threadIdx.x % kWave);
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const int hq = a.heads * a.group;
+  const int64_t unit = (int64_t)blockIdx.x * (kJoinThreads / kWave) + wave;
+  if (unit >= (int64_t)a.tokens * hq) return;
+  const int row = (int)(unit / hq), head = (int)(unit - (int64_t)row * hq);
+  int64_t part = row;
+  if (a.qptr != nullptr) {
+    const int s = last_sequence(a.seqs, [&](int q) { return query_begin(a, q) <= row; });
+    const int64_t b = query_begin(a, s), n = query_begin(a, s + 1) - b;
+    if (row < b || row >= b + n || n < a.least_rows || n > a.most_rows) return;
+    if (a.part_rows > 0) part = (int64_t)s * a.part_rows + (row - b);
+  }
+  const int64_t at = (part * hq + head) * a.splits;
+  float top = -INFINITY;
+  for (int z = lane; z < a.splits; z += kWave) top = fmaxf(top, a.part_ml[2 * (at + z)]);
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, sum[8] = {};
+  for (int z = 0; z < a.splits; ++z) {
+    const float l = a.part_ml[2 * (at + z) + 1];
+    if (l == 0.0f) continue;  // nothing was written for it
+    const float w = exp2f(a.part_ml[2 * (at + z)] - base);
+    total += w * l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int d = lane + j * kWave;
+      if (d < a.head_dim) sum[j] = fmaf(w, a.part_o[(at + z) * a.head_dim + d], sum[j]);
+    }
+  }
+  const bool none = top == -INFINITY && total == 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int d = lane + j * kWave;
+    if (d < a.head_dim)
+      store_out<IO>(a.out + row * a.o_tok + head * a.o_head + (int64_t)d * bytes_of_type<IO>(),
+                    none ? 0.0f : sum[j] / total);
+  }
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[(int64_t)row * hq + head] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+GeomBytes bytes_of(const Geom &g, int esize) {
+  return {g.s_block * esize, g.s_off * esize, g.s_head * esize, g.s_piece * esize,
+          g.s_inner * esize, g.pack, 0};
+}
+
+// `n` elements of a head that start at a multiple of n lie together and
+// aligned.
+bool chunks(const AttentionPlan &p, const Geom &g, const void *base, int n) {
+  const int e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
+  if (g.s_inner != 1 || g.pack % n != 0 || p.g.head_dim % n != 0) return false;
+  const int64_t b = (int64_t)n * e;
+  uint64_t low = (uint64_t)((g.s_off | g.s_head | g.s_piece) * e);
+  if (p.g.format == KVX_BLOCK_TABLE_KV_OFFSETS)
+    low |= (uint64_t)(uintptr_t)p.g.pool[0] | (uint64_t)(uintptr_t)p.g.pool[1] |
+           (uint64_t)p.g.bytes_per_block;
+  else
+    low |= (uint64_t)(uintptr_t)base | (uint64_t)(g.s_block * e);
+  return low % (uint64_t)b == 0;
+}
+
+// Most tokens that one sequence can have, as far as the host knows.
+int64_t longest(const AttentionPlan &p) {
+  const int64_t hold = p.g.format == KVX_BLOCK_TABLE_RAGGED
+                           ? p.g.table_count
+                           : (int64_t)p.g.max_blocks_per_seq * p.g.block_size;
+  return p.max_seq_len > 0 && p.max_seq_len < hold ? p.max_seq_len : hold;
+}
+
+// Rows of a kv head in tiles of at most `rows`.
+void tile_rows(AttentionArgs *a, int rows) {
+  a->tile_heads = a->group < rows ? a->group : rows;
+  a->head_tiles = (a->group + a->tile_heads - 1) / a->tile_heads;
+  a->tile_tokens = rows / a->tile_heads;
+  a->tiles = a->qptr != nullptr ? a->tokens / a->tile_tokens + a->seqs : a->seqs;
+}
+
+// Workgroups that share a tile's tokens, so that about `target` workgroups
+// run, each with at least `least` tokens of the longest sequence.
+int splits_for(const AttentionPlan &p, const AttentionArgs &a, int64_t target, int64_t least) {
+  const int64_t tiles = a.qptr != nullptr
+                            ? (a.tokens + a.tile_tokens - 1) / a.tile_tokens
+                            : a.seqs;
+  const int64_t units = tiles * a.heads * a.head_tiles;
+  int64_t n = target / (units > 0 ? units : 1);
+  const int64_t most = (longest(p) + least - 1) / least;
+  if (n > most) n = most;
+  // partial sums of at most 1 GiB
+  const int64_t each = (int64_t)a.tokens * a.heads * a.group * (a.head_dim + 2) * 4;
+  if (n * each > ((int64_t)1 << 30)) n = ((int64_t)1 << 30) / each;
+  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+}
+
+struct Plan {
+  AttentionArgs a;
+  bool rows;
+  uint64_t workspace;
+};
+
+Plan make_plan(const AttentionPlan &p) {
+  const GatherPlan &g = p.g;
+  const int cs = dtype_size((kvx_dtype_t)g.cache_dtype), is = dtype_size((kvx_dtype_t)g.io_dtype);
+  Plan r{};
+  AttentionArgs &a = r.a;
+  a.k = static_cast<const char *>(g.src_k);
+  a.v = static_cast<const char *>(g.src_v);
+  a.pool[0] = g.pool[0];
+  a.pool[1] = g.pool[1];
+  a.bytes_per_block = g.bytes_per_block;
+  a.table_count = g.table_count;
+  a.table = g.block_table;
+  a.indptr = g.indptr;
+  a.lens = g.seq_lens;
+  a.gk = bytes_of(g.gk, cs);
+  a.gv = bytes_of(g.gv, cs);
+  a.ks = g.k_scale;
+  a.vs = g.v_scale;
+  a.pool_blocks[0] = g.pool_blocks[0];
+  a.pool_blocks[1] = g.pool_blocks[1];
+  a.format = g.format;
+  a.index64 = g.index_is64;
+  a.indptr64 = g.indptr_is64;
+  a.lens64 = g.lens_is64;
+  a.max_blocks = g.max_blocks_per_seq;
+  a.block_size = g.block_size;
+  a.block_log2 = (g.block_size & (g.block_size - 1)) == 0 ? __builtin_ctz(g.block_size) : -1;
+  a.num_blocks = g.num_blocks;
+  a.q = static_cast<const char *>(p.query);
+  a.out = static_cast<char *>(p.out);
+  a.lse = p.lse;
+  a.qptr = p.query_indptr;
+  a.q_tok = p.q_tok * is;
+  a.q_head = p.q_head * is;
+  a.o_tok = p.o_tok * is;
+  a.o_head = p.o_head * is;
+  a.qptr64 = p.indptr_is64;
+  a.seqs = g.seq_count;
+  a.tokens = p.tokens;
+  a.heads = g.heads;
+  a.group = p.query_heads / g.heads;
+  a.head_dim = g.head_dim;
+  a.causal = p.causal;
+  a.window = p.window;
+  a.scale_log2 = p.scale * kLog2e;
+  a.cap = p.softcap * kLog2e;
+  a.cap_in = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
+  a.least_rows = 0;
+  a.most_rows = 0x7FFFFFFF;
+  r.rows = true;
+  tile_rows(&a, kRowTile);
+  a.chunk_k = chunks(p, g.gk, g.src_k, 4);
+  a.splits = splits_for(p, a, 1024, 256);
+  const int64_t parts = (int64_t)a.tokens * p.query_heads * a.splits;
+  r.workspace = a.splits > 1 ? (uint64_t)parts * (a.head_dim + 2) * 4 : 0;
+  a.part_o = static_cast<float *>(p.workspace);
+  a.part_ml = a.part_o + parts * a.head_dim;
+  return r;
+}
+
+template <int IO>
+void launch_join(const AttentionArgs &a, hipStream_t s) {
+  const int64_t units = (int64_t)a.tokens * a.heads * a.group;
+  const int64_t waves = kJoinThreads / kWave;
+  attention_join_kernel<IO><<<dim3((uint32_t)((units + waves - 1) / waves)), kJoinThreads, 0, s>>>(a);
+}
+
+bool launchable(const AttentionArgs &a) {
+  return (int64_t)a.heads * a.head_tiles <= 65535 && (int64_t)a.tiles * 1024 <= 0xFFFFFFFFll &&
+         (int64_t)a.tokens * a.heads * a.group * kWave <= 0xFFFFFFFFll;
+}
+
+}  // namespace
+}  // namespace dev
+
+using namespace dev;
+
+uint64_t attention_workspace(const AttentionPlan &p) { return make_plan(p).workspace; }
+
+kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
+  const Plan plan = make_plan(p);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (!launchable(plan.a)) return KVX_STATUS_UNSUPPORTED;
+  run_attention_rows(plan.a, p.g.io_dtype, p.g.cache_dtype, s);
+  if (plan.a.splits > 1) {
+    if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(plan.a, s);
+    else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(plan.a, s);
+    else launch_join<KVX_DTYPE_BF16>(plan.a, s);
+  }
+  return hipGetLastError() == hipSuccess ? KVX_STATUS_OK : KVX_STATUS_INTERNAL_ERROR;
+}
+
+}  // namespace kvx

@@ -20,13 +20,14 @@
 #include "kvx_paged_kv.h"
 
 namespace kvx {
-namespace {
 
 bool is_io_float(kvx_dtype_t dt) {
   return dt == KVX_DTYPE_F16 || dt == KVX_DTYPE_BF16 || dt == KVX_DTYPE_F32;
 }
 
 bool is_fp8(kvx_dtype_t dt) { return dt == KVX_DTYPE_F8_E4M3 || dt == KVX_DTYPE_F8_E5M2; }
+
+namespace {
 
 // reference kvx_paged_kv.cu:269-289 (no size/dtype/data checks on this path)
 kvx_status_t check_io_3d(const kvx_tensor_desc_t *t, int32_t num_tokens,
@@ -55,6 +56,8 @@ kvx_status_t check_io_4d(const kvx_tensor_desc_t *t, int32_t seq_count,
     return KVX_STATUS_UNSUPPORTED;
   return KVX_STATUS_OK;
 }
+
+}  // namespace
 
 // Descriptor -> Geom.  Status codes as reference kvx_fill_cache_params
 // (kernels/kvx_paged_kv.cu:18-52): PACKED needs pack > 0 dividing head_dim;
@@ -187,8 +190,6 @@ kvx_status_t resolve_write_scale(const kvx_scale_desc_t *desc, const void *raw,
   *out = ScaleRef{static_cast<const float *>(raw), 0, 0, 0, 0};
   return KVX_STATUS_OK;
 }
-
-}  // namespace
 
 // `expected` is the payload dtype of the per-dtype helper; KVX_DTYPE_F8_E4M3
 // and KVX_DTYPE_F8_E5M2 are this build's FP8 paths, where io may be

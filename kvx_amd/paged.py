@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import importlib.util
+import math
 import warnings
 from dataclasses import dataclass
 from pathlib import Path
@@ -444,3 +445,302 @@ def gather_kv(cache: PagedCache, key_out: torch.Tensor, value_out: torch.Tensor,
         return Status(lib.kvx_launch_gather_kv_dequant(C.byref(cd), C.byref(gd),
                                                        C.byref(ks), C.byref(vs), s))
     return Status(lib.kvx_launch_gather_kv(C.byref(cd), C.byref(gd), s))
+
+
+# ---------------------------------------------------------------------------
+# Operators of a serving step beside the write and the gather (kvx_ext.h; no
+# reference counterparts).
+
+@dataclass
+class Rope:
+    """Rotary positions: pair i of a head turns by position * inv_freq[i].
+    `inv_freq` is a contiguous float32 device tensor [rot_dim / 2]
+    (``rope_frequencies``); elements of a head from rot_dim on are not
+    rotated.  `interleaved` pairs are (2 i, 2 i + 1), others (i, i + rot_dim /
+    2); `magnitude` multiplies cosines and sines."""
+
+    inv_freq: torch.Tensor
+    interleaved: bool = False
+    magnitude: float = 1.0
+
+
+def rope_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: str | None = None,
+                     factor: float = 1.0, original_length: int | None = None,
+                     low_freq_factor: float = 1.0, high_freq_factor: float = 4.0,
+                     beta_fast: float = 32.0, beta_slow: float = 1.0,
+                     magnitude: float | None = None, device=None) -> tuple[torch.Tensor, float]:
+    """(inv_freq, magnitude) of a checkpoint's rotary settings, computed in 64
+    bits: inv_freq[i] = base ** (-2 i / rot_dim) in float32, scaled for
+    contexts `factor` times the trained `original_length`:
+
+      None      as they are
+      "linear"  all frequencies / factor
+      "ntk"     base * factor ** (rot_dim / (rot_dim - 2))
+      "llama3"  waves longer than original_length / low_freq_factor are
+                slowed by factor, those shorter than original_length /
+                high_freq_factor kept, those between blended by the number
+                of turns in original_length
+      "yarn"    pairs that turn fewer than beta_slow times in original_length
+                are slowed by factor, those that turn more than beta_fast
+                times kept, those between blended by their index; the
+                magnitude is 0.1 ln(factor) + 1
+
+    A given `magnitude` replaces the rule's."""
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError(f"rot_dim {rot_dim} is not a positive even number")
+    if not base > 1.0 or not factor > 0.0:
+        raise ValueError(f"base {base} or factor {factor} out of range")
+    if scaling in ("llama3", "yarn") and not (original_length and original_length > 0):
+        raise ValueError(f"scaling {scaling!r} needs original_length")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    gain = 1.0
+    if scaling == "ntk":
+        if rot_dim == 2:
+            raise ValueError("scaling 'ntk' needs rot_dim > 2")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    inv = torch.pow(torch.tensor(base, dtype=torch.float64), -2.0 * i / rot_dim)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "llama3":
+        if not high_freq_factor > low_freq_factor:
+            raise ValueError("high_freq_factor must exceed low_freq_factor")
+        turns = original_length * inv / (2 * math.pi)
+        keep = ((turns - low_freq_factor) / (high_freq_factor - low_freq_factor)).clamp(0, 1)
+        inv = inv * (keep + (1 - keep) / factor)
+    elif scaling == "yarn":
+        def pair_with(turns: float) -> float:
+            return (rot_dim * math.log(original_length / (2 * math.pi * turns))
+                    / (2 * math.log(base)))
+
+        low = max(math.floor(pair_with(beta_fast)), 0)
+        high = min(math.ceil(pair_with(beta_slow)), rot_dim - 1)
+        slowed = ((i - low) / max(high - low, 0.001)).clamp(0, 1)
+        inv = inv * (1 - slowed + slowed / factor)
+        gain = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return inv.float().to(device or "cpu"), gain if magnitude is None else float(magnitude)
+
+
+def _on_one_gpu(first: torch.Tensor, **tensors) -> torch.device:
+    """The device of all tensors; ValueError names one that is elsewhere."""
+    if not first.is_cuda:
+        raise ValueError("the cache is not on a GPU")
+    for name, t in tensors.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {first.device}")
+    return first.device
+
+
+def _indices(name: str, t: torch.Tensor, shape: tuple | None = None) -> torch.Tensor:
+    """`t`, an int32 / int64 tensor whose elements lie in order."""
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} is {t.dtype}, not int32 or int64")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} is not contiguous")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
+    return t
+
+
+def _row_tensor(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 3:
+        raise ValueError(f"{name} is not [tokens, heads, head_dim]")
+    return t
+
+
+def build_rope(query: torch.Tensor | None, query_out: torch.Tensor | None,
+               positions: torch.Tensor, rope: Rope) -> abi.RopeDesc:
+    """kvx_rope_desc_t for [T, Hq, D] queries (or None) and [T] positions."""
+    d = abi.RopeDesc()
+    d.size = C.sizeof(abi.RopeDesc)
+    d.style = int(abi.RopeStyle.INTERLEAVED if rope.interleaved else abi.RopeStyle.HALF)
+    d.rot_dim = 2 * rope.inv_freq.numel()
+    d.magnitude = rope.magnitude
+    d.position_dtype = int(dtype_code(positions))
+    d.positions = positions.data_ptr()
+    d.inv_freq = rope.inv_freq.data_ptr()
+    if query is not None:
+        d.query = tensor_desc(query)
+        d.query_out = tensor_desc(query_out)
+    return d
+
+
+def rope_write_kv(cache: PagedCache, query: torch.Tensor | None, key: torch.Tensor,
+                  value: torch.Tensor, positions: torch.Tensor, rope: Rope,
+                  slot_mapping: torch.Tensor, *, query_out: torch.Tensor | None = None,
+                  k_scale=None, v_scale=None, stream=None) -> Status:
+    """Rotates [T, Hq, D] queries into `query_out` (None: in place) and
+    [T, H, D] keys into the paged cache, and writes the values beside them:
+    ``write_kv`` of the rotated keys, each element rounded once.  Tensors may
+    have any token and head strides (views of one projection's output).  A
+    slot of -1 skips a row's key and value; its query is rotated.  `query`
+    None: keys and values alone.  kvx_launch_rope_write_kv."""
+    lib = abi.load()
+    if query is not None and query_out is None:
+        query_out = query
+    device = _on_one_gpu(cache.key_cache, value_cache=cache.value_cache, query=query, key=key,
+                         value=value, positions=positions, inv_freq=rope.inv_freq,
+                         slot_mapping=slot_mapping, query_out=query_out)
+    T = _row_tensor("key", key).shape[0]
+    _row_tensor("value", value)
+    if query is not None:
+        _row_tensor("query", query)
+        _row_tensor("query_out", query_out)
+    _indices("positions", positions, (T,))
+    _indices("slot_mapping", slot_mapping, (T,))
+    if rope.inv_freq.dtype != torch.float32 or not rope.inv_freq.is_contiguous():
+        raise ValueError("inv_freq is not a contiguous float32 tensor")
+    cd = cache.desc()
+    wd = build_write(cache, key, value, slot_mapping, k_scale, v_scale)
+    rd = build_rope(query, query_out, positions, rope)
+    with torch.cuda.device(device):
+        return Status(lib.kvx_launch_rope_write_kv(C.byref(cd), C.byref(wd), C.byref(rd),
+                                                   _stream_handle(stream)))
+
+
+def build_attention(query: torch.Tensor, out: torch.Tensor, block_table, seq_lens: torch.Tensor,
+                    query_indptr: torch.Tensor | None = None, *, causal: bool = True,
+                    scale: float | None = None, window: int = 0, softcap: float = 0.0,
+                    lse: torch.Tensor | None = None, max_seq_len: int = 0,
+                    max_query_len: int = 0, k_scale=None, v_scale=None) -> abi.AttentionDesc:
+    """kvx_attention_desc_t, without workspace and pool counts."""
+    d = abi.AttentionDesc()
+    d.size = C.sizeof(abi.AttentionDesc)
+    d.flags = abi.ATTENTION_CAUSAL if causal else 0
+    d.query = tensor_desc(query)
+    d.out = tensor_desc(out)
+    d.lse = None if lse is None else lse.data_ptr()
+    if query_indptr is not None:
+        d.query_indptr = query_indptr.data_ptr()
+        d.query_indptr_dtype = int(dtype_code(query_indptr))
+    d.window = window
+    d.scale = query.shape[-1] ** -0.5 if scale is None else scale
+    d.softcap = softcap
+    d.max_seq_len = max_seq_len
+    d.max_query_len = max_query_len
+    d.block_table = _table_desc(block_table)
+    d.seq_lens = abi.make_seq_lens(seq_lens.numel(), dtype_code(seq_lens), seq_lens.data_ptr())
+    if k_scale is not None:
+        d.k_scale = scale_desc_of(k_scale)
+    if v_scale is not None:
+        d.v_scale = scale_desc_of(v_scale)
+    return d
+
+
+def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_table,
+              seq_lens: torch.Tensor, query_indptr: torch.Tensor | None = None, *,
+              causal: bool = True, scale: float | None = None, window: int = 0,
+              softcap: float = 0.0, lse: torch.Tensor | None = None, max_seq_len: int = 0,
+              max_query_len: int = 0, k_scale=None, v_scale=None,
+              pool_blocks: tuple[int, int] | None = None,
+              workspace: torch.Tensor | None = None, stream=None) -> Status:
+    """Attention of new tokens over the paged cache that holds them already.
+
+    Sequence s has the rows query_indptr[s] .. query_indptr[s + 1] - 1 of
+    `query` [T, Hq, D] (`query_indptr` None: the one row s, a decode step) and
+    seq_lens[s] cached tokens, the new ones last.  A row at position p attends
+    to the tokens up to p (`causal`; else to all), with a `window` only to the
+    last `window` of them.  softmax(scale * q.k) v goes to `out` (like
+    `query`), the natural logarithm of the weights' sum to `lse` (float32 [T,
+    Hq], or None); `scale` is 1 / sqrt(D) unless given; `softcap` > 0 turns a
+    logit x into softcap * tanh(x / softcap).  Hq is a multiple of the cache's
+    heads.  Rows that attend to nothing are 0 with lse -inf; rows behind the
+    last sequence are left as they were.  `block_table`, `k_scale`, `v_scale`
+    and `pool_blocks` as in ``gather_kv``.
+
+    `max_seq_len` and `max_query_len`, the largest values in this batch, steer
+    how the work is split (0: not known) and not the result.  `workspace` is a
+    uint8 tensor of ``attention_workspace_size`` bytes, one for each call that
+    may run at the same time; None allocates it.  kvx_launch_attention."""
+    lib = abi.load()
+    table_tensors = {}
+    if isinstance(block_table, RaggedTable):
+        table_tensors = {"indices": _indices("indices", block_table.indices),
+                         "indptr": _indices("indptr", block_table.indptr)}
+    elif isinstance(block_table, OffsetsTable):
+        table_tensors = {"offsets": _indices("offsets", block_table.offsets),
+                         "primary": block_table.primary, "secondary": block_table.secondary}
+    else:
+        table_tensors = {"block_table": _indices("block_table", block_table)}
+        if block_table.dim() != 2:
+            raise ValueError("block_table is not [sequences, blocks]")
+    device = _on_one_gpu(cache.key_cache, value_cache=cache.value_cache, query=query, out=out,
+                         seq_lens=seq_lens, query_indptr=query_indptr, lse=lse,
+                         workspace=workspace, **table_tensors)
+    _row_tensor("query", query)
+    _row_tensor("out", out)
+    cd = gather_cache_desc(cache, block_table)
+    d = build_attention(query, out, block_table, seq_lens, query_indptr, causal=causal,
+                        scale=scale, window=window, softcap=softcap, lse=lse,
+                        max_seq_len=max_seq_len, max_query_len=max_query_len, k_scale=k_scale,
+                        v_scale=v_scale)
+    S = d.block_table.seq_count
+    _indices("seq_lens", seq_lens, (S,))
+    if query_indptr is not None:
+        _indices("query_indptr", query_indptr, (S + 1,))
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous()
+                            or tuple(lse.shape) != tuple(query.shape[:2])):
+        raise ValueError("lse is not a contiguous float32 [T, Hq] tensor")
+    pools = None
+    if pool_blocks is not None:
+        pools = abi.PoolBlocks(C.sizeof(abi.PoolBlocks), 0, pool_blocks[0], pool_blocks[1])
+        d.pool_blocks = C.pointer(pools)
+    size = C.c_uint64()
+    st = Status(lib.kvx_attention_workspace_size(C.byref(cd), C.byref(d), C.byref(size)))
+    if st != Status.OK:
+        return st
+    with torch.cuda.device(device):
+        if workspace is None and size.value:
+            if isinstance(stream, int):
+                stream = torch.cuda.ExternalStream(stream)
+            # of the stream that uses it, so that it is not handed out before
+            with torch.cuda.stream(stream):
+                workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+        if workspace is not None:
+            if not workspace.is_contiguous():
+                raise ValueError("workspace is not contiguous")
+            d.workspace = workspace.data_ptr()
+            d.workspace_size = workspace.numel() * workspace.element_size()
+        return Status(lib.kvx_launch_attention(C.byref(cd), C.byref(d), _stream_handle(stream)))
+
+
+def attention_workspace_size(cache: PagedCache, query: torch.Tensor, block_table,
+                             seq_lens: torch.Tensor, query_indptr: torch.Tensor | None = None, *,
+                             max_seq_len: int = 0, max_query_len: int = 0, k_scale=None,
+                             v_scale=None) -> int:
+    """Bytes of workspace that ``attention`` needs for such arguments."""
+    cd = gather_cache_desc(cache, block_table)
+    d = build_attention(query, query, block_table, seq_lens, query_indptr,
+                        max_seq_len=max_seq_len, max_query_len=max_query_len, k_scale=k_scale,
+                        v_scale=v_scale)
+    size = C.c_uint64()
+    st = Status(abi.load().kvx_attention_workspace_size(C.byref(cd), C.byref(d), C.byref(size)))
+    if st != Status.OK:
+        raise ValueError(f"no attention for these arguments: {st.name}")
+    return size.value
+
+
+def copy_blocks(caches, pairs: torch.Tensor, *, stream=None) -> Status:
+    """Copies blocks inside the caches of a model's layers: for each row (src,
+    dst) of `pairs` (int32 / int64 [n, 2]) block src of K and V to block dst,
+    in every PagedCache of `caches`.  Rows with an id outside the pool (such
+    as -1 padding) are skipped; no dst may be the src or dst of another row.
+    Block-indexed FP8 scales are the caller's to copy.
+    kvx_launch_copy_blocks."""
+    lib = abi.load()
+    caches = list(caches)
+    _indices("pairs", pairs)
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError(f"pairs has shape {tuple(pairs.shape)}, not (n, 2)")
+    if not caches:
+        return Status.OK
+    device = _on_one_gpu(caches[0].key_cache, pairs=pairs)
+    for c in caches:
+        _on_one_gpu(caches[0].key_cache, key_cache=c.key_cache, value_cache=c.value_cache)
+    descs = [c.desc() for c in caches]
+    ptrs = (C.POINTER(abi.CacheDesc) * len(descs))(*[C.pointer(d) for d in descs])
+    with torch.cuda.device(device):
+        return Status(lib.kvx_launch_copy_blocks(ptrs, len(descs), pairs.data_ptr(),
+                                                 int(dtype_code(pairs)), pairs.shape[0],
+                                                 _stream_handle(stream)))
