@@ -57,6 +57,7 @@ struct AttentionArgs {
   int32_t tile_heads, head_tiles, tile_tokens, tiles;
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
   int32_t splits;
+  int32_t split_steps;  // least steps of 64 tokens in a split
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
   float *part_ml;     // the same without head_dim: (maximum, sum of weights)
@@ -147,18 +148,19 @@ __device__ __forceinline__ void row_range(const AttentionArgs &a, const QueryTil
     *lo = (int)min(pos - a.window + 1, (int64_t)t.usable);
 }
 
-// Tokens of split z of a tile that sees [lo, hi): whole steps of 64 from the
-// step that holds lo.
-__device__ __forceinline__ void split_range(int lo, int hi, int splits, int z, int *from, int *to) {
+// Tokens of split z of a tile that sees [lo, hi): split_tokens each, or more
+// where the sequence is longer than the host knew; from a multiple of 64 on.
+__device__ __forceinline__ void split_range(const AttentionArgs &a, int lo, int hi, int z,
+                                            int *from, int *to) {
   const int start = lo & ~63;
   if (hi <= lo) {
     *from = *to = start;
     return;
   }
   const int steps = (hi - start + 63) >> 6;
-  const int per = (steps + splits - 1) / splits;
-  *from = min(start + z * per * 64, hi);
-  *to = min(start + (z + 1) * per * 64, hi);
+  const int per = max((steps + a.splits - 1) / a.splits, a.split_steps);
+  *from = (int)min((int64_t)start + (int64_t)z * per * 64, (int64_t)hi);
+  *to = (int)min((int64_t)start + (int64_t)(z + 1) * per * 64, (int64_t)hi);
 }
 
 // Where token `at` of a sequence lies: the addresses of its K and V rows (head
@@ -182,11 +184,12 @@ __device__ __forceinline__ bool token_rows(const AttentionArgs &a, int seq, int 
   if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
     const uint32_t *t = static_cast<const uint32_t *>(a.table) + (int64_t)seq * 2 * a.max_blocks + lb;
     const uint32_t ek = t[0], ev = t[a.max_blocks];
-    const char *pk = a.pool[ek >> 31], *pv = a.pool[ev >> 31];
+    // selected, not indexed: arguments stay in scalar registers
+    const char *pk = ek >> 31 ? a.pool[1] : a.pool[0], *pv = ev >> 31 ? a.pool[1] : a.pool[0];
+    const int32_t nk = ek >> 31 ? a.pool_blocks[1] : a.pool_blocks[0];
+    const int32_t nv = ev >> 31 ? a.pool_blocks[1] : a.pool_blocks[0];
     const int32_t ik = (int32_t)(ek & 0x7FFFFFFFu), iv = (int32_t)(ev & 0x7FFFFFFFu);
-    if (pk == nullptr || pv == nullptr || ik >= a.pool_blocks[ek >> 31] ||
-        iv >= a.pool_blocks[ev >> 31])
-      return false;
+    if (pk == nullptr || pv == nullptr || ik >= nk || iv >= nv) return false;
     kb = pk + ik * a.bytes_per_block;
     vb = pv + iv * a.bytes_per_block;
     r->block = 0;
@@ -252,6 +255,13 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 void run_attention_rows(const AttentionArgs &a, int io, int cache, hipStream_t s);
+// vt: values with the token axis innermost
+void run_attention_few_bf16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_few_bf16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_few_f16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
 
 }  // namespace dev
 }  // namespace kvx

@@ -97,25 +97,66 @@ void tile_rows(AttentionArgs *a, int rows) {
 
 // Workgroups that share a tile's tokens, so that about `target` workgroups
 // run, each with at least `least` tokens of the longest sequence.
-int splits_for(const AttentionPlan &p, const AttentionArgs &a, int64_t target, int64_t least) {
-  const int64_t tiles = a.qptr != nullptr
-                            ? (a.tokens + a.tile_tokens - 1) / a.tile_tokens
-                            : a.seqs;
-  const int64_t units = tiles * a.heads * a.head_tiles;
+void split_tokens(const AttentionPlan &p, AttentionArgs *a, int64_t target, int64_t least) {
+  const int64_t tiles =
+      a->qptr != nullptr ? (a->tokens + a->tile_tokens - 1) / a->tile_tokens : a->seqs;
+  const int64_t units = tiles * a->heads * a->head_tiles;
+  const int64_t tokens = longest(p);
   int64_t n = target / (units > 0 ? units : 1);
-  const int64_t most = (longest(p) + least - 1) / least;
-  if (n > most) n = most;
+  if (n > tokens / least) n = tokens / least;
   // partial sums of at most 1 GiB
-  const int64_t each = (int64_t)a.tokens * a.heads * a.group * (a.head_dim + 2) * 4;
+  const int64_t each = (int64_t)a->tokens * a->heads * a->group * (a->head_dim + 2) * 4;
   if (n * each > ((int64_t)1 << 30)) n = ((int64_t)1 << 30) / each;
-  return (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  a->splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  a->split_steps = (int)((tokens + 64 * (int64_t)a->splits - 1) / (64 * (int64_t)a->splits));
 }
+
+enum Kind { kRows, kFew };
 
 struct Plan {
   AttentionArgs a;
-  bool rows;
+  Kind kind;
+  bool vt;
   uint64_t workspace;
 };
+
+// Four tokens of one element of a value lie together and aligned.
+bool tokens_inner(const AttentionPlan &p) {
+  const Geom &g = p.g.gv;
+  const int e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
+  if (g.s_off != 1 || p.g.block_size % 4 != 0 || p.g.format == KVX_BLOCK_TABLE_RAGGED) return false;
+  uint64_t low = (uint64_t)((g.s_inner | g.s_head | g.s_piece) * e);
+  if (p.g.format == KVX_BLOCK_TABLE_KV_OFFSETS)
+    low |= (uint64_t)(uintptr_t)p.g.pool[0] | (uint64_t)(uintptr_t)p.g.pool[1] |
+           (uint64_t)p.g.bytes_per_block;
+  else
+    low |= (uint64_t)(uintptr_t)p.g.src_v | (uint64_t)(g.s_block * e);
+  return low % (uint64_t)(4 * e) == 0;
+}
+
+// Offsets inside a head fit 32 bits.
+bool near(const AttentionPlan &p, const Geom &g) {
+  const int64_t e = dtype_size((kvx_dtype_t)p.g.cache_dtype), most = (int64_t)1 << 30;
+  const int64_t pieces = p.g.head_dim / g.pack;
+  return g.s_piece >= 0 && g.s_inner >= 0 && g.s_piece < most && g.s_inner < most &&
+         (pieces * g.s_piece + (int64_t)g.pack * g.s_inner) * e < most;
+}
+
+// The matrix-core kernels read queries and write outputs 8 elements at a time,
+// keys 16 bytes and values DP / 16 elements (or four tokens) at a time.
+bool matrix_cores(const AttentionPlan &p, bool *vt) {
+  const int D = p.g.head_dim, e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
+  if (p.g.io_dtype == KVX_DTYPE_F32 || D % 8 != 0 || D > 256) return false;
+  if (((p.q_tok | p.q_head | p.o_tok | p.o_head) % 8) != 0 ||
+      (uintptr_t)p.query % 16 != 0 || (uintptr_t)p.out % 16 != 0)
+    return false;
+  if (!near(p, p.g.gk) || !near(p, p.g.gv) || !chunks(p, p.g.gk, p.g.src_k, 16 / e)) return false;
+  const int per_lane = D <= 64 ? 4 : D <= 128 || e == 2 ? 8 : 16;
+  *vt = false;
+  if (chunks(p, p.g.gv, p.g.src_v, per_lane)) return true;
+  *vt = tokens_inner(p);
+  return *vt;
+}
 
 Plan make_plan(const AttentionPlan &p) {
   const GatherPlan &g = p.g;
@@ -166,10 +207,14 @@ Plan make_plan(const AttentionPlan &p) {
   a.cap_in = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
   a.least_rows = 0;
   a.most_rows = 0x7FFFFFFF;
-  r.rows = true;
   tile_rows(&a, kRowTile);
-  a.chunk_k = chunks(p, g.gk, g.src_k, 4);
-  a.splits = splits_for(p, a, 1024, 256);
+  r.kind = matrix_cores(p, &r.vt) ? kFew : kRows;
+  if (r.kind == kFew) {
+    split_tokens(p, &a, 3072, 512);
+  } else {
+    a.chunk_k = chunks(p, g.gk, g.src_k, 4);
+    split_tokens(p, &a, 1024, 256);
+  }
   const int64_t parts = (int64_t)a.tokens * p.query_heads * a.splits;
   r.workspace = a.splits > 1 ? (uint64_t)parts * (a.head_dim + 2) * 4 : 0;
   a.part_o = static_cast<float *>(p.workspace);
@@ -184,9 +229,26 @@ void launch_join(const AttentionArgs &a, hipStream_t s) {
   attention_join_kernel<IO><<<dim3((uint32_t)((units + waves - 1) / waves)), kJoinThreads, 0, s>>>(a);
 }
 
-bool launchable(const AttentionArgs &a) {
-  return (int64_t)a.heads * a.head_tiles <= 65535 && (int64_t)a.tiles * 1024 <= 0xFFFFFFFFll &&
-         (int64_t)a.tokens * a.heads * a.group * kWave <= 0xFFFFFFFFll;
+int64_t few_grid(const AttentionArgs &a) {
+  return (int64_t)a.tiles * a.splits * a.heads * a.head_tiles;
+}
+
+bool launchable(const Plan &p) {
+  const AttentionArgs &a = p.a;
+  if ((int64_t)a.tokens * a.heads * a.group * kWave > 0xFFFFFFFFll) return false;
+  if (p.kind == kFew) return few_grid(a) * 256 <= 0xFFFFFFFFll;
+  return (int64_t)a.heads * a.head_tiles <= 65535 && (int64_t)a.tiles * 256 <= 0xFFFFFFFFll;
+}
+
+void run_few(const Plan &p, int io, int cache, hipStream_t s) {
+  const int64_t grid = few_grid(p.a);
+  const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
+  if (io == KVX_DTYPE_BF16)
+    (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
+                                           : run_attention_few_bf16)(p.a, p.vt, grid, s);
+  else
+    (e4 ? run_attention_few_f16_e4m3 : e5 ? run_attention_few_f16_e5m2
+                                          : run_attention_few_f16)(p.a, p.vt, grid, s);
 }
 
 }  // namespace
@@ -199,8 +261,9 @@ uint64_t attention_workspace(const AttentionPlan &p) { return make_plan(p).works
 kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
   const Plan plan = make_plan(p);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (!launchable(plan.a)) return KVX_STATUS_UNSUPPORTED;
-  run_attention_rows(plan.a, p.g.io_dtype, p.g.cache_dtype, s);
+  if (!launchable(plan)) return KVX_STATUS_UNSUPPORTED;
+  if (plan.kind == kFew) run_few(plan, p.g.io_dtype, p.g.cache_dtype, s);
+  else run_attention_rows(plan.a, p.g.io_dtype, p.g.cache_dtype, s);
   if (plan.a.splits > 1) {
     if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(plan.a, s);
     else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(plan.a, s);

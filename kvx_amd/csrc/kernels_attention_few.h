@@ -1,0 +1,676 @@
+// Attention of few rows per kv head (decode steps, drafts, short chunks) on
+// the matrix cores.
+//
+// Every cached key and value is read once per tile of 16 rows and takes part
+// in 16 products of each kind (4 * 16 operations for 2 elements), far below
+// the matrix rate: HBM bounds it, and all that matters is loads in flight.  So
+// the waves do not share anything while they run: a wave takes every fourth
+// step of 32 tokens of its workgroup's range, loads its keys and values
+// straight from HBM into the registers that the matrix instructions read, and
+// the four waves join their sums through LDS at the end.
+//
+// v_mfma_f32_16x16x32: lane l = 16 g + c holds A[row c][8 g .. 8 g + 7],
+// B[8 g .. 8 g + 7][column c] and D[rows 4 g .. 4 g + 3][column c].
+//
+//   S^T = K Q^T   A: 16 tokens, so that lane c reads 16 bytes of token c's key
+//                 where they lie.  D: lane c has row c of the queries, tokens
+//                 4 g + i of each half of the step.
+//   O^T = V^T P^T B: row c's weights of tokens 4 g + i and 16 + 4 g + i, which
+//                 are the lane's own logits; no exchange.  The order of the
+//                 sum's 32 tokens is free, so A takes them in the same order.
+//                 A: values by element, tokens across.  From rows, a lane
+//                 loads NV = DP / 16 elements of eight tokens and transposes
+//                 them with v_perm (half an operation an element); from a
+//                 cache whose token axis is innermost it loads four tokens of
+//                 one element, as they are.
+//
+// Maximum and sum are one register each, as a lane has one row; the maximum
+// is shared over the four lane groups, the sum only at the end.  Weights are
+// rounded to the queries' type for the product (half a step of 2^-8 or 2^-11
+// relative, as the output is rounded), their sum is not.
+#pragma once
+
+#include "attention.h"
+
+namespace kvx {
+namespace dev {
+
+constexpr int kFewWaves = 4;
+constexpr int kFewThreads = kFewWaves * kWave;
+constexpr int kFewStep = 32;  // tokens
+
+typedef uint32_t u32x4a __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// Four dwords that hold eight 16-bit elements: an operand of the product.
+struct Frag {
+  uint32_t w[4];
+};
+
+template <int IO>
+__device__ __forceinline__ f32x4 mfma16(const Frag &a, const Frag &b, f32x4 c) {
+  u32x4a x, y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = a.w[i];
+    y[i] = b.w[i];
+  }
+  if constexpr (IO == KVX_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
+                                                   __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x),
+                                                  __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+
+// Two f32 to two 16-bit elements, to nearest even.
+template <int IO>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  if constexpr (IO == KVX_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+
+// Two FP8 codes (a halfword of w) as two 16-bit elements: exact, every code of
+// both formats is a bf16 and an f16 value.
+template <int IO, int C>
+__device__ __forceinline__ uint32_t widen(uint32_t w, bool hi) {
+  if constexpr (IO == KVX_DTYPE_BF16) {
+    if constexpr (C == KVX_DTYPE_F8_E5M2)
+      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false));
+    else
+      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+  } else {
+    if constexpr (C == KVX_DTYPE_F8_E5M2)
+      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, false));
+    else
+      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  }
+}
+
+// An element of w that is NaN or infinite.
+template <int C>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  if constexpr (C == KVX_DTYPE_BF16) return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+  else if constexpr (C == KVX_DTYPE_F16) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+  else if constexpr (C == KVX_DTYPE_F8_E4M3)
+    return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  else return ((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u;
+}
+
+template <int IO>
+constexpr uint32_t kOne = IO == KVX_DTYPE_BF16 ? 0x3F80u : 0x3C00u;
+template <int IO>
+constexpr uint32_t kInf = IO == KVX_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+
+// acc + v w where v holds NaN or infinities that must not reach, as 0 * v, a
+// row whose weight is 0: the finite values as ever, and three products of
+// zeros and ones that say which rows meet an infinity of either sign or NaN
+// with a weight.
+template <int IO>
+__device__ __forceinline__ f32x4 guarded(const Frag &v, const Frag &w, f32x4 acc) {
+  Frag one, fine, met[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    one.w[i] = (w.w[i] & 0x7FFFu ? kOne<IO> : 0u) | (w.w[i] & 0x7FFF0000u ? kOne<IO> << 16 : 0u);
+    fine.w[i] = met[0].w[i] = met[1].w[i] = met[2].w[i] = 0;
+#pragma unroll
+    for (int half = 0; half < 32; half += 16) {
+      const uint32_t e = (v.w[i] >> half) & 0xFFFFu, size = e & 0x7FFFu;
+      const int kind = size > kInf<IO> ? 2 : (int)(e >> 15);
+      if (size < kInf<IO>) fine.w[i] |= e << half;
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (size >= kInf<IO> && kind == k) met[k].w[i] |= kOne<IO> << half;
+    }
+  }
+  const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
+  const f32x4 plus = mfma16<IO>(met[0], one, zero), minus = mfma16<IO>(met[1], one, zero),
+              nan = mfma16<IO>(met[2], one, zero);
+  acc = mfma16<IO>(fine, w, acc);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    acc[i] += (plus[i] > 0.0f ? INFINITY : 0.0f) + (minus[i] > 0.0f ? -INFINITY : 0.0f) +
+              (nan[i] > 0.0f ? NAN : 0.0f);
+  return acc;
+}
+
+// scale * q.k in units of log2, the scale of an FP8 key included in the
+// arguments; tanh(y) = 1 - 2 / (1 + e^2y).
+__device__ __forceinline__ float capped(const AttentionArgs &a, float x) {
+  const float e = __builtin_amdgcn_exp2f(x * a.cap_in * (2.0f * kLog2e));
+  return a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// Another lane's value; `at` = 4 * lane, so that constants added to it become
+// the instruction's offset.
+__device__ __forceinline__ uint32_t from_lane(uint32_t x, int at) {
+  return (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)x);
+}
+__device__ __forceinline__ float from_lane(float x, int at) {
+  return bits_f32(from_lane(f32_bits(x), at));
+}
+__device__ __forceinline__ uint64_t from_lane(uint64_t x, int at) {
+  return from_lane((uint32_t)x, at) | (uint64_t)from_lane((uint32_t)(x >> 32), at) << 32;
+}
+
+// Streaming load of B bytes of global memory (an address that went through
+// another lane is not known to be global).
+template <int B>
+__device__ __forceinline__ Raw<B> stream_load(uint64_t at) {
+  Raw<B> r;
+  if constexpr (B == 4) {
+    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<
+        const __attribute__((address_space(1))) uint32_t *>(at));
+  } else if constexpr (B == 8) {
+    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<
+        const __attribute__((address_space(1))) u32x2 *>(at));
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
+    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<
+        const __attribute__((address_space(1))) u32x4 *>(at));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = v[i];
+  }
+  return r;
+}
+
+// Token e of a lane's eight in a step, from its group's first.
+__device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12 + e; }
+
+// IO: type of queries and of the products; C: the cache's type; DP: head_dim
+// rounded up to 64, 128 or 256; VT: values with the token axis innermost;
+// INDEXED: scales by block.
+template <int IO, int C, int DP, bool VT, bool INDEXED>
+__global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_kernel(AttentionArgs a) {
+  constexpr bool kFp8 = C != IO;
+  constexpr int E = kFp8 ? 1 : 2;
+  constexpr int KC = DP / 32;          // products of a half step's logits
+  constexpr int KL = DP * E / 64;      // 16-byte key loads of a token and lane group
+  constexpr int NV = DP / 16;          // products of a step's sums; elements a lane loads
+  constexpr int VB = NV * E;           // bytes of them
+  constexpr int VW = VB / 4;           // dwords (VT: of four tokens)
+  __shared__ float sums[2][kRowTile][DP + 4];
+  __shared__ float states[kFewWaves][2][kRowTile];
+
+  const int hh = a.heads * a.head_tiles;
+  uint32_t id = blockIdx.x;
+  const int y = (int)(id % (uint32_t)hh);
+  id /= (uint32_t)hh;
+  const int z = (int)(id % (uint32_t)a.splits);
+  QueryTile t;
+  if (!find_tile(a, (int)(id / (uint32_t)a.splits), &t)) return;
+  const int lane = (int)(threadIdx.x % kWave);
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  const int c = lane % 16, g = lane / 16;
+  const int kvh = y / a.head_tiles;
+  const int head0 = (y - kvh * a.head_tiles) * a.tile_heads;
+  const int nheads = min(a.tile_heads, a.group - head0);
+  const int D = a.head_dim;
+
+  // This lane's row.
+  const int tok = c / a.tile_heads, h = c - tok * a.tile_heads;
+  const bool row = tok < t.count && h < nheads;
+  const int qh = kvh * a.group + head0 + h;
+  int rlo = 0, rhi = 0;
+  if (row) row_range(a, t, t.first + tok, &rlo, &rhi);
+  int lo, hi, first_hi, last_lo, from, to;
+  row_range(a, t, t.first, &lo, &first_hi);
+  row_range(a, t, t.first + t.count - 1, &last_lo, &hi);
+  split_range(a, lo, hi, z, &from, &to);
+  if (a.splits > 1 && from >= to) {  // nothing for this split: say so
+    if (wave == 0 && g == 0 && row) {
+      const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
+      a.part_ml[2 * at] = -INFINITY;
+      a.part_ml[2 * at + 1] = 0.0f;
+    }
+    return;
+  }
+
+  Frag q[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    // FP8: two products share a 16-byte load of 16 elements
+    const int d = kFp8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+    Raw<16> r{};
+    if (row && d < D)
+      r = ld<16>(a.q + (t.begin + t.first + tok) * a.q_tok + (int64_t)qh * a.q_head + 2 * d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[i].w[j] = r.w[j];
+  }
+
+  // Offsets of the lane's pieces from a token's row; a piece past the head's
+  // end is its first one (a key's counts as zero below, a value's sum is not
+  // stored).
+  int32_t koff[KL];
+#pragma unroll
+  for (int i = 0; i < KL; ++i) {
+    const int d0 = (i * 64 + g * 16) / E, d = d0 < D ? d0 : 0;
+    koff[i] = (d / a.gk.pack) * (int32_t)a.gk.s_piece + (d % a.gk.pack) * E;
+  }
+  constexpr int VL = VT ? NV : (VB + 15) / 16;  // value loads a token (VT: four tokens)
+  constexpr int VLB = VT ? 4 * E : VB / VL;      // bytes of one
+  int32_t voff[VL];
+#pragma unroll
+  for (int i = 0; i < VL; ++i) {
+    const int d0 = VT ? 16 * i + c : c * NV + i * (VLB / E), d = d0 < D ? d0 : 0;
+    voff[i] = (d / a.gv.pack) * (int32_t)a.gv.s_piece + (d % a.gv.pack) * (int32_t)a.gv.s_inner;
+  }
+  const int64_t khead = kvh * a.gk.s_head, vhead = kvh * a.gv.s_head;
+  float ks = 1.0f, vs = 1.0f;
+  if constexpr (kFp8 && !INDEXED) {
+    ks = scale_of(a.ks, 0, kvh);
+    vs = scale_of(a.vs, 0, kvh);
+  }
+
+  const float scale = a.scale_log2 * ks;
+  float m = -INFINITY, l = 0.0f, vref = 0.0f;
+  f32x4 acc[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  // Four tokens of a lane group lie in one block, so that their rows follow
+  // from the first's; RAGGED tables name every token's block.
+  const bool quads = VT || (a.block_size % 4 == 0 && a.format != KVX_BLOCK_TABLE_RAGGED);
+
+  struct Step {
+    uint64_t k, v;      // rows of token `lane` (lanes 0 .. 31)
+    uint32_t there;     // bit per token that some row may see
+    bool some;          // k and v can be read
+    float ks, vs;
+  };
+  auto resolve = [&](int base) -> Step {
+    Step s{0, 0, 0, false, 1.0f, 1.0f};
+    TokenRows r{nullptr, nullptr, 0};
+    const int at = base + lane;
+    const bool held = lane < kFewStep && at < to && token_rows(a, t.seq, at, &r);
+    if (held) {
+      s.k = reinterpret_cast<uint64_t>(r.k + khead);
+      s.v = reinterpret_cast<uint64_t>(r.v + vhead);
+      if constexpr (INDEXED) {
+        s.ks = scale_of(a.ks, r.block, kvh);
+        s.vs = scale_of(a.vs, r.block, kvh);
+      }
+    }
+    const uint64_t all = __ballot(held);
+    s.some = all != 0;
+    if (s.some && all != 0xFFFFFFFFull) {
+      // Tokens that are not there read another's rows, so that loads need no
+      // conditions.
+      const int first = 4 * __builtin_ctzll(all);
+      const uint64_t k = from_lane(s.k, first), v = from_lane(s.v, first);
+      if (!held) {
+        s.k = k;
+        s.v = v;
+      }
+    }
+    // Tokens in front of a window are of the block, but nobody's: they may hold
+    // anything.
+    s.there = (uint32_t)__ballot(held && at >= lo);
+    return s;
+  };
+  uint32_t kw[2][KL][4];
+  auto load_keys = [&](const Step &s) {
+    if (!s.some) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const uint64_t p = from_lane(s.k, 4 * c + 64 * b);
+#pragma unroll
+      for (int i = 0; i < KL; ++i) {
+        const Raw<16> r = stream_load<16>(p + koff[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kw[b][i][j] = r.w[j];
+      }
+    }
+  };
+  // Rows: [token e][dword]; VT: [half b][element j][dword].
+  uint32_t vw[VT ? 2 * NV : 8][VT ? E : VW];
+  auto load_values = [&](const Step &s) {
+    if (!s.some) return;
+    if constexpr (VT) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint64_t p = from_lane(s.v, 16 * g + 64 * b);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const Raw<VLB> r = stream_load<VLB>(p + voff[j]);
+#pragma unroll
+          for (int w = 0; w < E; ++w) vw[b * NV + j][w] = r.w[w];
+        }
+      }
+    } else {
+      const bool steps = quads && s.there == 0xFFFFFFFFu;
+      uint64_t rows[8];
+      if (steps) {
+        rows[0] = from_lane(s.v, 16 * g);
+        rows[4] = from_lane(s.v, 16 * g + 64);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) {
+          rows[e] = rows[e - 1] + a.gv.s_off;
+          rows[4 + e] = rows[3 + e] + a.gv.s_off;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rows[e] = from_lane(s.v, 16 * g + 4 * place_of(e));
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint64_t p = rows[e];
+#pragma unroll
+        for (int i = 0; i < VL; ++i) {
+          const Raw<VLB> r = stream_load<VLB>(p + voff[i]);
+#pragma unroll
+          for (int w = 0; w < VLB / 4; ++w) vw[e][i * (VLB / 4) + w] = r.w[w];
+        }
+      }
+    }
+  };
+  // Values of tokens that are not there become 0: their slots hold anything.
+  auto clear_values = [&](uint32_t there) {
+    if constexpr (VT) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t have = (there >> (4 * g)) >> (16 * b);
+#pragma unroll
+        for (int w = 0; w < E; ++w) {
+          const uint32_t keep =
+              E == 2 ? ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
+                           ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u)
+                     : (have & 1 ? 0xFFu : 0u) | (have & 2 ? 0xFF00u : 0u) |
+                           (have & 4 ? 0xFF0000u : 0u) | (have & 8 ? 0xFF000000u : 0u);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) vw[b * NV + j][w] &= keep;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t keep = ((there >> (4 * g)) >> place_of(e)) & 1 ? ~0u : 0u;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vw[e][w] &= keep;
+      }
+    }
+  };
+
+  int base = from + wave * kFewStep;
+  constexpr int kStride = kFewWaves * kFewStep;
+  if (base < to) {
+    Step now = resolve(base);
+    load_keys(now);
+    load_values(now);
+    Step next = resolve(base + kStride);  // nothing there past `to`
+    for (;;) {
+      if (D != DP) {  // pieces past the head's end
+#pragma unroll
+        for (int i = 0; i < KL; ++i) {
+          const uint32_t keep = (i * 64 + g * 16) / E < D ? ~0u : 0u;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            kw[0][i][j] &= keep;
+            kw[1][i][j] &= keep;
+          }
+        }
+      }
+      // Logits: lane c has its row's tokens base + 16 b + 4 g + i.
+      f32x4 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < KC; ++i) {
+          Frag k;
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              k.w[w] = widen<IO, C>(kw[b][i / 2][2 * (i % 2) + w / 2], w % 2);
+          } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) k.w[w] = kw[b][i][w];
+          }
+          s[b] = mfma16<IO>(k, q[i], s[b]);
+        }
+      }
+      const bool more = base + kStride < to;
+      if (more) load_keys(next);
+
+      const bool whole = now.there == 0xFFFFFFFFu && base >= last_lo && base + kFewStep <= first_hi;
+      float x[8], p[8], top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = s[e / 4][e % 4];
+        if constexpr (INDEXED) x[e] *= from_lane(now.ks, 16 * g + 4 * place_of(e));
+      }
+      if (a.cap != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = capped(a, x[e] * ks);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= scale;
+      }
+      if (!whole) {
+        const uint32_t there = now.there >> (4 * g);
+        const int start = base + 4 * g;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int at = start + place_of(e);
+          const bool seen = ((there >> place_of(e)) & 1) & (at >= rlo) & (at < rhi);
+          x[e] = seen ? x[e] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);  // NaN does not move it
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fmaxf(top, m);
+      const float shift = top == -INFINITY ? 0.0f : top;
+      if (__any(top > m)) {
+        const float alpha = __builtin_amdgcn_exp2f(m - shift);
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[j] *= alpha;
+      }
+      m = top;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(x[e] - shift);
+        l += p[e];
+      }
+      if constexpr (INDEXED) {
+        // Values stay codes; weights carry the tokens' scales, relative to the
+        // largest so far, so that they stay in the type's range.
+        float mine = lane < kFewStep && ((now.there >> lane) & 1) ? fabsf(now.vs) : 0.0f;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
+        if (mine > vref) {
+          const float ratio = vref / mine;
+#pragma unroll
+          for (int j = 0; j < NV; ++j) acc[j] *= ratio;
+          vref = mine;
+        }
+        const float inv = vref > 0.0f ? 1.0f / vref : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          p[e] *= from_lane(now.vs, 16 * g + 4 * place_of(e)) * inv;
+      }
+      Frag w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w.w[i] = pair_of<IO>(p[2 * i], p[2 * i + 1]);
+
+      if (now.there != 0xFFFFFFFFu) clear_values(now.there);
+      uint32_t odd = 0;
+      if (!whole && t.count > 1) {  // a token may be there for some rows only
+#pragma unroll
+        for (int e = 0; e < (VT ? 2 * NV : 8); ++e)
+#pragma unroll
+          for (int i = 0; i < (VT ? E : VW); ++i) odd |= not_finite<C>(vw[e][i]);
+      }
+      // Values by element: v[j], token order of the weights.
+      auto by_element = [&](int d, Frag *v) {  // v[2 d] and v[2 d + 1]
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (VT) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int at = (i / 2) * NV + 2 * d + k;
+              v[k].w[i] = kFp8 ? widen<IO, C>(vw[at][0], i % 2) : vw[at][kFp8 ? 0 : i % 2];
+            }
+          } else {
+            uint32_t t0, t1;
+            if constexpr (kFp8) {
+              t0 = widen<IO, C>(vw[2 * i][d / 2], d % 2);
+              t1 = widen<IO, C>(vw[2 * i + 1][d / 2], d % 2);
+            } else {
+              t0 = vw[2 * i][d];
+              t1 = vw[2 * i + 1][d];
+            }
+            v[0].w[i] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+            v[1].w[i] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+          }
+        }
+      };
+      if (__any(odd != 0)) {
+#pragma unroll
+        for (int d = 0; d < NV / 2; ++d) {
+          Frag v[2];
+          by_element(d, v);
+          acc[2 * d] = guarded<IO>(v[0], w, acc[2 * d]);
+          acc[2 * d + 1] = guarded<IO>(v[1], w, acc[2 * d + 1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < NV / 2; ++d) {
+          Frag v[2];
+          by_element(d, v);
+          acc[2 * d] = mfma16<IO>(v[0], w, acc[2 * d]);
+          acc[2 * d + 1] = mfma16<IO>(v[1], w, acc[2 * d + 1]);
+        }
+      }
+      if (!more) break;
+      load_values(next);
+      now = next;
+      base += kStride;
+      next = resolve(base + kStride);
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if constexpr (INDEXED) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) acc[j] *= vref;
+  }
+
+  // Join the waves: every wave brings its sums to the common maximum, then two
+  // and two add up.
+  if (g == 0) {
+    states[wave][0][c] = m;
+    states[wave][1][c] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i) top = fmaxf(top, states[i][0][c]);
+  const float shift = top == -INFINITY ? 0.0f : top;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kFewWaves; ++i)
+    l += states[i][1][c] * __builtin_amdgcn_exp2f(states[i][0][c] - shift);
+  const float mine = __builtin_amdgcn_exp2f(m - shift);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) acc[j] *= mine;
+  // Element of the head that acc[j][i] is.
+  auto element = [&](int j, int i) { return VT ? 16 * j + 4 * g + i : NV * (4 * g + i) + j; };
+#pragma unroll
+  for (int half = kFewWaves / 2; half > 0; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[wave - half][c][element(j, i)] = acc[j][i];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] += sums[wave][c][element(j, i)];
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  // Through LDS once more, so that rows leave as whole lines.
+  const bool none = top == -INFINITY && l == 0.0f;
+  const float norm = a.splits > 1 ? vs : none ? 0.0f : vs / l;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      sums[0][c][element(j, i)] = a.splits == 1 && none ? 0.0f : acc[j][i] * norm;
+  const int64_t line = t.begin + t.first + tok;
+  if (row && g == 0) {
+    if (a.splits > 1) {
+      const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
+      a.part_ml[2 * at] = top;
+      a.part_ml[2 * at + 1] = l;
+    } else if (a.lse != nullptr) {
+      a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (top + log2f(l)) * kLn2;
+    }
+  }
+  wave_sync();
+  const int rows = t.count * a.tile_heads;
+  constexpr int kLanes = DP / 8;  // lanes of a row
+#pragma unroll
+  for (int r0 = 0; r0 < kRowTile; r0 += kWave / kLanes) {
+    const int r = r0 + lane / kLanes, d = (lane % kLanes) * 8;
+    const int rt = r / a.tile_heads, rh = r - rt * a.tile_heads;
+    if (r >= rows || rh >= nheads || d >= D) continue;
+    const int64_t out_row = t.begin + t.first + rt;
+    const int head = kvh * a.group + head0 + rh;
+    const float *x = &sums[0][r][d];
+    if (a.splits > 1) {
+      const int64_t at = part_index(a, t, t.first + rt, head) * a.splits + z;
+      float *o = a.part_o + at * D + d;
+      *reinterpret_cast<f32x4 *>(o) = f32x4{x[0], x[1], x[2], x[3]};
+      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      Raw<16> o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.w[i] = pack_pair<IO>(f32x2{x[2 * i], x[2 * i + 1]});
+      st<16>(a.out + out_row * a.o_tok + (int64_t)head * a.o_head + 2 * d, o);
+    }
+  }
+}
+
+template <int IO, int C>
+void launch_few(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s) {
+  const dim3 b((uint32_t)grid);
+  const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
+  auto go = [&](auto dp, auto vt_, auto indexed_) {
+    attention_few_kernel<IO, C, decltype(dp)::value, decltype(vt_)::value,
+                         decltype(indexed_)::value><<<b, kFewThreads, 0, s>>>(a);
+  };
+  auto by_dim = [&](auto vt_, auto indexed_) {
+    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_);
+    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_);
+    else go(std::integral_constant<int, 256>{}, vt_, indexed_);
+  };
+  auto by_scale = [&](auto vt_) {
+    if constexpr (C != IO) {
+      if (indexed) return by_dim(vt_, std::true_type{});
+    }
+    by_dim(vt_, std::false_type{});
+  };
+  if (vt) by_scale(std::true_type{});
+  else by_scale(std::false_type{});
+}
+
+}  // namespace dev
+}  // namespace kvx

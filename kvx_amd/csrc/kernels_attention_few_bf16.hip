@@ -1,0 +1,13 @@
+// Attention of few rows: BF16 queries over a BF16 cache.
+#include "kernels_attention_few.h"
+
+namespace kvx {
+namespace dev {
+
+void run_attention_few_bf16(const AttentionArgs &a, bool vt, int64_t grid,
+                            hipStream_t s) {
+  launch_few<KVX_DTYPE_BF16, KVX_DTYPE_BF16>(a, vt, grid, s);
+}
+
+}  // namespace dev
+}  // namespace kvx

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(AttentionA
   int lo, hi, x0, x1, from, to;
   row_range(a, t, t.first, &lo, &x0);
   row_range(a, t, t.first + t.count - 1, &x1, &hi);
-  split_range(lo, hi, a.splits, z, &from, &to);
+  split_range(a, lo, hi, z, &from, &to);
   __syncthreads();
 
   float m[kRowTile], l[kRowTile], acc[kRowTile][DJ];
