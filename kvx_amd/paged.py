@@ -238,6 +238,15 @@ def _scale_args(scale) -> tuple:
     return scale, -1
 
 
+def _table_args(table) -> tuple:
+    """(table, indptr, primary, secondary, bytes_per_block) of a block table."""
+    if isinstance(table, RaggedTable):
+        return table.indices, table.indptr, None, None, 0
+    if isinstance(table, OffsetsTable):
+        return table.offsets, None, table.primary, table.secondary, table.bytes_per_block
+    return table, None, None, None, 0
+
+
 def build_write(cache: PagedCache, key: torch.Tensor, value: torch.Tensor,
                 slot_mapping: torch.Tensor, k_scale=None, v_scale=None) -> abi.WriteDesc:
     """kvx_write_desc_t for [T, H, D] key/value rows and [T] slots.  FP8
@@ -411,13 +420,7 @@ def gather_kv(cache: PagedCache, key_out: torch.Tensor, value_out: torch.Tensor,
     host = _host()
     if (host and type(cache) is PagedCache and pool_blocks is None
             and (entry != "abi" or k_scale is None)):
-        if isinstance(block_table, RaggedTable):
-            table = (block_table.indices, block_table.indptr, None, None, 0)
-        elif isinstance(block_table, OffsetsTable):
-            table = (block_table.offsets, None, block_table.primary, block_table.secondary,
-                     block_table.bytes_per_block)
-        else:
-            table = (block_table, None, None, None, 0)
+        table = _table_args(block_table)
         name = ("kvx_gather_kv" if entry == "abi" else "kvx_launch_gather_kv"
                 if k_scale is None and v_scale is None else "kvx_launch_gather_kv_dequant")
         code = host.gather(
@@ -579,6 +582,17 @@ def rope_write_kv(cache: PagedCache, query: torch.Tensor | None, key: torch.Tens
     lib = abi.load()
     if query is not None and query_out is None:
         query_out = query
+    host = _host()
+    if host and type(cache) is PagedCache:
+        code = host.rope_write(
+            _address(lib, "kvx_launch_rope_write_kv"),
+            None if stream is None else _stream_handle(stream), *_cache_args(cache), query,
+            query_out if query is not None else None, key, value, positions, rope.inv_freq,
+            1 if rope.interleaved else 0, rope.magnitude, slot_mapping, *_scale_args(k_scale),
+            *_scale_args(v_scale))
+        if code is not None:
+            return _STATUS[code]
+    # what the native builder leaves to the descriptor helpers
     device = _on_one_gpu(cache.key_cache, value_cache=cache.value_cache, query=query, key=key,
                          value=value, positions=positions, inv_freq=rope.inv_freq,
                          slot_mapping=slot_mapping, query_out=query_out)
@@ -654,7 +668,18 @@ def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_t
     uint8 tensor of ``attention_workspace_size`` bytes, one for each call that
     may run at the same time; None allocates it.  kvx_launch_attention."""
     lib = abi.load()
-    table_tensors = {}
+    host = _host()
+    if host and type(cache) is PagedCache and pool_blocks is None:
+        code = host.attention(
+            _address(lib, "kvx_launch_attention"),
+            _address(lib, "kvx_attention_workspace_size"),
+            None if stream is None else _stream_handle(stream), *_cache_args(cache), query, out,
+            *_table_args(block_table), seq_lens, query_indptr, 1 if causal else 0,
+            query.shape[-1] ** -0.5 if scale is None else scale, window, softcap, lse,
+            max_seq_len, max_query_len, *_scale_args(k_scale), *_scale_args(v_scale), workspace)
+        if code is not None:
+            return _STATUS[code]
+    # what the native builder leaves to the descriptor helpers
     if isinstance(block_table, RaggedTable):
         table_tensors = {"indices": _indices("indices", block_table.indices),
                          "indptr": _indices("indptr", block_table.indptr)}
@@ -729,7 +754,14 @@ def copy_blocks(caches, pairs: torch.Tensor, *, stream=None) -> Status:
     Block-indexed FP8 scales are the caller's to copy.
     kvx_launch_copy_blocks."""
     lib = abi.load()
-    caches = list(caches)
+    caches = caches if isinstance(caches, list) else list(caches)
+    host = _host()
+    if host:
+        code = host.copy_blocks(_address(lib, "kvx_launch_copy_blocks"),
+                                None if stream is None else _stream_handle(stream), PagedCache,
+                                caches, pairs)
+        if code is not None:
+            return _STATUS[code]
     _indices("pairs", pairs)
     if pairs.dim() != 2 or pairs.shape[1] != 2:
         raise ValueError(f"pairs has shape {tuple(pairs.shape)}, not (n, 2)")
