@@ -8,7 +8,8 @@
 // same keys and values.  Tiles are numbered without knowing each sequence's
 // length on the host: sequence s starts at tile begin(s) / tile_tokens + s,
 // begin(s) its first row.  That leaves every sequence room for its
-// ceil(n / tile_tokens) tiles, at most one of them unused.
+// ceil(n / tile_tokens) tiles, at most one of them unused.  A kernel that takes
+// only sequences of a few rows gives each sequence the same number of tiles.
 //
 // Splits.  Where the tiles alone do not fill the machine, a tile's tokens are
 // divided among `splits` workgroups.  Each writes its unnormalised sum, its
@@ -26,7 +27,8 @@
 namespace kvx {
 namespace dev {
 
-constexpr int kRowTile = 16;  // rows of attention_rows_kernel's tile
+constexpr int kRowTile = 16;       // rows of a tile of the kernels for few rows
+constexpr int kManyRowTile = 128;  // and of the one for many
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -58,6 +60,7 @@ struct AttentionArgs {
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
   int32_t splits;
   int32_t split_steps;  // least steps of 64 tokens in a split
+  int32_t seq_tiles;  // tiles of every sequence; 0: numbered as above
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
   float *part_ml;     // the same without head_dim: (maximum, sum of weights)
@@ -110,11 +113,11 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
     t->begin = tile;
     t->rows = 1;
   } else {
-    const int lo = last_sequence(a.seqs, [&](int q) {
+    const int lo = a.seq_tiles > 0 ? tile / a.seq_tiles : last_sequence(a.seqs, [&](int q) {
       return query_begin(a, q) / a.tile_tokens + q <= (int64_t)tile;
     });
     const int64_t b = query_begin(a, lo), e = query_begin(a, lo + 1);
-    const int64_t j = tile - (b / a.tile_tokens + lo);
+    const int64_t j = tile - (a.seq_tiles > 0 ? (int64_t)lo * a.seq_tiles : b / a.tile_tokens + lo);
     const int64_t n = e > b ? e - b : 0;
     if (j < 0 || j * a.tile_tokens >= n || n < a.least_rows || n > a.most_rows) return false;
     t->seq = lo;
@@ -262,6 +265,12 @@ void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, 
 void run_attention_few_f16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
 void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
 void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_bf16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_bf16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_f16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_f16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+void run_attention_many_f16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
 
 }  // namespace dev
 }  // namespace kvx

@@ -92,46 +92,54 @@ void tile_rows(AttentionArgs *a, int rows) {
   a->tile_heads = a->group < rows ? a->group : rows;
   a->head_tiles = (a->group + a->tile_heads - 1) / a->tile_heads;
   a->tile_tokens = rows / a->tile_heads;
+  a->seq_tiles = 0;
   a->tiles = a->qptr != nullptr ? a->tokens / a->tile_tokens + a->seqs : a->seqs;
 }
 
 // Workgroups that share a tile's tokens, so that about `target` workgroups
 // run, each with at least `least` tokens of the longest sequence.
-void split_tokens(const AttentionPlan &p, AttentionArgs *a, int64_t target, int64_t least) {
-  const int64_t tiles =
-      a->qptr != nullptr ? (a->tokens + a->tile_tokens - 1) / a->tile_tokens : a->seqs;
+// `rows`: rows of partial sums per query head.
+void split_tokens(const AttentionPlan &p, AttentionArgs *a, int64_t target, int64_t least,
+                  int64_t rows) {
+  const int64_t tiles = a->qptr == nullptr ? a->seqs
+                        : a->seq_tiles > 0 ? (int64_t)a->seqs * a->seq_tiles
+                                           : (a->tokens + a->tile_tokens - 1) / a->tile_tokens;
   const int64_t units = tiles * a->heads * a->head_tiles;
   const int64_t tokens = longest(p);
   int64_t n = target / (units > 0 ? units : 1);
   if (n > tokens / least) n = tokens / least;
   // partial sums of at most 1 GiB
-  const int64_t each = (int64_t)a->tokens * a->heads * a->group * (a->head_dim + 2) * 4;
+  const int64_t each = rows * a->heads * a->group * (a->head_dim + 2) * 4;
   if (n * each > ((int64_t)1 << 30)) n = ((int64_t)1 << 30) / each;
   a->splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
   a->split_steps = (int)((tokens + 64 * (int64_t)a->splits - 1) / (64 * (int64_t)a->splits));
 }
 
-enum Kind { kRows, kFew };
+enum Kind { kRows, kFew, kMany };
 
+// Up to two launches: sequences of few and of many new tokens.
 struct Plan {
-  AttentionArgs a;
-  Kind kind;
+  struct Part {
+    AttentionArgs a;
+    Kind kind;
+  } part[2];
+  int parts;
   bool vt;
   uint64_t workspace;
 };
 
-// Four tokens of one element of a value lie together and aligned.
-bool tokens_inner(const AttentionPlan &p) {
+// `n` tokens of one element of a value lie together and aligned.
+bool tokens_inner(const AttentionPlan &p, int n) {
   const Geom &g = p.g.gv;
   const int e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
-  if (g.s_off != 1 || p.g.block_size % 4 != 0 || p.g.format == KVX_BLOCK_TABLE_RAGGED) return false;
+  if (g.s_off != 1 || p.g.block_size % n != 0 || p.g.format == KVX_BLOCK_TABLE_RAGGED) return false;
   uint64_t low = (uint64_t)((g.s_inner | g.s_head | g.s_piece) * e);
   if (p.g.format == KVX_BLOCK_TABLE_KV_OFFSETS)
     low |= (uint64_t)(uintptr_t)p.g.pool[0] | (uint64_t)(uintptr_t)p.g.pool[1] |
            (uint64_t)p.g.bytes_per_block;
   else
     low |= (uint64_t)(uintptr_t)p.g.src_v | (uint64_t)(g.s_block * e);
-  return low % (uint64_t)(4 * e) == 0;
+  return low % (uint64_t)(n * e) == 0;
 }
 
 // Offsets inside a head fit 32 bits.
@@ -142,27 +150,30 @@ bool near(const AttentionPlan &p, const Geom &g) {
          (pieces * g.s_piece + (int64_t)g.pack * g.s_inner) * e < most;
 }
 
-// The matrix-core kernels read queries and write outputs 8 elements at a time,
-// keys 16 bytes and values DP / 16 elements (or four tokens) at a time.
-bool matrix_cores(const AttentionPlan &p, bool *vt) {
+// The matrix-core kernels read queries and write outputs 8 elements at a time
+// and keys 16 bytes at a time.
+bool matrix_cores(const AttentionPlan &p) {
   const int D = p.g.head_dim, e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
   if (p.g.io_dtype == KVX_DTYPE_F32 || D % 8 != 0 || D > 256) return false;
   if (((p.q_tok | p.q_head | p.o_tok | p.o_head) % 8) != 0 ||
       (uintptr_t)p.query % 16 != 0 || (uintptr_t)p.out % 16 != 0)
     return false;
-  if (!near(p, p.g.gk) || !near(p, p.g.gv) || !chunks(p, p.g.gk, p.g.src_k, 16 / e)) return false;
-  const int per_lane = D <= 64 ? 4 : D <= 128 || e == 2 ? 8 : 16;
-  *vt = false;
-  if (chunks(p, p.g.gv, p.g.src_v, per_lane)) return true;
-  *vt = tokens_inner(p);
-  return *vt;
+  return near(p, p.g.gk) && near(p, p.g.gv) && chunks(p, p.g.gk, p.g.src_k, 16 / e);
+}
+
+// Values: DP / 16 elements at a time (few rows) or 16 bytes (many); with the
+// token axis innermost 4 tokens or 8 (vt).
+bool values_fit(const AttentionPlan &p, Kind kind, bool *vt) {
+  const int D = p.g.head_dim, e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
+  const int n = kind == kMany || D > 128 ? 16 / e : D <= 64 ? 4 : 8;
+  *vt = !chunks(p, p.g.gv, p.g.src_v, n);
+  return !*vt || tokens_inner(p, kind == kMany ? 8 : 4);
 }
 
 Plan make_plan(const AttentionPlan &p) {
   const GatherPlan &g = p.g;
   const int cs = dtype_size((kvx_dtype_t)g.cache_dtype), is = dtype_size((kvx_dtype_t)g.io_dtype);
-  Plan r{};
-  AttentionArgs &a = r.a;
+  AttentionArgs a{};
   a.k = static_cast<const char *>(g.src_k);
   a.v = static_cast<const char *>(g.src_v);
   a.pool[0] = g.pool[0];
@@ -207,18 +218,57 @@ Plan make_plan(const AttentionPlan &p) {
   a.cap_in = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
   a.least_rows = 0;
   a.most_rows = 0x7FFFFFFF;
-  tile_rows(&a, kRowTile);
-  r.kind = matrix_cores(p, &r.vt) ? kFew : kRows;
-  if (r.kind == kFew) {
-    split_tokens(p, &a, 3072, 512);
+  Plan r{};
+  auto add = [&](Kind kind, const AttentionArgs &x) -> AttentionArgs & {
+    r.part[r.parts].a = x;
+    r.part[r.parts].kind = kind;
+    return r.part[r.parts++].a;
+  };
+  const bool cores = matrix_cores(p);
+  // Sequences of at most `few` new tokens go to the kernel for few rows: about
+  // two of its tiles.  How many new tokens each has is known here where there
+  // is one sequence, one token each, or a hint that bounds all; else both
+  // kernels run and each takes its own.
+  const int few = a.group >= 2 * kRowTile ? 1 : 2 * kRowTile / a.group;
+  const bool all_few = a.qptr == nullptr || a.tokens <= few ||
+                       (p.max_query_len > 0 && p.max_query_len <= few);
+  const bool all_many = !all_few && a.seqs == 1;
+  const bool few_ok = cores && values_fit(p, kFew, &r.vt);
+  bool vt_many = false;
+  const bool many_ok = few_ok && values_fit(p, kMany, &vt_many) && vt_many == r.vt;
+  if (!few_ok) {
+    AttentionArgs &x = add(kRows, a);
+    tile_rows(&x, kRowTile);
+    x.chunk_k = chunks(p, g.gk, g.src_k, 4);
+    split_tokens(p, &x, 1024, 256, x.tokens);
+  } else if (all_few || !many_ok) {
+    AttentionArgs &x = add(kFew, a);
+    tile_rows(&x, kRowTile);
+    split_tokens(p, &x, 3072, 512, x.tokens);
   } else {
-    a.chunk_k = chunks(p, g.gk, g.src_k, 4);
-    split_tokens(p, &a, 1024, 256);
+    AttentionArgs &x = add(kMany, a);
+    tile_rows(&x, kManyRowTile);
+    if (!all_many) x.least_rows = few + 1;
+    split_tokens(p, &x, 512, 512, x.tokens);
+    if (!all_many) {
+      AttentionArgs &y = add(kFew, a);
+      tile_rows(&y, kRowTile);
+      y.most_rows = few;
+      y.part_rows = few;
+      y.seq_tiles = (few + y.tile_tokens - 1) / y.tile_tokens;
+      y.tiles = y.seqs * y.seq_tiles;
+      split_tokens(p, &y, 3072, 512, (int64_t)y.seqs * few);
+    }
   }
-  const int64_t parts = (int64_t)a.tokens * p.query_heads * a.splits;
-  r.workspace = a.splits > 1 ? (uint64_t)parts * (a.head_dim + 2) * 4 : 0;
-  a.part_o = static_cast<float *>(p.workspace);
-  a.part_ml = a.part_o + parts * a.head_dim;
+  for (int i = 0; i < r.parts; ++i) {
+    AttentionArgs &x = r.part[i].a;
+    if (x.splits == 1) continue;
+    const int64_t rows = x.part_rows > 0 ? (int64_t)x.seqs * x.part_rows : x.tokens;
+    const int64_t sums = rows * p.query_heads * x.splits;
+    x.part_o = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + r.workspace);
+    x.part_ml = x.part_o + sums * x.head_dim;
+    r.workspace += ((uint64_t)sums * (x.head_dim + 2) * 4 + 15) & ~(uint64_t)15;
+  }
   return r;
 }
 
@@ -229,26 +279,37 @@ void launch_join(const AttentionArgs &a, hipStream_t s) {
   attention_join_kernel<IO><<<dim3((uint32_t)((units + waves - 1) / waves)), kJoinThreads, 0, s>>>(a);
 }
 
-int64_t few_grid(const AttentionArgs &a) {
+int64_t workgroups(const AttentionArgs &a) {
   return (int64_t)a.tiles * a.splits * a.heads * a.head_tiles;
 }
 
 bool launchable(const Plan &p) {
-  const AttentionArgs &a = p.a;
-  if ((int64_t)a.tokens * a.heads * a.group * kWave > 0xFFFFFFFFll) return false;
-  if (p.kind == kFew) return few_grid(a) * 256 <= 0xFFFFFFFFll;
-  return (int64_t)a.heads * a.head_tiles <= 65535 && (int64_t)a.tiles * 256 <= 0xFFFFFFFFll;
+  for (int i = 0; i < p.parts; ++i) {
+    const AttentionArgs &a = p.part[i].a;
+    if ((int64_t)a.tokens * a.heads * a.group * kWave > 0xFFFFFFFFll) return false;
+    if (workgroups(a) * 256 > 0xFFFFFFFFll) return false;
+    if (p.part[i].kind == kRows && (int64_t)a.heads * a.head_tiles > 65535) return false;
+  }
+  return true;
 }
 
-void run_few(const Plan &p, int io, int cache, hipStream_t s) {
-  const int64_t grid = few_grid(p.a);
+void run_part(const Plan::Part &p, bool vt, int io, int cache, hipStream_t s) {
+  const int64_t grid = workgroups(p.a);
   const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
-  if (io == KVX_DTYPE_BF16)
+  if (p.kind == kRows)
+    run_attention_rows(p.a, io, cache, s);
+  else if (p.kind == kFew && io == KVX_DTYPE_BF16)
     (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
-                                           : run_attention_few_bf16)(p.a, p.vt, grid, s);
-  else
+                                           : run_attention_few_bf16)(p.a, vt, grid, s);
+  else if (p.kind == kFew)
     (e4 ? run_attention_few_f16_e4m3 : e5 ? run_attention_few_f16_e5m2
-                                          : run_attention_few_f16)(p.a, p.vt, grid, s);
+                                          : run_attention_few_f16)(p.a, vt, grid, s);
+  else if (io == KVX_DTYPE_BF16)
+    (e4 ? run_attention_many_bf16_e4m3 : e5 ? run_attention_many_bf16_e5m2
+                                            : run_attention_many_bf16)(p.a, vt, grid, s);
+  else
+    (e4 ? run_attention_many_f16_e4m3 : e5 ? run_attention_many_f16_e5m2
+                                           : run_attention_many_f16)(p.a, vt, grid, s);
 }
 
 }  // namespace
@@ -262,12 +323,13 @@ kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
   const Plan plan = make_plan(p);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!launchable(plan)) return KVX_STATUS_UNSUPPORTED;
-  if (plan.kind == kFew) run_few(plan, p.g.io_dtype, p.g.cache_dtype, s);
-  else run_attention_rows(plan.a, p.g.io_dtype, p.g.cache_dtype, s);
-  if (plan.a.splits > 1) {
-    if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(plan.a, s);
-    else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(plan.a, s);
-    else launch_join<KVX_DTYPE_BF16>(plan.a, s);
+  for (int i = 0; i < plan.parts; ++i) {
+    run_part(plan.part[i], plan.vt, p.g.io_dtype, p.g.cache_dtype, s);
+    const AttentionArgs &a = plan.part[i].a;
+    if (a.splits == 1) continue;
+    if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(a, s);
+    else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(a, s);
+    else launch_join<KVX_DTYPE_BF16>(a, s);
   }
   return hipGetLastError() == hipSuccess ? KVX_STATUS_OK : KVX_STATUS_INTERNAL_ERROR;
 }

@@ -30,7 +30,7 @@
 // relative, as the output is rounded), their sum is not.
 #pragma once
 
-#include "attention.h"
+#include "attention_mfma.h"
 
 namespace kvx {
 namespace dev {
@@ -38,150 +38,6 @@ namespace dev {
 constexpr int kFewWaves = 4;
 constexpr int kFewThreads = kFewWaves * kWave;
 constexpr int kFewStep = 32;  // tokens
-
-typedef uint32_t u32x4a __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-// Four dwords that hold eight 16-bit elements: an operand of the product.
-struct Frag {
-  uint32_t w[4];
-};
-
-template <int IO>
-__device__ __forceinline__ f32x4 mfma16(const Frag &a, const Frag &b, f32x4 c) {
-  u32x4a x, y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[i] = a.w[i];
-    y[i] = b.w[i];
-  }
-  if constexpr (IO == KVX_DTYPE_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
-                                                   __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x),
-                                                  __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
-}
-
-// Two f32 to two 16-bit elements, to nearest even.
-template <int IO>
-__device__ __forceinline__ uint32_t pair_of(float a, float b) {
-  if constexpr (IO == KVX_DTYPE_BF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-}
-
-// Two FP8 codes (a halfword of w) as two 16-bit elements: exact, every code of
-// both formats is a bf16 and an f16 value.
-template <int IO, int C>
-__device__ __forceinline__ uint32_t widen(uint32_t w, bool hi) {
-  if constexpr (IO == KVX_DTYPE_BF16) {
-    if constexpr (C == KVX_DTYPE_F8_E5M2)
-      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, 1.0f, false));
-    else
-      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-  } else {
-    if constexpr (C == KVX_DTYPE_F8_E5M2)
-      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_bf8(w, 1.0f, false));
-    else
-      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))
-                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
-  }
-}
-
-// An element of w that is NaN or infinite.
-template <int C>
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  if constexpr (C == KVX_DTYPE_BF16) return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-  else if constexpr (C == KVX_DTYPE_F16) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-  else if constexpr (C == KVX_DTYPE_F8_E4M3)
-    return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-  else return ((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u;
-}
-
-template <int IO>
-constexpr uint32_t kOne = IO == KVX_DTYPE_BF16 ? 0x3F80u : 0x3C00u;
-template <int IO>
-constexpr uint32_t kInf = IO == KVX_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
-
-// acc + v w where v holds NaN or infinities that must not reach, as 0 * v, a
-// row whose weight is 0: the finite values as ever, and three products of
-// zeros and ones that say which rows meet an infinity of either sign or NaN
-// with a weight.
-template <int IO>
-__device__ __forceinline__ f32x4 guarded(const Frag &v, const Frag &w, f32x4 acc) {
-  Frag one, fine, met[3];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    one.w[i] = (w.w[i] & 0x7FFFu ? kOne<IO> : 0u) | (w.w[i] & 0x7FFF0000u ? kOne<IO> << 16 : 0u);
-    fine.w[i] = met[0].w[i] = met[1].w[i] = met[2].w[i] = 0;
-#pragma unroll
-    for (int half = 0; half < 32; half += 16) {
-      const uint32_t e = (v.w[i] >> half) & 0xFFFFu, size = e & 0x7FFFu;
-      const int kind = size > kInf<IO> ? 2 : (int)(e >> 15);
-      if (size < kInf<IO>) fine.w[i] |= e << half;
-#pragma unroll
-      for (int k = 0; k < 3; ++k)
-        if (size >= kInf<IO> && kind == k) met[k].w[i] |= kOne<IO> << half;
-    }
-  }
-  const f32x4 zero{0.0f, 0.0f, 0.0f, 0.0f};
-  const f32x4 plus = mfma16<IO>(met[0], one, zero), minus = mfma16<IO>(met[1], one, zero),
-              nan = mfma16<IO>(met[2], one, zero);
-  acc = mfma16<IO>(fine, w, acc);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    acc[i] += (plus[i] > 0.0f ? INFINITY : 0.0f) + (minus[i] > 0.0f ? -INFINITY : 0.0f) +
-              (nan[i] > 0.0f ? NAN : 0.0f);
-  return acc;
-}
-
-// scale * q.k in units of log2, the scale of an FP8 key included in the
-// arguments; tanh(y) = 1 - 2 / (1 + e^2y).
-__device__ __forceinline__ float capped(const AttentionArgs &a, float x) {
-  const float e = __builtin_amdgcn_exp2f(x * a.cap_in * (2.0f * kLog2e));
-  return a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + e);
-}
-
-// Another lane's value; `at` = 4 * lane, so that constants added to it become
-// the instruction's offset.
-__device__ __forceinline__ uint32_t from_lane(uint32_t x, int at) {
-  return (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)x);
-}
-__device__ __forceinline__ float from_lane(float x, int at) {
-  return bits_f32(from_lane(f32_bits(x), at));
-}
-__device__ __forceinline__ uint64_t from_lane(uint64_t x, int at) {
-  return from_lane((uint32_t)x, at) | (uint64_t)from_lane((uint32_t)(x >> 32), at) << 32;
-}
-
-// Streaming load of B bytes of global memory (an address that went through
-// another lane is not known to be global).
-template <int B>
-__device__ __forceinline__ Raw<B> stream_load(uint64_t at) {
-  Raw<B> r;
-  if constexpr (B == 4) {
-    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) uint32_t *>(at));
-  } else if constexpr (B == 8) {
-    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) u32x2 *>(at));
-    r.w[0] = v[0];
-    r.w[1] = v[1];
-  } else {
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) u32x4 *>(at));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = v[i];
-  }
-  return r;
-}
 
 // Token e of a lane's eight in a step, from its group's first.
 __device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12 + e; }
@@ -271,7 +127,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     vs = scale_of(a.vs, 0, kvh);
   }
 
-  const float scale = a.scale_log2 * ks;
+  const float scale = positive_scale<IO>(a, ks, q);
   float m = -INFINITY, l = 0.0f, vref = 0.0f;
   f32x4 acc[NV];
 #pragma unroll
@@ -435,7 +291,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 #pragma unroll
             for (int w = 0; w < 4; ++w) k.w[w] = kw[b][i][w];
           }
-          s[b] = mfma16<IO>(k, q[i], s[b]);
+          s[b] = mma<IO>(k, q[i], s[b]);
         }
       }
       const bool more = base + kStride < to;
@@ -451,9 +307,6 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       if (a.cap != 0.0f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = capped(a, x[e] * ks);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= scale;
       }
       if (!whole) {
         const uint32_t there = now.there >> (4 * g);
@@ -468,7 +321,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);  // NaN does not move it
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
       top = fmaxf(top, m);
       const float shift = top == -INFINITY ? 0.0f : top;
       if (__any(top > m)) {
@@ -480,7 +333,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       m = top;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(x[e] - shift);
+        p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], scale, -shift));
         l += p[e];
       }
       if constexpr (INDEXED) {
@@ -550,8 +403,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         for (int d = 0; d < NV / 2; ++d) {
           Frag v[2];
           by_element(d, v);
-          acc[2 * d] = mfma16<IO>(v[0], w, acc[2 * d]);
-          acc[2 * d + 1] = mfma16<IO>(v[1], w, acc[2 * d + 1]);
+          acc[2 * d] = mma<IO>(v[0], w, acc[2 * d]);
+          acc[2 * d + 1] = mma<IO>(v[1], w, acc[2 * d + 1]);
         }
       }
       if (!more) break;

@@ -1,0 +1,516 @@
+// Attention of many rows per kv head (prefill chunks) on the matrix cores.
+//
+// 4 * D operations for every (row, token) pair; rows of a tile share its keys
+// and values, so that 128 rows make it compute-bound: the matrix cores, and
+// beside them the vector unit, which owes every pair a maximum, a
+// multiply-add, an exp2, a sum and half a conversion.
+//
+// Four waves with 32 rows each share steps of 64 tokens through LDS, two
+// buffers, loaded one step ahead through registers (where FP8 codes become
+// 16-bit elements, and values of slots without a token zeros).
+//
+// v_mfma_f32_32x32x16: lane l = 32 h + c holds A[row c][8 h .. 8 h + 7],
+// B[8 h ..][column c], D[rows 8 (i / 4) + 4 h + i % 4][column c], i < 16.
+//
+//   S^T = K Q^T   lane c has row c of its wave's queries (held in registers)
+//                 and half of the step's tokens: maximum and sum are a chain in
+//                 the lane and one exchange with lane c ^ 32.
+//   O^T = V^T P^T a lane's weights are the B operand as they stand: the sum's
+//                 tokens may come in any order, and A takes them in that one,
+//                 through ds_read_b64_tr_b16, which transposes 4 tokens by 16
+//                 elements (values with the token axis innermost are kept as
+//                 they are and read plainly).
+//   The sums of a row are a lane's own, so rescaling them is one multiplication
+//   each; it is put off until a maximum has grown by more than 8 (weights then
+//   reach 2^8, which changes neither their relative rounding nor the F32 sums).
+//
+// LDS rows are not padded; the 16-byte chunks of a row are permuted by the
+// token's number, so that the 8 lanes that read one element range of 8 keys
+// (and the 16 that transpose 4 values) meet all banks.
+#pragma once
+
+#include "attention_mfma.h"
+
+namespace kvx {
+namespace dev {
+
+constexpr int kManyWaves = 4;
+constexpr int kManyThreads = kManyWaves * kWave;
+static_assert(kManyRowTile == 32 * kManyWaves, "32 rows a wave");
+constexpr int kManyStep = 64;
+
+template <int DP>
+constexpr int many_buffers() {
+  return DP <= 128 ? 2 : 1;
+}
+
+template <int DP, bool INDEXED>
+constexpr size_t many_lds() {
+  return (size_t)many_buffers<DP>() *
+         (2 * kManyStep * DP * 2 + (INDEXED ? 2 * kManyStep * 4 : 0));
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ u32x2 lds_transposed(const char *p) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (__attribute__((address_space(3))) s16x4 *)(p)));
+}
+
+template <int B>
+__device__ __forceinline__ Raw<B> plain_load(uint64_t at) {
+  Raw<B> r;
+  if constexpr (B == 8) {
+    const u32x2 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x2 *>(at);
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  } else {
+    const u32x4 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>(at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = v[i];
+  }
+  return r;
+}
+
+template <int IO, int C, int DP, bool VT, bool INDEXED>
+__global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : 2)
+attention_many_kernel(AttentionArgs a) {
+  constexpr bool kFp8 = C != IO;
+  constexpr int E = kFp8 ? 1 : 2;
+  constexpr int KC = DP / 16;                   // products of 32 tokens' logits
+  constexpr int NJ = DP / 32;                   // blocks of elements of the sums
+  constexpr int ROW = DP * 2;                   // bytes of a row in LDS
+  constexpr int CPR = DP * E / 16;              // 16-byte chunks of a cached row
+  constexpr int NL = kManyStep * CPR / kManyThreads;  // of them a thread loads
+  constexpr int NB = many_buffers<DP>();
+  constexpr int NVL = VT ? DP / 32 : NL;        // value loads (VT: 8 tokens of an element)
+  constexpr int VLB = VT ? 8 * E : 16;
+  constexpr int TENSOR = kManyStep * ROW;
+  extern __shared__ __align__(16) char lds[];
+  char *const kbuf = lds, *const vbuf = lds + NB * TENSOR;
+  float *const scales = reinterpret_cast<float *>(lds + 2 * NB * TENSOR);  // [buffer][k, v][64]
+
+  // The last tiles of a causal chunk see most tokens: they start first.
+  const int hh = a.heads * a.head_tiles;
+  uint32_t id = blockIdx.x;
+  const int y = (int)(id % (uint32_t)hh);
+  id /= (uint32_t)hh;
+  const int z = (int)(id % (uint32_t)a.splits);
+  QueryTile t;
+  if (!find_tile(a, a.tiles - 1 - (int)(id / (uint32_t)a.splits), &t)) return;
+  const int tid = (int)threadIdx.x, lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int c = lane % 32, h = lane / 32;
+  const int kvh = y / a.head_tiles;
+  const int head0 = (y - kvh * a.head_tiles) * a.tile_heads;
+  const int nheads = min(a.tile_heads, a.group - head0);
+  const int D = a.head_dim;
+
+  // This lane's row.
+  const int r = 32 * wave + c;
+  const int tok = r / a.tile_heads, rh = r - tok * a.tile_heads;
+  const bool row = tok < t.count && rh < nheads;
+  const int qh = kvh * a.group + head0 + rh;
+  int rlo = 0, rhi = 0;
+  if (row) row_range(a, t, t.first + tok, &rlo, &rhi);
+  int lo, hi, from, to, skip;
+  row_range(a, t, t.first, &lo, &skip);
+  row_range(a, t, t.first + t.count - 1, &skip, &hi);
+  split_range(a, lo, hi, z, &from, &to);
+  // The wave's rows see all of [all_lo, all_hi) and nothing outside [any_lo, any_hi).
+  const int tok0 = 32 * wave / a.tile_heads;
+  const int tok1 = min((32 * wave + 31) / a.tile_heads, t.count - 1);
+  int any_lo = 0, any_hi = 0, all_lo = 0, all_hi = 0;
+  if (tok0 < t.count) {
+    row_range(a, t, t.first + tok0, &any_lo, &all_hi);
+    row_range(a, t, t.first + tok1, &all_lo, &any_hi);
+  }
+
+  Frag q[KC];
+#pragma unroll
+  for (int i = 0; i < KC; ++i) {
+    const int d = 16 * i + 8 * h;
+    Raw<16> x{};
+    if (row && d < D)
+      x = ld<16>(a.q + (t.begin + t.first + tok) * a.q_tok + (int64_t)qh * a.q_head + 2 * d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[i].w[j] = x.w[j];
+  }
+
+  // What this thread loads of a step: chunk `chunk` of tokens tok_l + l * (256 /
+  // CPR); VT: tokens 8 (tid % 8) .. of elements tid / 8 + 32 l.
+  const int chunk = tid % CPR;
+  const int d0 = chunk * 16 / E;
+  const bool inside = d0 < D;
+  const int kd = inside ? d0 : 0;
+  const int32_t koff = (kd / a.gk.pack) * (int32_t)a.gk.s_piece + (kd % a.gk.pack) * E;
+  int32_t voff[VT ? NVL : 1];
+  if constexpr (VT) {
+#pragma unroll
+    for (int l = 0; l < NVL; ++l) {
+      const int e = tid / 8 + 32 * l, d = e < D ? e : 0;
+      voff[l] = (d / a.gv.pack) * (int32_t)a.gv.s_piece + (d % a.gv.pack) * (int32_t)a.gv.s_inner;
+    }
+  } else {
+    voff[0] = (kd / a.gv.pack) * (int32_t)a.gv.s_piece + (kd % a.gv.pack) * E;
+  }
+  const int64_t khead = kvh * a.gk.s_head, vhead = kvh * a.gv.s_head;
+  float ks = 1.0f, vs = 1.0f;
+  if constexpr (kFp8 && !INDEXED) {
+    ks = scale_of(a.ks, 0, kvh);
+    vs = scale_of(a.vs, 0, kvh);
+  }
+  const float scale = positive_scale<IO>(a, ks, q);
+
+  struct Step {
+    uint64_t k, v;  // rows of token `lane`
+    uint64_t there;
+    float ks, vs;
+    bool some;
+  };
+  auto resolve = [&](int base) -> Step {
+    Step s{0, 0, 0, 1.0f, 1.0f, false};
+    TokenRows x{nullptr, nullptr, 0};
+    const int at = base + lane;
+    const bool held = at < to && token_rows(a, t.seq, at, &x);
+    if (held) {
+      s.k = reinterpret_cast<uint64_t>(x.k + khead);
+      s.v = reinterpret_cast<uint64_t>(x.v + vhead);
+      if constexpr (INDEXED) {
+        s.ks = scale_of(a.ks, x.block, kvh);
+        s.vs = scale_of(a.vs, x.block, kvh);
+      }
+    }
+    const uint64_t all = __ballot(held);
+    s.some = all != 0;
+    if (s.some && all != ~0ull) {  // tokens that are not there read another's rows
+      const int first = 4 * __builtin_ctzll(all);
+      const uint64_t k = from_lane(s.k, first), v = from_lane(s.v, first);
+      if (!held) {
+        s.k = k;
+        s.v = v;
+      }
+    }
+    s.there = __ballot(held && at >= lo);  // slots in front of a window hold anything
+    return s;
+  };
+
+  Raw<16> kreg[NL];
+  Raw<VLB> vreg[NVL];
+  auto load = [&](const Step &s) {
+    if (!s.some) return;
+#pragma unroll
+    for (int l = 0; l < NL; ++l)
+      kreg[l] = plain_load<16>(from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)) + koff);
+    if constexpr (VT) {
+      const uint64_t p = from_lane(s.v, 32 * (tid % 8));
+#pragma unroll
+      for (int l = 0; l < NVL; ++l) vreg[l] = plain_load<VLB>(p + voff[l]);
+    } else {
+#pragma unroll
+      for (int l = 0; l < NL; ++l)
+        vreg[l] =
+            plain_load<16>(from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)) + voff[0]);
+    }
+  };
+  // A 16-byte chunk of a cached row as one (16-bit) or two (FP8) chunks in LDS;
+  // `swap` is XORed to their numbers.
+  auto put = [&](char *line, int swap, const Raw<16> &x) {
+    if constexpr (kFp8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u32x4 o;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) o[w] = widen<IO, C>(x.w[2 * i + w / 2], w % 2);
+        *reinterpret_cast<u32x4 *>(line + 16 * ((2 * chunk + i) ^ swap)) = o;
+      }
+    } else {
+      *reinterpret_cast<u32x4 *>(line + 16 * (chunk ^ swap)) = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+    }
+  };
+  auto store = [&](const Step &s, int buffer) {
+    char *kb = kbuf + buffer * TENSOR, *vb = vbuf + buffer * TENSOR;
+    const bool whole = s.there == ~0ull;
+#pragma unroll
+    for (int l = 0; l < NL; ++l) {
+      const int at = tid / CPR + l * (kManyThreads / CPR);
+      Raw<16> x = kreg[l];
+      if (!inside) x = Raw<16>{};
+      put(kb + at * ROW, at & 7, x);
+    }
+    if constexpr (VT) {
+      const uint32_t have = (uint32_t)(s.there >> (8 * (tid % 8))) & 0xFFu;
+#pragma unroll
+      for (int l = 0; l < NVL; ++l) {
+        const int e = tid / 8 + 32 * l;
+        u32x4 o;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (kFp8) o[w] = widen<IO, C>(vreg[l].w[w / 2], w % 2);
+          else o[w] = vreg[l].w[w];
+          if (!whole)
+            o[w] &= ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
+                    ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
+        }
+        *reinterpret_cast<u32x4 *>(vb + e * (kManyStep * 2) + 16 * ((tid % 8) ^ (e & 7))) = o;
+      }
+    } else {
+#pragma unroll
+      for (int l = 0; l < NL; ++l) {
+        const int at = tid / CPR + l * (kManyThreads / CPR);
+        Raw<16> x = vreg[l];
+        if (!whole && !((s.there >> at) & 1)) x = Raw<16>{};
+        put(vb + at * ROW, 2 * (at & 3), x);
+      }
+    }
+    if constexpr (INDEXED) {
+      if (wave == 0) {
+        scales[(2 * buffer) * kManyStep + lane] = s.ks;
+        scales[(2 * buffer + 1) * kManyStep + lane] = s.vs;
+      }
+    }
+  };
+
+  float m = -INFINITY, l = 0.0f, vref = 0.0f;
+  f32x16 acc[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j] = f32x16{};
+
+  auto step = [&](const Step &now, int base, int buffer) {
+    if (base >= any_hi || base + kManyStep <= any_lo || now.there == 0) return;
+    const char *kb = kbuf + buffer * TENSOR + c * ROW;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      s[b] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + b * 32 * ROW +
+                                                         16 * ((2 * i + h) ^ (c & 7)));
+        Frag k;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) k.w[w] = x[w];
+        s[b] = mma<IO>(k, q[i], s[b]);
+      }
+    }
+    const bool whole = now.there == ~0ull && base >= all_lo && base + kManyStep <= all_hi;
+    float top = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if constexpr (INDEXED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(
+              scales + 2 * buffer * kManyStep + 32 * b + 8 * i + 4 * h);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) s[b][4 * i + w] *= x[w];
+        }
+      }
+      if (a.cap != 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = capped(a, s[b][i] * ks);
+      }
+      if (!whole) {
+        const uint32_t there = (uint32_t)(now.there >> (32 * b)) >> (4 * h);
+        const int start = base + 32 * b + 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 8 * (i / 4) + i % 4;
+          const bool seen = ((there >> at) & 1) & (start + at >= rlo) & (start + at < rhi);
+          s[b][i] = seen ? s[b][i] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);  // NaN does not move it
+    }
+    top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+    if (__any(top > m + 8.0f)) {
+      const float now_m = fmaxf(top, m);
+      const float alpha = __builtin_amdgcn_exp2f(m - (now_m == -INFINITY ? 0.0f : now_m));
+      m = now_m;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= alpha;
+    }
+    const float shift = m == -INFINITY ? 0.0f : m;
+    float inv = 1.0f;
+    if constexpr (INDEXED) {
+      float mine = (now.there >> lane) & 1 ? fabsf(now.vs) : 0.0f;
+#pragma unroll
+      for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
+      if (mine > vref) {
+        const float ratio = vref / mine;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] *= ratio;
+        vref = mine;
+      }
+      inv = vref > 0.0f ? 1.0f / vref : 0.0f;
+    }
+    Frag w[4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float part = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[b][i] = __builtin_amdgcn_exp2f(fmaf(s[b][i], scale, -shift));
+        part += s[b][i];
+      }
+      l += part;
+      asm volatile("" : "+v"(l));  // summed here, not after the products: fewer live registers
+      if constexpr (INDEXED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(
+              scales + (2 * buffer + 1) * kManyStep + 32 * b + 8 * i + 4 * h);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[b][4 * i + k] *= x[k] * inv;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        w[2 * b + i / 4].w[i % 4] = pair_of<IO>(s[b][2 * i], s[b][2 * i + 1]);
+    }
+    const char *vb = vbuf + buffer * TENSOR;
+    // Values of 16 tokens (in the weights' order) of element 32 j + c.
+    auto values = [&](int kk, int j) -> Frag {
+      Frag f;
+      if constexpr (VT) {
+        const int e = 32 * j + c;
+        const char *line = vb + e * (kManyStep * 2) + 8 * h;
+        const u32x2 x = *reinterpret_cast<const u32x2 *>(line + 16 * ((2 * kk) ^ (e & 7)));
+        const u32x2 y = *reinterpret_cast<const u32x2 *>(line + 16 * ((2 * kk + 1) ^ (e & 7)));
+        f.w[0] = x[0];
+        f.w[1] = x[1];
+        f.w[2] = y[0];
+        f.w[3] = y[1];
+      } else {
+        const int i = lane % 16, token = 16 * kk + 4 * h + i / 4;
+        const int piece = (4 * j + 2 * ((lane / 16) % 2) + (i % 4) / 2) ^ (2 * (i / 4));
+        const char *p = vb + token * ROW + 16 * piece + 8 * (i % 2);
+        const u32x2 x = lds_transposed(p), y = lds_transposed(p + 8 * ROW);
+        f.w[0] = x[0];
+        f.w[1] = x[1];
+        f.w[2] = y[0];
+        f.w[3] = y[1];
+      }
+      return f;
+    };
+    if (whole) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] = mma<IO>(values(kk, j), w[kk], acc[j]);
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const Frag v = values(kk, j);
+          const uint32_t odd = not_finite<IO>(v.w[0]) | not_finite<IO>(v.w[1]) |
+                               not_finite<IO>(v.w[2]) | not_finite<IO>(v.w[3]);
+          if (__any(odd != 0)) acc[j] = guarded<IO>(v, w[kk], acc[j]);
+          else acc[j] = mma<IO>(v, w[kk], acc[j]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  };
+
+  if (from < to) {
+    Step now = resolve(from);
+    load(now);
+    Step next = resolve(from + kManyStep);  // nothing there past `to`
+    store(now, 0);
+    __syncthreads();
+    int buffer = 0;
+    for (int base = from;; base += kManyStep) {
+      const bool more = base + kManyStep < to;
+      Step after{};
+      if (more) {
+        load(next);
+        after = resolve(base + 2 * kManyStep);
+      }
+      step(now, base, buffer);
+      if (!more) break;
+      if constexpr (NB == 1) __syncthreads();
+      else buffer ^= 1;
+      store(next, buffer);
+      __syncthreads();
+      now = next;
+      next = after;
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if constexpr (INDEXED) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] *= vref;
+  }
+  if (!row) return;
+  const bool none = m == -INFINITY && l == 0.0f;
+  const int64_t line = t.begin + t.first + tok;
+  if (a.splits > 1) {
+    const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
+    if (h == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+    if (none) return;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * j + 8 * i + 4 * h;
+        if (d < D)
+          *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) =
+              f32x4{acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]} * vs;
+      }
+    return;
+  }
+  if (h == 0 && a.lse != nullptr)
+    a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+  const float norm = vs / l;
+  char *out = a.out + line * a.o_tok + (int64_t)qh * a.o_head;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * j + 8 * i + 4 * h;
+      if (d >= D) continue;
+      Raw<8> o;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const float x0 = none ? 0.0f : acc[j][4 * i + 2 * k] * norm;
+        const float x1 = none ? 0.0f : acc[j][4 * i + 2 * k + 1] * norm;
+        o.w[k] = pack_pair<IO>(f32x2{x0, x1});
+      }
+      st<8>(out + 2 * d, o);
+    }
+}
+
+template <int IO, int C>
+void launch_many(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s) {
+  const dim3 b((uint32_t)grid);
+  const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
+  auto go = [&](auto dp, auto vt_, auto indexed_) {
+    constexpr int kDim = decltype(dp)::value;
+    constexpr bool kIndexed = decltype(indexed_)::value;
+    attention_many_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed>
+        <<<b, kManyThreads, many_lds<kDim, kIndexed>(), s>>>(a);
+  };
+  auto by_dim = [&](auto vt_, auto indexed_) {
+    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_);
+    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_);
+    else go(std::integral_constant<int, 256>{}, vt_, indexed_);
+  };
+  auto by_scale = [&](auto vt_) {
+    if constexpr (C != IO) {
+      if (indexed) return by_dim(vt_, std::true_type{});
+    }
+    by_dim(vt_, std::false_type{});
+  };
+  if (vt) by_scale(std::true_type{});
+  else by_scale(std::false_type{});
+}
+
+}  // namespace dev
+}  // namespace kvx

@@ -1,0 +1,13 @@
+// Attention of many rows: BF16 queries over an E5M2 cache.
+#include "kernels_attention_many.h"
+
+namespace kvx {
+namespace dev {
+
+void run_attention_many_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid,
+                                  hipStream_t s) {
+  launch_many<KVX_DTYPE_BF16, KVX_DTYPE_F8_E5M2>(a, vt, grid, s);
+}
+
+}  // namespace dev
+}  // namespace kvx
