@@ -75,6 +75,7 @@ struct QueryTile {
   int32_t rows;    // the sequence's new tokens
   int64_t length;  // its cached tokens, as given
   int32_t usable;  // of those, the ones the table can hold
+  int64_t ragged;  // RAGGED: number of its first token
 };
 
 __device__ __forceinline__ int64_t index_at(const void *p, bool is64, int64_t i) {
@@ -128,8 +129,10 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
   }
   t->length = index_at(a.lens, a.lens64, t->seq);
   int64_t hold;
+  t->ragged = 0;
   if (a.format == KVX_BLOCK_TABLE_RAGGED) {
-    hold = index_at(a.indptr, a.indptr64, t->seq + 1) - index_at(a.indptr, a.indptr64, t->seq);
+    t->ragged = index_at(a.indptr, a.indptr64, t->seq);
+    hold = index_at(a.indptr, a.indptr64, t->seq + 1) - t->ragged;
     if (hold > 0x7FFF0000) hold = 0x7FFF0000;
   } else {
     hold = (int64_t)a.max_blocks * a.block_size;
@@ -166,27 +169,57 @@ __device__ __forceinline__ void split_range(const AttentionArgs &a, int lo, int 
   *to = (int)min((int64_t)start + (int64_t)(z + 1) * per * 64, (int64_t)hi);
 }
 
-// Where token `at` of a sequence lies: the addresses of its K and V rows (head
+// Table entry of token `at` of a sequence, as loaded: nothing looks at it, so
+// that the load stays in flight until token_rows does.  `at` < the sequence's
+// usable tokens.
+struct TokenEntry {
+  uint32_t lo, hi;  // an id's words; KV_OFFSETS: the entries of K and of V
+};
+
+__device__ __forceinline__ TokenEntry token_entry(const AttentionArgs &a, const QueryTile &t,
+                                                  int at) {
+  const int lb = a.block_log2 >= 0 ? at >> a.block_log2 : at / a.block_size;
+  TokenEntry e;
+  if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
+    const uint32_t *p =
+        static_cast<const uint32_t *>(a.table) + (int64_t)t.seq * 2 * a.max_blocks + lb;
+    e.lo = p[0];
+    e.hi = p[a.max_blocks];
+    return e;
+  }
+  int64_t i = (int64_t)t.seq * a.max_blocks + lb;
+  if (a.format == KVX_BLOCK_TABLE_RAGGED) {
+    i = t.ragged + at;
+    if (i < 0 || i >= a.table_count) {
+      e.lo = e.hi = 0xFFFFFFFFu;
+      return e;
+    }
+  }
+  if (a.index64) {
+    const u32x2 w = static_cast<const u32x2 *>(a.table)[i];
+    e.lo = w[0];
+    e.hi = w[1];
+  } else {
+    e.lo = static_cast<const uint32_t *>(a.table)[i];
+    e.hi = 0;
+  }
+  return e;
+}
+
+// Where the token with that entry lies: the addresses of its K and V rows (head
 // 0), or false for a token that is not there.  `block` is the physical block
-// for block-indexed scales.  `at` < the sequence's usable tokens.
+// for block-indexed scales.
 struct TokenRows {
   const char *k, *v;
   int32_t block;
 };
 
-__device__ __forceinline__ bool token_rows(const AttentionArgs &a, int seq, int at, TokenRows *r) {
-  int lb, off;
-  if (a.block_log2 >= 0) {
-    lb = at >> a.block_log2;
-    off = at - (lb << a.block_log2);
-  } else {
-    lb = at / a.block_size;
-    off = at - lb * a.block_size;
-  }
+__device__ __forceinline__ bool token_rows(const AttentionArgs &a, const TokenEntry &e, int at,
+                                           TokenRows *r) {
+  const int off = a.block_log2 >= 0 ? at & (a.block_size - 1) : at % a.block_size;
   const char *kb, *vb;
   if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
-    const uint32_t *t = static_cast<const uint32_t *>(a.table) + (int64_t)seq * 2 * a.max_blocks + lb;
-    const uint32_t ek = t[0], ev = t[a.max_blocks];
+    const uint32_t ek = e.lo, ev = e.hi;
     // selected, not indexed: arguments stay in scalar registers
     const char *pk = ek >> 31 ? a.pool[1] : a.pool[0], *pv = ev >> 31 ? a.pool[1] : a.pool[0];
     const int32_t nk = ek >> 31 ? a.pool_blocks[1] : a.pool_blocks[0];
@@ -197,12 +230,7 @@ __device__ __forceinline__ bool token_rows(const AttentionArgs &a, int seq, int 
     vb = pv + iv * a.bytes_per_block;
     r->block = 0;
   } else {
-    int64_t i = (int64_t)seq * a.max_blocks + lb;
-    if (a.format == KVX_BLOCK_TABLE_RAGGED) {
-      i = index_at(a.indptr, a.indptr64, seq) + at;
-      if (i < 0 || i >= a.table_count) return false;
-    }
-    const int64_t b = index_at(a.table, a.index64, i);
+    const int64_t b = a.index64 ? (int64_t)(((uint64_t)e.hi << 32) | e.lo) : (int64_t)(int32_t)e.lo;
     if (b < 0 || b >= a.num_blocks) return false;
     kb = a.k + b * a.gk.s_block;
     vb = a.v + b * a.gv.s_block;

@@ -83,47 +83,52 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   else return ((w & 0x7C7C7C7Cu) + 0x04040404u) & 0x80808080u;
 }
 
-template <int IO>
-constexpr uint32_t kOne = IO == KVX_DTYPE_BF16 ? 0x3F80u : 0x3C00u;
-template <int IO>
-constexpr uint32_t kInf = IO == KVX_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+// w with its NaN and infinite elements 0.
+template <int C>
+__device__ __forceinline__ uint32_t only_finite(uint32_t w) {
+  const uint32_t top = not_finite<C>(w);  // the top bit of each such element
+  constexpr int kBits = bytes_of_type<C>() * 8 - 1;
+  return w & ~(top | (top - (top >> kBits)));
+}
 
-// acc + v w where v holds NaN or infinities that must not reach, as 0 * v, a
-// row whose weight is 0: the finite values as ever, and three products of
-// zeros and ones that say which rows meet an infinity of either sign or NaN
-// with a weight.
-template <int IO, typename Acc>
-__device__ __forceinline__ Acc guarded(const Frag &v, const Frag &w, Acc acc) {
-  Frag one, fine;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    one.w[i] = (w.w[i] & 0x7FFFu ? kOne<IO> : 0u) | (w.w[i] & 0x7FFF0000u ? kOne<IO> << 16 : 0u);
-    fine.w[i] = ((v.w[i] & 0x7FFFu) < kInf<IO> ? v.w[i] & 0xFFFFu : 0u) |
-                ((v.w[i] & 0x7FFF0000u) < kInf<IO> << 16 ? v.w[i] & 0xFFFF0000u : 0u);
-  }
-  acc = mma<IO>(fine, w, acc);
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {  // infinity, -infinity, NaN: one at a time, in few registers
-    __builtin_amdgcn_sched_barrier(0);
-    Frag met;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      met.w[i] = 0;
-#pragma unroll
-      for (int half = 0; half < 32; half += 16) {
-        const uint32_t e = (v.w[i] >> half) & 0xFFFFu;
-        const bool is = k == 0 ? e == kInf<IO> : k == 1 ? e == (kInf<IO> | 0x8000u)
-                                                        : (e & 0x7FFFu) > kInf<IO>;
-        if (is) met.w[i] |= kOne<IO> << half;
+// 0 * infinity must not reach a row that does not see a token.  The kernels
+// therefore take NaN and infinities out of the values of steps that not all
+// rows of a tile see whole, note that there were some, and call this after the
+// tile's outputs are written (and a barrier): it looks at those steps again and
+// adds what they hold to the rows that see it.  A thread has elements of its
+// own, so the additions need no order.  step: tokens of a step; [all_lo, all_hi):
+// tokens that all rows see.
+template <int IO, int C>
+__device__ __forceinline__ void add_infinities(const AttentionArgs &a, const QueryTile &t, int kvh,
+                                            int head0, int nheads, int z, int from, int to, int lo,
+                                            int all_lo, int all_hi, int step) {
+  for (int d = (int)threadIdx.x; d < a.head_dim; d += (int)blockDim.x) {
+    const int64_t at_d = (d / a.gv.pack) * a.gv.s_piece + (d % a.gv.pack) * a.gv.s_inner;
+    for (int at = from > lo ? from : lo; at < to; ++at) {
+      const int base = from + (at - from) / step * step;
+      if (base >= all_lo && base + step <= all_hi) continue;
+      TokenRows r;
+      if (!token_rows(a, token_entry(a, t, at), at, &r)) continue;
+      float x = value_at<C>(r.v + kvh * a.gv.s_head + at_d);
+      if (fabsf(x) < INFINITY) continue;
+      if constexpr (C != IO) x *= scale_of(a.vs, r.block, kvh);
+      for (int i = 0; i < t.count; ++i) {
+        int rlo, rhi;
+        row_range(a, t, t.first + i, &rlo, &rhi);
+        if (at < rlo || at >= rhi) continue;
+        for (int h = 0; h < nheads; ++h) {
+          const int head = kvh * a.group + head0 + h;
+          if (a.splits > 1) {
+            float *p = a.part_o + (part_index(a, t, t.first + i, head) * a.splits + z) * a.head_dim;
+            p[d] += x;
+          } else {
+            char *p = a.out + (t.begin + t.first + i) * a.o_tok + head * a.o_head + 2 * d;
+            store_out<IO>(p, value_at<IO>(p) + x);
+          }
+        }
       }
     }
-    const Acc n = mma<IO>(met, one, Acc{});
-    const float what = k == 0 ? INFINITY : k == 1 ? -INFINITY : NAN;
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof(Acc) / 4); ++i) acc[i] += n[i] > 0.0f ? what : 0.0f;
   }
-  __builtin_amdgcn_sched_barrier(0);
-  return acc;
 }
 
 // scale * q.k in units of log2, the scale of an FP8 key included in the
@@ -161,22 +166,29 @@ __device__ __forceinline__ uint64_t from_lane(uint64_t x, int at) {
   return from_lane((uint32_t)x, at) | (uint64_t)from_lane((uint32_t)(x >> 32), at) << 32;
 }
 
-// Streaming load of B bytes of global memory (an address that went through
-// another lane is not known to be global).
-template <int B>
-__device__ __forceinline__ Raw<B> stream_load(uint64_t at) {
+// A wave-uniform copy of lane `lane`'s address.
+__device__ __forceinline__ uint64_t address_of_lane(uint64_t x, int lane) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32;
+}
+
+// B bytes of global memory at an address that went through another lane, and so
+// is not known to be global.  A uniform address and a 32-bit offset make the
+// scalar form of the load, without a vector operation for the address.  NT:
+// streamed.
+template <int B, bool NT>
+__device__ __forceinline__ Raw<B> global_load(uint64_t base, uint32_t offset) {
+  const auto *p = reinterpret_cast<const __attribute__((address_space(1))) char *>(base) + offset;
+  auto read = [](const auto *q) { return NT ? __builtin_nontemporal_load(q) : *q; };
   Raw<B> r;
   if constexpr (B == 4) {
-    r.w[0] = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) uint32_t *>(at));
+    r.w[0] = read(reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(p));
   } else if constexpr (B == 8) {
-    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) u32x2 *>(at));
+    const u32x2 v = read(reinterpret_cast<const __attribute__((address_space(1))) u32x2 *>(p));
     r.w[0] = v[0];
     r.w[1] = v[1];
   } else {
-    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<
-        const __attribute__((address_space(1))) u32x4 *>(at));
+    const u32x4 v = read(reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>(p));
 #pragma unroll
     for (int i = 0; i < 4; ++i) r.w[i] = v[i];
   }

@@ -11,6 +11,11 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 
+// Rows that have partial sums.
+__host__ __device__ __forceinline__ int64_t join_rows(const AttentionArgs &a) {
+  return a.part_rows > 0 ? (int64_t)a.seqs * a.part_rows : a.tokens;
+}
+
 // Adds up the splits of one row and head: with M the largest maximum,
 //   out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
 // One wave has a row and head; the splits' partial sums are adjacent.
@@ -20,14 +25,18 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionA
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const int hq = a.heads * a.group;
   const int64_t unit = (int64_t)blockIdx.x * (kJoinThreads / kWave) + wave;
-  if (unit >= (int64_t)a.tokens * hq) return;
-  const int row = (int)(unit / hq), head = (int)(unit - (int64_t)row * hq);
-  int64_t part = row;
+  if (unit >= join_rows(a) * hq) return;
+  const int64_t part = unit / hq;
+  const int head = (int)(unit - part * hq);
+  int64_t row = part;
   if (a.qptr != nullptr) {
-    const int s = last_sequence(a.seqs, [&](int q) { return query_begin(a, q) <= row; });
+    const int s = a.part_rows > 0 ? (int)(part / a.part_rows)
+                                  : last_sequence(a.seqs, [&](int q) {
+                                      return query_begin(a, q) <= part;
+                                    });
     const int64_t b = query_begin(a, s), n = query_begin(a, s + 1) - b;
+    if (a.part_rows > 0) row = b + part - (int64_t)s * a.part_rows;
     if (row < b || row >= b + n || n < a.least_rows || n > a.most_rows) return;
-    if (a.part_rows > 0) part = (int64_t)s * a.part_rows + (row - b);
   }
   const int64_t at = (part * hq + head) * a.splits;
   float top = -INFINITY;
@@ -56,7 +65,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionA
                     none ? 0.0f : sum[j] / total);
   }
   if (lane == 0 && a.lse != nullptr)
-    a.lse[(int64_t)row * hq + head] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+    a.lse[row * hq + head] = none ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
 GeomBytes bytes_of(const Geom &g, int esize) {
@@ -263,8 +272,7 @@ Plan make_plan(const AttentionPlan &p) {
   for (int i = 0; i < r.parts; ++i) {
     AttentionArgs &x = r.part[i].a;
     if (x.splits == 1) continue;
-    const int64_t rows = x.part_rows > 0 ? (int64_t)x.seqs * x.part_rows : x.tokens;
-    const int64_t sums = rows * p.query_heads * x.splits;
+    const int64_t sums = join_rows(x) * p.query_heads * x.splits;
     x.part_o = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + r.workspace);
     x.part_ml = x.part_o + sums * x.head_dim;
     r.workspace += ((uint64_t)sums * (x.head_dim + 2) * 4 + 15) & ~(uint64_t)15;
@@ -274,7 +282,7 @@ Plan make_plan(const AttentionPlan &p) {
 
 template <int IO>
 void launch_join(const AttentionArgs &a, hipStream_t s) {
-  const int64_t units = (int64_t)a.tokens * a.heads * a.group;
+  const int64_t units = join_rows(a) * a.heads * a.group;
   const int64_t waves = kJoinThreads / kWave;
   attention_join_kernel<IO><<<dim3((uint32_t)((units + waves - 1) / waves)), kJoinThreads, 0, s>>>(a);
 }
@@ -286,7 +294,7 @@ int64_t workgroups(const AttentionArgs &a) {
 bool launchable(const Plan &p) {
   for (int i = 0; i < p.parts; ++i) {
     const AttentionArgs &a = p.part[i].a;
-    if ((int64_t)a.tokens * a.heads * a.group * kWave > 0xFFFFFFFFll) return false;
+    if (join_rows(a) * a.heads * a.group * kWave > 0xFFFFFF00ll) return false;
     if (workgroups(a) * 256 > 0xFFFFFFFFll) return false;
     if (p.part[i].kind == kRows && (int64_t)a.heads * a.head_tiles > 65535) return false;
   }

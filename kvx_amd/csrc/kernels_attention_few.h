@@ -56,6 +56,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   constexpr int VW = VB / 4;           // dwords (VT: of four tokens)
   __shared__ float sums[2][kRowTile][DP + 4];
   __shared__ float states[kFewWaves][2][kRowTile];
+  __shared__ int infinities;  // see add_infinities
 
   const int hh = a.heads * a.head_tiles;
   uint32_t id = blockIdx.x;
@@ -91,6 +92,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     return;
   }
 
+  if (threadIdx.x == 0) infinities = 0;
+  __syncthreads();
   Frag q[KC];
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   // Offsets of the lane's pieces from a token's row; a piece past the head's
   // end is its first one (a key's counts as zero below, a value's sum is not
   // stored).
-  int32_t koff[KL];
+  uint32_t koff[KL];
 #pragma unroll
   for (int i = 0; i < KL; ++i) {
     const int d0 = (i * 64 + g * 16) / E, d = d0 < D ? d0 : 0;
@@ -114,7 +117,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   }
   constexpr int VL = VT ? NV : (VB + 15) / 16;  // value loads a token (VT: four tokens)
   constexpr int VLB = VT ? 4 * E : VB / VL;      // bytes of one
-  int32_t voff[VL];
+  uint32_t voff[VL];
 #pragma unroll
   for (int i = 0; i < VL; ++i) {
     const int d0 = VT ? 16 * i + c : c * NV + i * (VLB / E), d = d0 < D ? d0 : 0;
@@ -133,21 +136,32 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // Four tokens of a lane group lie in one block, so that their rows follow
-  // from the first's; RAGGED tables name every token's block.
-  const bool quads = VT || (a.block_size % 4 == 0 && a.format != KVX_BLOCK_TABLE_RAGGED);
+  // Where blocks hold whole half steps, a half step's rows follow from its
+  // first, a scalar address.  RAGGED tables name every token's block.
+  const bool grouped = a.block_size % (kFewStep / 2) == 0 &&
+                       a.format != KVX_BLOCK_TABLE_RAGGED && a.gk.s_off >= 0 &&
+                       a.gv.s_off >= 0 && a.gk.s_off < (1 << 24) && a.gv.s_off < (1 << 24);
+  const uint32_t krow = (uint32_t)(c * (int)a.gk.s_off);
+  const uint32_t vrow = (uint32_t)(4 * g * (int)a.gv.s_off);
 
   struct Step {
-    uint64_t k, v;      // rows of token `lane` (lanes 0 .. 31)
+    uint64_t k, v;      // rows of token `lane` (one that is not there: of another)
     uint32_t there;     // bit per token that some row may see
     bool some;          // k and v can be read
     float ks, vs;
   };
-  auto resolve = [&](int base) -> Step {
+  // A step's table entries are loaded two steps ahead and looked at one step
+  // later.
+  auto entries = [&](int base) -> TokenEntry {
+    TokenEntry e{0, 0};
+    if (lane < kFewStep && base + lane < to) e = token_entry(a, t, base + lane);
+    return e;
+  };
+  auto resolve = [&](int base, const TokenEntry &entry) -> Step {
     Step s{0, 0, 0, false, 1.0f, 1.0f};
     TokenRows r{nullptr, nullptr, 0};
     const int at = base + lane;
-    const bool held = lane < kFewStep && at < to && token_rows(a, t.seq, at, &r);
+    const bool held = lane < kFewStep && at < to && token_rows(a, entry, at, &r);
     if (held) {
       s.k = reinterpret_cast<uint64_t>(r.k + khead);
       s.v = reinterpret_cast<uint64_t>(r.v + vhead);
@@ -176,15 +190,18 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   uint32_t kw[2][KL][4];
   auto load_keys = [&](const Step &s) {
     if (!s.some) return;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint64_t p = from_lane(s.k, 4 * c + 64 * b);
+    auto one = [&](int b, uint64_t p, uint32_t row) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
-        const Raw<16> r = stream_load<16>(p + koff[i]);
+        const Raw<16> r = global_load<16, true>(p, row + koff[i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) kw[b][i][j] = r.w[j];
       }
+    };
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (grouped) one(b, address_of_lane(s.k, 16 * b), krow);
+      else one(b, from_lane(s.k, 4 * c + 64 * b), 0);
     }
   };
   // Rows: [token e][dword]; VT: [half b][element j][dword].
@@ -197,35 +214,24 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         const uint64_t p = from_lane(s.v, 16 * g + 64 * b);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const Raw<VLB> r = stream_load<VLB>(p + voff[j]);
+          const Raw<VLB> r = global_load<VLB, true>(p, voff[j]);
 #pragma unroll
           for (int w = 0; w < E; ++w) vw[b * NV + j][w] = r.w[w];
         }
       }
     } else {
-      const bool steps = quads && s.there == 0xFFFFFFFFu;
-      uint64_t rows[8];
-      if (steps) {
-        rows[0] = from_lane(s.v, 16 * g);
-        rows[4] = from_lane(s.v, 16 * g + 64);
-#pragma unroll
-        for (int e = 1; e < 4; ++e) {
-          rows[e] = rows[e - 1] + a.gv.s_off;
-          rows[4 + e] = rows[3 + e] + a.gv.s_off;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) rows[e] = from_lane(s.v, 16 * g + 4 * place_of(e));
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint64_t p = rows[e];
+      auto one = [&](int e, uint64_t p, uint32_t row) {
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-          const Raw<VLB> r = stream_load<VLB>(p + voff[i]);
+          const Raw<VLB> r = global_load<VLB, true>(p, row + voff[i]);
 #pragma unroll
           for (int w = 0; w < VLB / 4; ++w) vw[e][i * (VLB / 4) + w] = r.w[w];
         }
+      };
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (grouped) one(e, address_of_lane(s.v, 4 * (e - e % 4)) + (e % 4) * a.gv.s_off, vrow);
+        else one(e, from_lane(s.v, 16 * g + 4 * place_of(e)), 0);
       }
     }
   };
@@ -259,10 +265,11 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   int base = from + wave * kFewStep;
   constexpr int kStride = kFewWaves * kFewStep;
   if (base < to) {
-    Step now = resolve(base);
+    TokenEntry ahead = entries(base), after = entries(base + kStride);
+    Step now = resolve(base, ahead);
     load_keys(now);
     load_values(now);
-    Step next = resolve(base + kStride);  // nothing there past `to`
+    Step next = resolve(base + kStride, after);  // nothing there past `to`
     for (;;) {
       if (D != DP) {  // pieces past the head's end
 #pragma unroll
@@ -295,7 +302,10 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         }
       }
       const bool more = base + kStride < to;
-      if (more) load_keys(next);
+      if (more) {
+        ahead = entries(base + 2 * kStride);
+        load_keys(next);
+      }
 
       const bool whole = now.there == 0xFFFFFFFFu && base >= last_lo && base + kFewStep <= first_hi;
       float x[8], p[8], top = -INFINITY;
@@ -358,12 +368,16 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       for (int i = 0; i < 4; ++i) w.w[i] = pair_of<IO>(p[2 * i], p[2 * i + 1]);
 
       if (now.there != 0xFFFFFFFFu) clear_values(now.there);
-      uint32_t odd = 0;
-      if (!whole && t.count > 1) {  // a token may be there for some rows only
+      if (t.count > 1 && (base < last_lo || base + kFewStep > first_hi)) {
+        uint32_t odd = 0;  // some rows do not see some tokens
 #pragma unroll
         for (int e = 0; e < (VT ? 2 * NV : 8); ++e)
 #pragma unroll
-          for (int i = 0; i < (VT ? E : VW); ++i) odd |= not_finite<C>(vw[e][i]);
+          for (int i = 0; i < (VT ? E : VW); ++i) {
+            odd |= not_finite<C>(vw[e][i]);
+            vw[e][i] = only_finite<C>(vw[e][i]);
+          }
+        if (odd != 0) infinities = 1;
       }
       // Values by element: v[j], token order of the weights.
       auto by_element = [&](int d, Frag *v) {  // v[2 d] and v[2 d + 1]
@@ -389,29 +403,18 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
           }
         }
       };
-      if (__any(odd != 0)) {
 #pragma unroll
-        for (int d = 0; d < NV / 2; ++d) {
-          Frag v[2];
-          by_element(d, v);
-          acc[2 * d] = guarded<IO>(v[0], w, acc[2 * d]);
-          acc[2 * d + 1] = guarded<IO>(v[1], w, acc[2 * d + 1]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      } else {
-#pragma unroll
-        for (int d = 0; d < NV / 2; ++d) {
-          Frag v[2];
-          by_element(d, v);
-          acc[2 * d] = mma<IO>(v[0], w, acc[2 * d]);
-          acc[2 * d + 1] = mma<IO>(v[1], w, acc[2 * d + 1]);
-        }
+      for (int d = 0; d < NV / 2; ++d) {
+        Frag v[2];
+        by_element(d, v);
+        acc[2 * d] = mma<IO>(v[0], w, acc[2 * d]);
+        acc[2 * d + 1] = mma<IO>(v[1], w, acc[2 * d + 1]);
       }
       if (!more) break;
       load_values(next);
       now = next;
       base += kStride;
-      next = resolve(base + kStride);
+      next = resolve(base + kStride, ahead);
     }
   }
   l += __shfl_xor(l, 16);
@@ -458,48 +461,52 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     }
     __syncthreads();
   }
-  if (wave != 0) return;
-  // Through LDS once more, so that rows leave as whole lines.
-  const bool none = top == -INFINITY && l == 0.0f;
-  const float norm = a.splits > 1 ? vs : none ? 0.0f : vs / l;
+  if (wave == 0) {
+    // Through LDS once more, so that rows leave as whole lines.
+    const bool none = top == -INFINITY && l == 0.0f;
+    const float norm = a.splits > 1 ? vs : none ? 0.0f : vs / l;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      sums[0][c][element(j, i)] = a.splits == 1 && none ? 0.0f : acc[j][i] * norm;
-  const int64_t line = t.begin + t.first + tok;
-  if (row && g == 0) {
-    if (a.splits > 1) {
-      const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
-      a.part_ml[2 * at] = top;
-      a.part_ml[2 * at + 1] = l;
-    } else if (a.lse != nullptr) {
-      a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (top + log2f(l)) * kLn2;
+      for (int i = 0; i < 4; ++i)
+        sums[0][c][element(j, i)] = a.splits == 1 && none ? 0.0f : acc[j][i] * norm;
+    const int64_t line = t.begin + t.first + tok;
+    if (row && g == 0) {
+      if (a.splits > 1) {
+        const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
+        a.part_ml[2 * at] = top;
+        a.part_ml[2 * at + 1] = l;
+      } else if (a.lse != nullptr) {
+        a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (top + log2f(l)) * kLn2;
+      }
+    }
+    wave_sync();
+    const int rows = t.count * a.tile_heads;
+    constexpr int kLanes = DP / 8;  // lanes of a row
+#pragma unroll
+    for (int r0 = 0; r0 < kRowTile; r0 += kWave / kLanes) {
+      const int r = r0 + lane / kLanes, d = (lane % kLanes) * 8;
+      const int rt = r / a.tile_heads, rh = r - rt * a.tile_heads;
+      if (r >= rows || rh >= nheads || d >= D) continue;
+      const int64_t out_row = t.begin + t.first + rt;
+      const int head = kvh * a.group + head0 + rh;
+      const float *x = &sums[0][r][d];
+      if (a.splits > 1) {
+        const int64_t at = part_index(a, t, t.first + rt, head) * a.splits + z;
+        float *o = a.part_o + at * D + d;
+        *reinterpret_cast<f32x4 *>(o) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4 *>(o + 4) = f32x4{x[4], x[5], x[6], x[7]};
+      } else {
+        Raw<16> o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.w[i] = pack_pair<IO>(f32x2{x[2 * i], x[2 * i + 1]});
+        st<16>(a.out + out_row * a.o_tok + (int64_t)head * a.o_head + 2 * d, o);
+      }
     }
   }
-  wave_sync();
-  const int rows = t.count * a.tile_heads;
-  constexpr int kLanes = DP / 8;  // lanes of a row
-#pragma unroll
-  for (int r0 = 0; r0 < kRowTile; r0 += kWave / kLanes) {
-    const int r = r0 + lane / kLanes, d = (lane % kLanes) * 8;
-    const int rt = r / a.tile_heads, rh = r - rt * a.tile_heads;
-    if (r >= rows || rh >= nheads || d >= D) continue;
-    const int64_t out_row = t.begin + t.first + rt;
-    const int head = kvh * a.group + head0 + rh;
-    const float *x = &sums[0][r][d];
-    if (a.splits > 1) {
-      const int64_t at = part_index(a, t, t.first + rt, head) * a.splits + z;
-      float *o = a.part_o + at * D + d;
-      *reinterpret_cast<f32x4 *>(o) = f32x4{x[0], x[1], x[2], x[3]};
-      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
-      Raw<16> o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o.w[i] = pack_pair<IO>(f32x2{x[2 * i], x[2 * i + 1]});
-      st<16>(a.out + out_row * a.o_tok + (int64_t)head * a.o_head + 2 * d, o);
-    }
-  }
+  if (infinities == 0) return;
+  __syncthreads();
+  add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kFewStep);
 }
 
 template <int IO, int C>

@@ -47,7 +47,8 @@ constexpr int many_buffers() {
 template <int DP, bool INDEXED>
 constexpr size_t many_lds() {
   return (size_t)many_buffers<DP>() *
-         (2 * kManyStep * DP * 2 + (INDEXED ? 2 * kManyStep * 4 : 0));
+             (2 * kManyStep * DP * 2 + (INDEXED ? 2 * kManyStep * 4 : 0)) +
+         16;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -56,21 +57,6 @@ __device__ __forceinline__ u32x2 lds_transposed(const char *p) {
   return __builtin_bit_cast(
       u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                  (__attribute__((address_space(3))) s16x4 *)(p)));
-}
-
-template <int B>
-__device__ __forceinline__ Raw<B> plain_load(uint64_t at) {
-  Raw<B> r;
-  if constexpr (B == 8) {
-    const u32x2 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x2 *>(at);
-    r.w[0] = v[0];
-    r.w[1] = v[1];
-  } else {
-    const u32x4 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>(at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.w[i] = v[i];
-  }
-  return r;
 }
 
 template <int IO, int C, int DP, bool VT, bool INDEXED>
@@ -90,6 +76,8 @@ attention_many_kernel(AttentionArgs a) {
   extern __shared__ __align__(16) char lds[];
   char *const kbuf = lds, *const vbuf = lds + NB * TENSOR;
   float *const scales = reinterpret_cast<float *>(lds + 2 * NB * TENSOR);  // [buffer][k, v][64]
+  int *const infinities =
+      reinterpret_cast<int *>(lds + many_lds<DP, INDEXED>() - 16);  // see add_infinities
 
   // The last tiles of a causal chunk see most tokens: they start first.
   const int hh = a.heads * a.head_tiles;
@@ -114,9 +102,9 @@ attention_many_kernel(AttentionArgs a) {
   const int qh = kvh * a.group + head0 + rh;
   int rlo = 0, rhi = 0;
   if (row) row_range(a, t, t.first + tok, &rlo, &rhi);
-  int lo, hi, from, to, skip;
-  row_range(a, t, t.first, &lo, &skip);
-  row_range(a, t, t.first + t.count - 1, &skip, &hi);
+  int lo, hi, first_hi, last_lo, from, to;
+  row_range(a, t, t.first, &lo, &first_hi);
+  row_range(a, t, t.first + t.count - 1, &last_lo, &hi);
   split_range(a, lo, hi, z, &from, &to);
   // The wave's rows see all of [all_lo, all_hi) and nothing outside [any_lo, any_hi).
   const int tok0 = 32 * wave / a.tile_heads;
@@ -144,8 +132,8 @@ attention_many_kernel(AttentionArgs a) {
   const int d0 = chunk * 16 / E;
   const bool inside = d0 < D;
   const int kd = inside ? d0 : 0;
-  const int32_t koff = (kd / a.gk.pack) * (int32_t)a.gk.s_piece + (kd % a.gk.pack) * E;
-  int32_t voff[VT ? NVL : 1];
+  const uint32_t koff = (kd / a.gk.pack) * (int32_t)a.gk.s_piece + (kd % a.gk.pack) * E;
+  uint32_t voff[VT ? NVL : 1];
   if constexpr (VT) {
 #pragma unroll
     for (int l = 0; l < NVL; ++l) {
@@ -164,16 +152,23 @@ attention_many_kernel(AttentionArgs a) {
   const float scale = positive_scale<IO>(a, ks, q);
 
   struct Step {
-    uint64_t k, v;  // rows of token `lane`
+    uint64_t k, v;  // rows of token `lane` (one that is not there: of another)
     uint64_t there;
     float ks, vs;
     bool some;
   };
-  auto resolve = [&](int base) -> Step {
+  // A step's table entries are loaded two steps ahead and looked at one step
+  // later.
+  auto entries = [&](int base) -> TokenEntry {
+    TokenEntry e{0, 0};
+    if (base + lane < to) e = token_entry(a, t, base + lane);
+    return e;
+  };
+  auto resolve = [&](int base, const TokenEntry &entry) -> Step {
     Step s{0, 0, 0, 1.0f, 1.0f, false};
     TokenRows x{nullptr, nullptr, 0};
     const int at = base + lane;
-    const bool held = at < to && token_rows(a, t.seq, at, &x);
+    const bool held = at < to && token_rows(a, entry, at, &x);
     if (held) {
       s.k = reinterpret_cast<uint64_t>(x.k + khead);
       s.v = reinterpret_cast<uint64_t>(x.v + vhead);
@@ -196,22 +191,43 @@ attention_many_kernel(AttentionArgs a) {
     return s;
   };
 
+  // A wave's load takes kGroup tokens of one block, where blocks hold whole
+  // groups: one scalar address.  RAGGED tables name every token's block.
+  constexpr int kGroup = kWave / CPR;
+  const bool grouped = a.block_size % kGroup == 0 && a.format != KVX_BLOCK_TABLE_RAGGED &&
+                       a.gk.s_off >= 0 && a.gv.s_off >= 0 && a.gk.s_off < (1 << 24) &&
+                       a.gv.s_off < (1 << 24);
+  const uint32_t kgroup = koff + (uint32_t)((lane / CPR) * (int)a.gk.s_off);
+  const uint32_t vgroup = voff[0] + (uint32_t)((lane / CPR) * (int)a.gv.s_off);
   Raw<16> kreg[NL];
   Raw<VLB> vreg[NVL];
   auto load = [&](const Step &s) {
     if (!s.some) return;
+    if (grouped) {
 #pragma unroll
-    for (int l = 0; l < NL; ++l)
-      kreg[l] = plain_load<16>(from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)) + koff);
-    if constexpr (VT) {
-      const uint64_t p = from_lane(s.v, 32 * (tid % 8));
-#pragma unroll
-      for (int l = 0; l < NVL; ++l) vreg[l] = plain_load<VLB>(p + voff[l]);
+      for (int l = 0; l < NL; ++l)
+        kreg[l] = global_load<16, false>(
+            address_of_lane(s.k, wave * kGroup + l * (kManyThreads / CPR)), kgroup);
     } else {
 #pragma unroll
       for (int l = 0; l < NL; ++l)
-        vreg[l] =
-            plain_load<16>(from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)) + voff[0]);
+        kreg[l] = global_load<16, false>(
+            from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), koff);
+    }
+    if constexpr (VT) {
+      const uint64_t p = from_lane(s.v, 32 * (tid % 8));
+#pragma unroll
+      for (int l = 0; l < NVL; ++l) vreg[l] = global_load<VLB, false>(p, voff[l]);
+    } else if (grouped) {
+#pragma unroll
+      for (int l = 0; l < NL; ++l)
+        vreg[l] = global_load<16, false>(
+            address_of_lane(s.v, wave * kGroup + l * (kManyThreads / CPR)), vgroup);
+    } else {
+#pragma unroll
+      for (int l = 0; l < NL; ++l)
+        vreg[l] = global_load<16, false>(
+            from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), voff[0]);
     }
   };
   // A 16-byte chunk of a cached row as one (16-bit) or two (FP8) chunks in LDS;
@@ -229,14 +245,25 @@ attention_many_kernel(AttentionArgs a) {
       *reinterpret_cast<u32x4 *>(line + 16 * (chunk ^ swap)) = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
     }
   };
-  auto store = [&](const Step &s, int buffer) {
+  auto store = [&](const Step &s, int base, int buffer) {
     char *kb = kbuf + buffer * TENSOR, *vb = vbuf + buffer * TENSOR;
     const bool whole = s.there == ~0ull;
+    if (base < last_lo || base + kManyStep > first_hi) {  // some rows do not see some tokens
+      uint32_t odd = 0;
+#pragma unroll
+      for (int l = 0; l < NVL; ++l)
+#pragma unroll
+        for (int w = 0; w < VLB / 4; ++w) {
+          odd |= not_finite<C>(vreg[l].w[w]);
+          vreg[l].w[w] = only_finite<C>(vreg[l].w[w]);
+        }
+      if (odd != 0) *infinities = 1;
+    }
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int at = tid / CPR + l * (kManyThreads / CPR);
       Raw<16> x = kreg[l];
-      if (!inside) x = Raw<16>{};
+      if (D != DP && !inside) x = Raw<16>{};
       put(kb + at * ROW, at & 7, x);
     }
     if constexpr (VT) {
@@ -396,48 +423,36 @@ attention_many_kernel(AttentionArgs a) {
       }
       return f;
     };
-    if (whole) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+    for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = mma<IO>(values(kk, j), w[kk], acc[j]);
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const Frag v = values(kk, j);
-          const uint32_t odd = not_finite<IO>(v.w[0]) | not_finite<IO>(v.w[1]) |
-                               not_finite<IO>(v.w[2]) | not_finite<IO>(v.w[3]);
-          if (__any(odd != 0)) acc[j] = guarded<IO>(v, w[kk], acc[j]);
-          else acc[j] = mma<IO>(v, w[kk], acc[j]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+      for (int j = 0; j < NJ; ++j) acc[j] = mma<IO>(values(kk, j), w[kk], acc[j]);
   };
 
+  if (tid == 0) *infinities = 0;
+  __syncthreads();
   if (from < to) {
-    Step now = resolve(from);
+    TokenEntry ahead = entries(from), after = entries(from + kManyStep);
+    Step now = resolve(from, ahead);
     load(now);
-    Step next = resolve(from + kManyStep);  // nothing there past `to`
-    store(now, 0);
+    Step next = resolve(from + kManyStep, after);  // nothing there past `to`
+    store(now, from, 0);
     __syncthreads();
     int buffer = 0;
     for (int base = from;; base += kManyStep) {
       const bool more = base + kManyStep < to;
-      Step after{};
       if (more) {
+        ahead = entries(base + 2 * kManyStep);
         load(next);
-        after = resolve(base + 2 * kManyStep);
       }
       step(now, base, buffer);
       if (!more) break;
       if constexpr (NB == 1) __syncthreads();
       else buffer ^= 1;
-      store(next, buffer);
-      __syncthreads();
+      store(next, base + kManyStep, buffer);
       now = next;
-      next = after;
+      next = resolve(base + 2 * kManyStep, ahead);
+      __syncthreads();
     }
   }
   l += __shfl_xor(l, 32);
@@ -445,46 +460,49 @@ attention_many_kernel(AttentionArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] *= vref;
   }
-  if (!row) return;
   const bool none = m == -INFINITY && l == 0.0f;
   const int64_t line = t.begin + t.first + tok;
-  if (a.splits > 1) {
+  if (row && a.splits > 1) {
     const int64_t at = part_index(a, t, t.first + tok, qh) * a.splits + z;
     if (h == 0) {
       a.part_ml[2 * at] = m;
       a.part_ml[2 * at + 1] = l;
     }
-    if (none) return;
+    if (!none) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 32 * j + 8 * i + 4 * h;
+          if (d < D)
+            *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) =
+                f32x4{acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]} * vs;
+        }
+    }
+  } else if (row) {
+    if (h == 0 && a.lse != nullptr)
+      a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (m + log2f(l)) * kLn2;
+    const float norm = vs / l;
+    char *out = a.out + line * a.o_tok + (int64_t)qh * a.o_head;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * j + 8 * i + 4 * h;
-        if (d < D)
-          *reinterpret_cast<f32x4 *>(a.part_o + at * D + d) =
-              f32x4{acc[j][4 * i], acc[j][4 * i + 1], acc[j][4 * i + 2], acc[j][4 * i + 3]} * vs;
+        if (d >= D) continue;
+        Raw<8> o;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float x0 = none ? 0.0f : acc[j][4 * i + 2 * k] * norm;
+          const float x1 = none ? 0.0f : acc[j][4 * i + 2 * k + 1] * norm;
+          o.w[k] = pack_pair<IO>(f32x2{x0, x1});
+        }
+        st<8>(out + 2 * d, o);
       }
-    return;
   }
-  if (h == 0 && a.lse != nullptr)
-    a.lse[line * (a.heads * a.group) + qh] = none ? -INFINITY : (m + log2f(l)) * kLn2;
-  const float norm = vs / l;
-  char *out = a.out + line * a.o_tok + (int64_t)qh * a.o_head;
-#pragma unroll
-  for (int j = 0; j < NJ; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * j + 8 * i + 4 * h;
-      if (d >= D) continue;
-      Raw<8> o;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float x0 = none ? 0.0f : acc[j][4 * i + 2 * k] * norm;
-        const float x1 = none ? 0.0f : acc[j][4 * i + 2 * k + 1] * norm;
-        o.w[k] = pack_pair<IO>(f32x2{x0, x1});
-      }
-      st<8>(out + 2 * d, o);
-    }
+  __syncthreads();
+  if (*infinities != 0)
+    add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kManyStep);
 }
 
 template <int IO, int C>

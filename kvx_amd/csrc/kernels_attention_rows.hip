@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(AttentionA
   for (int base = from + wave * kWave; base < to; base += kRowsThreads) {
     const int at = base + lane;
     TokenRows tr{nullptr, nullptr, 0};
-    const bool there = at < to && token_rows(a, t.seq, at, &tr);
+    const bool there = at < to && token_rows(a, token_entry(a, t, at), at, &tr);
     float s[kRowTile];
 #pragma unroll
     for (int r = 0; r < kRowTile; ++r) s[r] = 0.0f;

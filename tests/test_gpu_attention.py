@@ -183,6 +183,38 @@ def test_masked_tokens_do_not_reach_rows(io, bad):
     c.check()
 
 
+@pytest.mark.parametrize("io,cache", [("bf16", None), ("f16", None), ("f16", "e5m2"),
+                                      ("bf16", "e4m3"), ("f32", None)])
+@pytest.mark.parametrize("layout", ["nhd", "vllm"])
+@pytest.mark.parametrize("new", [[40, 6], [5, 6]])
+@pytest.mark.parametrize("long", [0, 3000])
+def test_infinities_of_single_elements(io, cache, layout, new, long):
+    """One element of a value infinite (or NaN): that element of the rows that
+    see the token, and nothing else; also where tokens are split."""
+    bad = float("inf") if cache != "e4m3" else float("nan")
+    c = AttentionCase(io=io, cache=cache, layout=layout, lens=[60 + long, 90], new=new, D=64, H=2,
+                      G=2)
+    want, _, tol, _ = c.reference()
+    for s, back, h, d, sign in ((0, 2, 1, 17, 1), (0, 3, 0, 40, -1), (1, 4, 1, 63, 1)):
+        t = c.lens[s] - back
+        v = c.rows[1][int(c.tb[s, t // 16]), t % 16, h]
+        v[d] = sign * bad
+        rows = range(sum(new[:s]) + new[s] - back, sum(new[: s + 1]))
+        for r in rows:
+            for j in range(h * c.G, h * c.G + c.G):
+                want[r, j, d] = want[r, j, d] + sign * bad
+    set_rows(c.cache.value_cache, c.cache.v_layout, c.rows[1])
+    assert c.run() == Status.OK
+    torch.cuda.synchronize()
+    got = c.out.cpu().double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[~fine & ~torch.isnan(want)], want[~fine & ~torch.isnan(want)])
+    half = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}[io]
+    over = (got - want).abs()[fine] - (tol + half * (want.abs() + tol) + 2.0 ** -25)[fine]
+    assert (over <= 0).all()
+
+
 @pytest.mark.parametrize("io", ["bf16", "f32"])
 @pytest.mark.parametrize("new", [None, [50, 3]])
 def test_large_logits(io, new):
