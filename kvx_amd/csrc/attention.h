@@ -44,6 +44,8 @@ struct AttentionArgs {
   int32_t pool_blocks[2];
   int32_t format, index64, indptr64, lens64;
   int32_t max_blocks, block_size, block_log2, num_blocks;  // block_log2 < 0: not a power of two
+  int32_t entry_log2;    // bytes of a table entry
+  int64_t entry_second;  // from an entry's low word (or K's entry) to its high (V's)
   // queries; strides in bytes
   const char *q;
   char *out;
@@ -75,7 +77,7 @@ struct QueryTile {
   int32_t rows;    // the sequence's new tokens
   int64_t length;  // its cached tokens, as given
   int32_t usable;  // of those, the ones the table can hold
-  int64_t ragged;  // RAGGED: number of its first token
+  const char *entries;  // its table entries: one per block (RAGGED: per token)
 };
 
 __device__ __forceinline__ int64_t index_at(const void *p, bool is64, int64_t i) {
@@ -128,17 +130,19 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
     t->count = min(a.tile_tokens, t->rows - t->first);
   }
   t->length = index_at(a.lens, a.lens64, t->seq);
-  int64_t hold;
-  t->ragged = 0;
+  int64_t hold, first;
   if (a.format == KVX_BLOCK_TABLE_RAGGED) {
-    t->ragged = index_at(a.indptr, a.indptr64, t->seq);
-    hold = index_at(a.indptr, a.indptr64, t->seq + 1) - t->ragged;
+    first = index_at(a.indptr, a.indptr64, t->seq);
+    hold = index_at(a.indptr, a.indptr64, t->seq + 1);
+    hold = first < 0 ? 0 : min(hold, a.table_count) - first;
     if (hold > 0x7FFF0000) hold = 0x7FFF0000;
   } else {
+    first = (int64_t)t->seq * a.max_blocks * (a.format == KVX_BLOCK_TABLE_KV_OFFSETS ? 2 : 1);
     hold = (int64_t)a.max_blocks * a.block_size;
   }
   hold = min(hold, t->length);
   t->usable = hold < 0 ? 0 : (int32_t)hold;
+  t->entries = static_cast<const char *>(a.table) + first * (a.index64 ? 8 : 4);
   return true;
 }
 
@@ -173,37 +177,17 @@ __device__ __forceinline__ void split_range(const AttentionArgs &a, int lo, int 
 // that the load stays in flight until token_rows does.  `at` < the sequence's
 // usable tokens.
 struct TokenEntry {
-  uint32_t lo, hi;  // an id's words; KV_OFFSETS: the entries of K and of V
+  uint32_t lo, hi;  // an id's words (hi = lo for 32 bits); KV_OFFSETS: of K and of V
 };
 
 __device__ __forceinline__ TokenEntry token_entry(const AttentionArgs &a, const QueryTile &t,
                                                   int at) {
-  const int lb = a.block_log2 >= 0 ? at >> a.block_log2 : at / a.block_size;
-  TokenEntry e;
-  if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
-    const uint32_t *p =
-        static_cast<const uint32_t *>(a.table) + (int64_t)t.seq * 2 * a.max_blocks + lb;
-    e.lo = p[0];
-    e.hi = p[a.max_blocks];
-    return e;
-  }
-  int64_t i = (int64_t)t.seq * a.max_blocks + lb;
-  if (a.format == KVX_BLOCK_TABLE_RAGGED) {
-    i = t.ragged + at;
-    if (i < 0 || i >= a.table_count) {
-      e.lo = e.hi = 0xFFFFFFFFu;
-      return e;
-    }
-  }
-  if (a.index64) {
-    const u32x2 w = static_cast<const u32x2 *>(a.table)[i];
-    e.lo = w[0];
-    e.hi = w[1];
-  } else {
-    e.lo = static_cast<const uint32_t *>(a.table)[i];
-    e.hi = 0;
-  }
-  return e;
+  uint32_t i = (uint32_t)at;
+  if (a.format != KVX_BLOCK_TABLE_RAGGED)
+    i = a.block_log2 >= 0 ? i >> a.block_log2 : i / (uint32_t)a.block_size;
+  const char *p = t.entries + ((int64_t)i << a.entry_log2);
+  return {*reinterpret_cast<const uint32_t *>(p),
+          *reinterpret_cast<const uint32_t *>(p + a.entry_second)};
 }
 
 // Where the token with that entry lies: the addresses of its K and V rows (head
@@ -216,7 +200,8 @@ struct TokenRows {
 
 __device__ __forceinline__ bool token_rows(const AttentionArgs &a, const TokenEntry &e, int at,
                                            TokenRows *r) {
-  const int off = a.block_log2 >= 0 ? at & (a.block_size - 1) : at % a.block_size;
+  const int off = (int)(a.block_log2 >= 0 ? (uint32_t)at & (uint32_t)(a.block_size - 1)
+                                          : (uint32_t)at % (uint32_t)a.block_size);
   const char *kb, *vb;
   if (a.format == KVX_BLOCK_TABLE_KV_OFFSETS) {
     const uint32_t ek = e.lo, ev = e.hi;
@@ -286,19 +271,32 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 void run_attention_rows(const AttentionArgs &a, int io, int cache, hipStream_t s);
-// vt: values with the token axis innermost
-void run_attention_few_bf16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_few_bf16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_few_f16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_bf16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_bf16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_bf16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_f16(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_f16_e4m3(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
-void run_attention_many_f16_e5m2(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s);
+// vt: values with the token axis innermost; grouped: blocks hold whole groups of
+// the tokens that a wave loads together, whose rows follow from the first's
+void run_attention_few_bf16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_bf16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_f16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_bf16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_bf16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_bf16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_f16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_f16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_many_f16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
 
 }  // namespace dev
 }  // namespace kvx

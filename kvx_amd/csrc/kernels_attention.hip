@@ -134,6 +134,7 @@ struct Plan {
   } part[2];
   int parts;
   bool vt;
+  bool grouped;
   uint64_t workspace;
 };
 
@@ -206,6 +207,10 @@ Plan make_plan(const AttentionPlan &p) {
   a.block_size = g.block_size;
   a.block_log2 = (g.block_size & (g.block_size - 1)) == 0 ? __builtin_ctz(g.block_size) : -1;
   a.num_blocks = g.num_blocks;
+  a.entry_log2 = g.index_is64 ? 3 : 2;
+  a.entry_second = g.format == KVX_BLOCK_TABLE_KV_OFFSETS ? (int64_t)g.max_blocks_per_seq * 4
+                   : g.index_is64                         ? 4
+                                                          : 0;
   a.q = static_cast<const char *>(p.query);
   a.out = static_cast<char *>(p.out);
   a.lse = p.lse;
@@ -242,6 +247,11 @@ Plan make_plan(const AttentionPlan &p) {
   const bool all_few = a.qptr == nullptr || a.tokens <= few ||
                        (p.max_query_len > 0 && p.max_query_len <= few);
   const bool all_many = !all_few && a.seqs == 1;
+  // Groups of 16 tokens at most share a load.  RAGGED tables name every token's
+  // block.
+  auto steps_fit = [&](const Geom &x) { return x.s_off >= 0 && x.s_off * cs < (1 << 24); };
+  r.grouped = g.block_size % 16 == 0 && g.format != KVX_BLOCK_TABLE_RAGGED && steps_fit(g.gk) &&
+              steps_fit(g.gv);
   const bool few_ok = cores && values_fit(p, kFew, &r.vt);
   bool vt_many = false;
   const bool many_ok = few_ok && values_fit(p, kMany, &vt_many) && vt_many == r.vt;
@@ -301,23 +311,23 @@ bool launchable(const Plan &p) {
   return true;
 }
 
-void run_part(const Plan::Part &p, bool vt, int io, int cache, hipStream_t s) {
+void run_part(const Plan::Part &p, bool vt, bool grouped, int io, int cache, hipStream_t s) {
   const int64_t grid = workgroups(p.a);
   const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
   if (p.kind == kRows)
     run_attention_rows(p.a, io, cache, s);
   else if (p.kind == kFew && io == KVX_DTYPE_BF16)
     (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
-                                           : run_attention_few_bf16)(p.a, vt, grid, s);
+                                           : run_attention_few_bf16)(p.a, vt, grouped, grid, s);
   else if (p.kind == kFew)
     (e4 ? run_attention_few_f16_e4m3 : e5 ? run_attention_few_f16_e5m2
-                                          : run_attention_few_f16)(p.a, vt, grid, s);
+                                          : run_attention_few_f16)(p.a, vt, grouped, grid, s);
   else if (io == KVX_DTYPE_BF16)
     (e4 ? run_attention_many_bf16_e4m3 : e5 ? run_attention_many_bf16_e5m2
-                                            : run_attention_many_bf16)(p.a, vt, grid, s);
+                                            : run_attention_many_bf16)(p.a, vt, grouped, grid, s);
   else
     (e4 ? run_attention_many_f16_e4m3 : e5 ? run_attention_many_f16_e5m2
-                                           : run_attention_many_f16)(p.a, vt, grid, s);
+                                           : run_attention_many_f16)(p.a, vt, grouped, grid, s);
 }
 
 }  // namespace
@@ -332,7 +342,7 @@ kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!launchable(plan)) return KVX_STATUS_UNSUPPORTED;
   for (int i = 0; i < plan.parts; ++i) {
-    run_part(plan.part[i], plan.vt, p.g.io_dtype, p.g.cache_dtype, s);
+    run_part(plan.part[i], plan.vt, plan.grouped, p.g.io_dtype, p.g.cache_dtype, s);
     const AttentionArgs &a = plan.part[i].a;
     if (a.splits == 1) continue;
     if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(a, s);

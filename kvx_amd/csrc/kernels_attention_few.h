@@ -45,7 +45,7 @@ __device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12
 // IO: type of queries and of the products; C: the cache's type; DP: head_dim
 // rounded up to 64, 128 or 256; VT: values with the token axis innermost;
 // INDEXED: scales by block.
-template <int IO, int C, int DP, bool VT, bool INDEXED>
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
 __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_kernel(AttentionArgs a) {
   constexpr bool kFp8 = C != IO;
   constexpr int E = kFp8 ? 1 : 2;
@@ -136,11 +136,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  // Where blocks hold whole half steps, a half step's rows follow from its
-  // first, a scalar address.  RAGGED tables name every token's block.
-  const bool grouped = a.block_size % (kFewStep / 2) == 0 &&
-                       a.format != KVX_BLOCK_TABLE_RAGGED && a.gk.s_off >= 0 &&
-                       a.gv.s_off >= 0 && a.gk.s_off < (1 << 24) && a.gv.s_off < (1 << 24);
+  // GROUPED: blocks hold whole half steps, whose rows follow from the first, a
+  // scalar address.
   const uint32_t krow = (uint32_t)(c * (int)a.gk.s_off);
   const uint32_t vrow = (uint32_t)(4 * g * (int)a.gv.s_off);
 
@@ -200,7 +197,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     };
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      if (grouped) one(b, address_of_lane(s.k, 16 * b), krow);
+      if constexpr (GROUPED) one(b, address_of_lane(s.k, 16 * b), krow);
       else one(b, from_lane(s.k, 4 * c + 64 * b), 0);
     }
   };
@@ -230,7 +227,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       };
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (grouped) one(e, address_of_lane(s.v, 4 * (e - e % 4)) + (e % 4) * a.gv.s_off, vrow);
+        if constexpr (GROUPED)
+          one(e, address_of_lane(s.v, 4 * (e - e % 4)) + (e % 4) * a.gv.s_off, vrow);
         else one(e, from_lane(s.v, 16 * g + 4 * place_of(e)), 0);
       }
     }
@@ -510,26 +508,32 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 }
 
 template <int IO, int C>
-void launch_few(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s) {
+void launch_few(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hipStream_t s) {
   const dim3 b((uint32_t)grid);
   const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
-  auto go = [&](auto dp, auto vt_, auto indexed_) {
-    attention_few_kernel<IO, C, decltype(dp)::value, decltype(vt_)::value,
-                         decltype(indexed_)::value><<<b, kFewThreads, 0, s>>>(a);
+  auto go = [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
+    constexpr int kDim = decltype(dp)::value;
+    constexpr bool kIndexed = decltype(indexed_)::value;
+    attention_few_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed, decltype(grouped_)::value>
+        <<<b, kFewThreads, 0, s>>>(a);
   };
-  auto by_dim = [&](auto vt_, auto indexed_) {
-    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_);
-    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_);
-    else go(std::integral_constant<int, 256>{}, vt_, indexed_);
+  auto by_dim = [&](auto vt_, auto indexed_, auto grouped_) {
+    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_, grouped_);
+    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_, grouped_);
+    else go(std::integral_constant<int, 256>{}, vt_, indexed_, grouped_);
   };
-  auto by_scale = [&](auto vt_) {
+  auto by_scale = [&](auto vt_, auto grouped_) {
     if constexpr (C != IO) {
-      if (indexed) return by_dim(vt_, std::true_type{});
+      if (indexed) return by_dim(vt_, std::true_type{}, grouped_);
     }
-    by_dim(vt_, std::false_type{});
+    by_dim(vt_, std::false_type{}, grouped_);
   };
-  if (vt) by_scale(std::true_type{});
-  else by_scale(std::false_type{});
+  auto by_values = [&](auto grouped_) {
+    if (vt) by_scale(std::true_type{}, grouped_);
+    else by_scale(std::false_type{}, grouped_);
+  };
+  if (grouped) by_values(std::true_type{});
+  else by_values(std::false_type{});
 }
 
 }  // namespace dev

@@ -51,6 +51,19 @@ constexpr size_t many_lds() {
          16;
 }
 
+// What is XORed to the number of a 16-byte chunk of a token's key or value.  LDS
+// has 64 banks of 4 bytes: 16 lanes that read the same chunk of 16 keys, and 32
+// that transpose 4 chunks of 4 values, meet all of them (a row of 128 bytes
+// takes half of the banks, by its token's parity).
+template <int DP>
+__device__ __forceinline__ int key_swap(int token) {
+  return DP == 64 ? (token >> 1) & 7 : token & 15;
+}
+template <int DP>
+__device__ __forceinline__ int value_swap(int token) {
+  return DP == 64 ? 4 * ((token >> 1) & 1) : 4 * (token & 3);
+}
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x2 lds_transposed(const char *p) {
@@ -59,7 +72,7 @@ __device__ __forceinline__ u32x2 lds_transposed(const char *p) {
                  (__attribute__((address_space(3))) s16x4 *)(p)));
 }
 
-template <int IO, int C, int DP, bool VT, bool INDEXED>
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
 __global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : 2)
 attention_many_kernel(AttentionArgs a) {
   constexpr bool kFp8 = C != IO;
@@ -191,19 +204,16 @@ attention_many_kernel(AttentionArgs a) {
     return s;
   };
 
-  // A wave's load takes kGroup tokens of one block, where blocks hold whole
-  // groups: one scalar address.  RAGGED tables name every token's block.
+  // GROUPED: a wave's load takes kGroup tokens of one block, from one scalar
+  // address.
   constexpr int kGroup = kWave / CPR;
-  const bool grouped = a.block_size % kGroup == 0 && a.format != KVX_BLOCK_TABLE_RAGGED &&
-                       a.gk.s_off >= 0 && a.gv.s_off >= 0 && a.gk.s_off < (1 << 24) &&
-                       a.gv.s_off < (1 << 24);
   const uint32_t kgroup = koff + (uint32_t)((lane / CPR) * (int)a.gk.s_off);
   const uint32_t vgroup = voff[0] + (uint32_t)((lane / CPR) * (int)a.gv.s_off);
   Raw<16> kreg[NL];
   Raw<VLB> vreg[NVL];
   auto load = [&](const Step &s) {
     if (!s.some) return;
-    if (grouped) {
+    if constexpr (GROUPED) {
 #pragma unroll
       for (int l = 0; l < NL; ++l)
         kreg[l] = global_load<16, false>(
@@ -218,7 +228,7 @@ attention_many_kernel(AttentionArgs a) {
       const uint64_t p = from_lane(s.v, 32 * (tid % 8));
 #pragma unroll
       for (int l = 0; l < NVL; ++l) vreg[l] = global_load<VLB, false>(p, voff[l]);
-    } else if (grouped) {
+    } else if constexpr (GROUPED) {
 #pragma unroll
       for (int l = 0; l < NL; ++l)
         vreg[l] = global_load<16, false>(
@@ -264,7 +274,7 @@ attention_many_kernel(AttentionArgs a) {
       const int at = tid / CPR + l * (kManyThreads / CPR);
       Raw<16> x = kreg[l];
       if (D != DP && !inside) x = Raw<16>{};
-      put(kb + at * ROW, at & 7, x);
+      put(kb + at * ROW, key_swap<DP>(at), x);
     }
     if constexpr (VT) {
       const uint32_t have = (uint32_t)(s.there >> (8 * (tid % 8))) & 0xFFu;
@@ -280,7 +290,9 @@ attention_many_kernel(AttentionArgs a) {
             o[w] &= ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
                     ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
         }
-        *reinterpret_cast<u32x4 *>(vb + e * (kManyStep * 2) + 16 * ((tid % 8) ^ (e & 7))) = o;
+        const int swap = (e / 2) % 16;
+        if (swap & 1) o = u32x4{o[2], o[3], o[0], o[1]};
+        *reinterpret_cast<u32x4 *>(vb + e * (kManyStep * 2) + 16 * ((tid % 8) ^ (swap / 2))) = o;
       }
     } else {
 #pragma unroll
@@ -288,7 +300,7 @@ attention_many_kernel(AttentionArgs a) {
         const int at = tid / CPR + l * (kManyThreads / CPR);
         Raw<16> x = vreg[l];
         if (!whole && !((s.there >> at) & 1)) x = Raw<16>{};
-        put(vb + at * ROW, 2 * (at & 3), x);
+        put(vb + at * ROW, value_swap<DP>(at), x);
       }
     }
     if constexpr (INDEXED) {
@@ -314,7 +326,7 @@ attention_many_kernel(AttentionArgs a) {
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
         const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + b * 32 * ROW +
-                                                         16 * ((2 * i + h) ^ (c & 7)));
+                                                         16 * ((2 * i + h) ^ key_swap<DP>(c)));
         Frag k;
 #pragma unroll
         for (int w = 0; w < 4; ++w) k.w[w] = x[w];
@@ -403,17 +415,18 @@ attention_many_kernel(AttentionArgs a) {
     auto values = [&](int kk, int j) -> Frag {
       Frag f;
       if constexpr (VT) {
-        const int e = 32 * j + c;
-        const char *line = vb + e * (kManyStep * 2) + 8 * h;
-        const u32x2 x = *reinterpret_cast<const u32x2 *>(line + 16 * ((2 * kk) ^ (e & 7)));
-        const u32x2 y = *reinterpret_cast<const u32x2 *>(line + 16 * ((2 * kk + 1) ^ (e & 7)));
+        // units of 4 tokens, permuted by the element
+        const char *line = vb + (32 * j + c) * (kManyStep * 2);
+        const int swap = (c / 2) % 16;
+        const u32x2 x = *reinterpret_cast<const u32x2 *>(line + 8 * ((4 * kk + h) ^ swap));
+        const u32x2 y = *reinterpret_cast<const u32x2 *>(line + 8 * ((4 * kk + 2 + h) ^ swap));
         f.w[0] = x[0];
         f.w[1] = x[1];
         f.w[2] = y[0];
         f.w[3] = y[1];
       } else {
         const int i = lane % 16, token = 16 * kk + 4 * h + i / 4;
-        const int piece = (4 * j + 2 * ((lane / 16) % 2) + (i % 4) / 2) ^ (2 * (i / 4));
+        const int piece = (4 * j + 2 * ((lane / 16) % 2) + (i % 4) / 2) ^ value_swap<DP>(i / 4);
         const char *p = vb + token * ROW + 16 * piece + 8 * (i % 2);
         const u32x2 x = lds_transposed(p), y = lds_transposed(p + 8 * ROW);
         f.w[0] = x[0];
@@ -506,28 +519,32 @@ attention_many_kernel(AttentionArgs a) {
 }
 
 template <int IO, int C>
-void launch_many(const AttentionArgs &a, bool vt, int64_t grid, hipStream_t s) {
+void launch_many(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hipStream_t s) {
   const dim3 b((uint32_t)grid);
   const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
-  auto go = [&](auto dp, auto vt_, auto indexed_) {
+  auto go = [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
     constexpr int kDim = decltype(dp)::value;
     constexpr bool kIndexed = decltype(indexed_)::value;
-    attention_many_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed>
+    attention_many_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed, decltype(grouped_)::value>
         <<<b, kManyThreads, many_lds<kDim, kIndexed>(), s>>>(a);
   };
-  auto by_dim = [&](auto vt_, auto indexed_) {
-    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_);
-    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_);
-    else go(std::integral_constant<int, 256>{}, vt_, indexed_);
+  auto by_dim = [&](auto vt_, auto indexed_, auto grouped_) {
+    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_, grouped_);
+    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_, grouped_);
+    else go(std::integral_constant<int, 256>{}, vt_, indexed_, grouped_);
   };
-  auto by_scale = [&](auto vt_) {
+  auto by_scale = [&](auto vt_, auto grouped_) {
     if constexpr (C != IO) {
-      if (indexed) return by_dim(vt_, std::true_type{});
+      if (indexed) return by_dim(vt_, std::true_type{}, grouped_);
     }
-    by_dim(vt_, std::false_type{});
+    by_dim(vt_, std::false_type{}, grouped_);
   };
-  if (vt) by_scale(std::true_type{});
-  else by_scale(std::false_type{});
+  auto by_values = [&](auto grouped_) {
+    if (vt) by_scale(std::true_type{}, grouped_);
+    else by_scale(std::false_type{}, grouped_);
+  };
+  if (grouped) by_values(std::true_type{});
+  else by_values(std::false_type{});
 }
 
 }  // namespace dev
