@@ -6,8 +6,8 @@
 // multiply-add, an exp2, a sum and half a conversion.
 //
 // Four waves with 32 rows each share steps of 64 tokens through LDS, two
-// buffers, loaded one step ahead through registers (where FP8 codes become
-// 16-bit elements, and values of slots without a token zeros).
+// buffers, loaded one step ahead: straight from memory, or through registers
+// where FP8 codes become 16-bit elements or something has to be left out.
 //
 // v_mfma_f32_32x32x16: lane l = 32 h + c holds A[row c][8 h .. 8 h + 7],
 // B[8 h ..][column c], D[rows 8 (i / 4) + 4 h + i % 4][column c], i < 16.
@@ -39,16 +39,15 @@ constexpr int kManyThreads = kManyWaves * kWave;
 static_assert(kManyRowTile == 32 * kManyWaves, "32 rows a wave");
 constexpr int kManyStep = 64;
 
-template <int DP>
-constexpr int many_buffers() {
-  return DP <= 128 ? 2 : 1;
-}
+// Operands are read from LDS this many products before they are used (about 128
+// cycles of 32 each); scheduling barriers, which vector and scalar operations
+// may cross, keep the compiler from moving the reads to their uses.
+constexpr int kAhead = 4;
+constexpr int kMayCross = 0x2 | 0x4;
 
 template <int DP, bool INDEXED>
 constexpr size_t many_lds() {
-  return (size_t)many_buffers<DP>() *
-             (2 * kManyStep * DP * 2 + (INDEXED ? 2 * kManyStep * 4 : 0)) +
-         16;
+  return (size_t)2 * (2 * kManyStep * DP * 2 + (INDEXED ? 2 * kManyStep * 4 : 0)) + 16;
 }
 
 // What is XORed to the number of a 16-byte chunk of a token's key or value.  LDS
@@ -57,7 +56,8 @@ constexpr size_t many_lds() {
 // takes half of the banks, by its token's parity).
 template <int DP>
 __device__ __forceinline__ int key_swap(int token) {
-  return DP == 64 ? (token >> 1) & 7 : token & 15;
+  // DP 256: a thread's loads step by 8 tokens, which the permutation must not see
+  return DP == 64 ? (token >> 1) & 7 : DP == 128 ? token & 15 : token & 7;
 }
 template <int DP>
 __device__ __forceinline__ int value_swap(int token) {
@@ -66,10 +66,24 @@ __device__ __forceinline__ int value_swap(int token) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ u32x2 lds_transposed(const char *p) {
-  return __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                 (__attribute__((address_space(3))) s16x4 *)(p)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+// 16 bytes a lane of global memory into LDS, lane after lane from `to` (uniform)
+// on; there once vmcnt is 0.
+__device__ __forceinline__ void copy_to_lds(uint64_t base, uint32_t offset, lds_char *to) {
+  __builtin_amdgcn_global_load_lds(
+      reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(
+          reinterpret_cast<const __attribute__((address_space(1))) char *>(base) + offset),
+      reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(to), 16, 0, 0);
+}
+
+template <typename V>
+__device__ __forceinline__ V lds_read(const lds_char *at) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) V *>(at);
+}
+__device__ __forceinline__ u32x2 lds_transposed(const lds_char *at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4 *)(at)));
 }
 
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
@@ -82,13 +96,13 @@ attention_many_kernel(AttentionArgs a) {
   constexpr int ROW = DP * 2;                   // bytes of a row in LDS
   constexpr int CPR = DP * E / 16;              // 16-byte chunks of a cached row
   constexpr int NL = kManyStep * CPR / kManyThreads;  // of them a thread loads
-  constexpr int NB = many_buffers<DP>();
+  constexpr int NB = 2;                         // buffers
   constexpr int NVL = VT ? DP / 32 : NL;        // value loads (VT: 8 tokens of an element)
   constexpr int VLB = VT ? 8 * E : 16;
   constexpr int TENSOR = kManyStep * ROW;
-  extern __shared__ __align__(16) char lds[];
-  char *const kbuf = lds, *const vbuf = lds + NB * TENSOR;
-  float *const scales = reinterpret_cast<float *>(lds + 2 * NB * TENSOR);  // [buffer][k, v][64]
+  extern __shared__ __align__(1024) char lds[];
+  constexpr int BUFFER = 2 * TENSOR;  // keys, then values
+  float *const scales = reinterpret_cast<float *>(lds + NB * BUFFER);  // [buffer][k, v][64]
   int *const infinities =
       reinterpret_cast<int *>(lds + many_lds<DP, INDEXED>() - 16);  // see add_infinities
 
@@ -139,13 +153,17 @@ attention_many_kernel(AttentionArgs a) {
     for (int j = 0; j < 4; ++j) q[i].w[j] = x.w[j];
   }
 
-  // What this thread loads of a step: chunk `chunk` of tokens tok_l + l * (256 /
-  // CPR); VT: tokens 8 (tid % 8) .. of elements tid / 8 + 32 l.
+  // What this thread loads of a step: a chunk each of the keys and values of
+  // tokens tid / CPR + l * (256 / CPR); VT: 8 tokens of elements tid / 8 + 32 l.
+  // Sixteen-bit elements go to LDS as they are, lane after lane, so that the
+  // permutation of a row's chunks is one of what the lanes read.
   const int chunk = tid % CPR;
-  const int d0 = chunk * 16 / E;
-  const bool inside = d0 < D;
-  const int kd = inside ? d0 : 0;
+  const int kd0 = (kFp8 ? chunk : chunk ^ key_swap<DP>(tid / CPR)) * 16 / E;
+  const int vd0 = (kFp8 ? chunk : chunk ^ value_swap<DP>(tid / CPR)) * 16 / E;
+  const bool kinside = kd0 < D;
+  const int kd = kinside ? kd0 : 0, vd = vd0 < D ? vd0 : 0;
   const uint32_t koff = (kd / a.gk.pack) * (int32_t)a.gk.s_piece + (kd % a.gk.pack) * E;
+  const int vgroup8 = (tid % 8) ^ ((tid / 16) & 7);  // VT: 8 tokens of the step
   uint32_t voff[VT ? NVL : 1];
   if constexpr (VT) {
 #pragma unroll
@@ -154,7 +172,7 @@ attention_many_kernel(AttentionArgs a) {
       voff[l] = (d / a.gv.pack) * (int32_t)a.gv.s_piece + (d % a.gv.pack) * (int32_t)a.gv.s_inner;
     }
   } else {
-    voff[0] = (kd / a.gv.pack) * (int32_t)a.gv.s_piece + (kd % a.gv.pack) * E;
+    voff[0] = (vd / a.gv.pack) * (int32_t)a.gv.s_piece + (vd % a.gv.pack) * E;
   }
   const int64_t khead = kvh * a.gk.s_head, vhead = kvh * a.gv.s_head;
   float ks = 1.0f, vs = 1.0f;
@@ -209,39 +227,55 @@ attention_many_kernel(AttentionArgs a) {
   constexpr int kGroup = kWave / CPR;
   const uint32_t kgroup = koff + (uint32_t)((lane / CPR) * (int)a.gk.s_off);
   const uint32_t vgroup = voff[0] + (uint32_t)((lane / CPR) * (int)a.gv.s_off);
-  Raw<16> kreg[NL];
-  Raw<VLB> vreg[NVL];
-  auto load = [&](const Step &s) {
-    if (!s.some) return;
-    if constexpr (GROUPED) {
+  // f(l, address, offset) for this thread's key and value loads.
+  auto each_key = [&](const Step &s, auto f) {
 #pragma unroll
-      for (int l = 0; l < NL; ++l)
-        kreg[l] = global_load<16, false>(
-            address_of_lane(s.k, wave * kGroup + l * (kManyThreads / CPR)), kgroup);
-    } else {
-#pragma unroll
-      for (int l = 0; l < NL; ++l)
-        kreg[l] = global_load<16, false>(
-            from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), koff);
-    }
-    if constexpr (VT) {
-      const uint64_t p = from_lane(s.v, 32 * (tid % 8));
-#pragma unroll
-      for (int l = 0; l < NVL; ++l) vreg[l] = global_load<VLB, false>(p, voff[l]);
-    } else if constexpr (GROUPED) {
-#pragma unroll
-      for (int l = 0; l < NL; ++l)
-        vreg[l] = global_load<16, false>(
-            address_of_lane(s.v, wave * kGroup + l * (kManyThreads / CPR)), vgroup);
-    } else {
-#pragma unroll
-      for (int l = 0; l < NL; ++l)
-        vreg[l] = global_load<16, false>(
-            from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), voff[0]);
+    for (int l = 0; l < NL; ++l) {
+      if constexpr (GROUPED)
+        f(l, address_of_lane(s.k, wave * kGroup + l * (kManyThreads / CPR)), kgroup);
+      else
+        f(l, from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), koff);
     }
   };
-  // A 16-byte chunk of a cached row as one (16-bit) or two (FP8) chunks in LDS;
-  // `swap` is XORed to their numbers.
+  auto each_value = [&](const Step &s, auto f) {
+    if constexpr (VT) {
+      const uint64_t p = from_lane(s.v, 32 * vgroup8);
+#pragma unroll
+      for (int l = 0; l < NVL; ++l) f(l, p, voff[l]);
+    } else {
+#pragma unroll
+      for (int l = 0; l < NL; ++l) {
+        if constexpr (GROUPED)
+          f(l, address_of_lane(s.v, wave * kGroup + l * (kManyThreads / CPR)), vgroup);
+        else
+          f(l, from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), voff[0]);
+      }
+    }
+  };
+  struct Staged {
+    Raw<16> k[NL];
+    Raw<VLB> v[NVL];
+  };
+  auto load = [&](const Step &s) -> Staged {
+    Staged x{};
+    if (!s.some) return x;
+    each_key(s, [&](int l, uint64_t p, uint32_t o) { x.k[l] = global_load<16, false>(p, o); });
+    each_value(s, [&](int l, uint64_t p, uint32_t o) { x.v[l] = global_load<VLB, false>(p, o); });
+    return x;
+  };
+  // Straight into LDS, where nothing has to be changed on the way.
+  auto load_lds = [&](const Step &s, lds_char *to) {
+    to += wave * 1024;
+    each_key(s, [&](int l, uint64_t p, uint32_t o) { copy_to_lds(p, o, to + l * 4096); });
+    each_value(s, [&](int l, uint64_t p, uint32_t o) { copy_to_lds(p, o, to + TENSOR + l * 4096); });
+  };
+  // Whether all rows see all tokens of the step.
+  auto plain = [&](const Step &s, int base) {
+    return s.there == ~0ull && base >= last_lo && base + kManyStep <= first_hi;
+  };
+  // From registers: FP8 codes become elements, values of tokens that are not
+  // there, NaN and infinities of tokens that some rows do not see, and what is
+  // past a key's end become 0.
   auto put = [&](char *line, int swap, const Raw<16> &x) {
     if constexpr (kFp8) {
 #pragma unroll
@@ -252,55 +286,57 @@ attention_many_kernel(AttentionArgs a) {
         *reinterpret_cast<u32x4 *>(line + 16 * ((2 * chunk + i) ^ swap)) = o;
       }
     } else {
-      *reinterpret_cast<u32x4 *>(line + 16 * (chunk ^ swap)) = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+      *reinterpret_cast<u32x4 *>(line + 16 * chunk) = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
     }
   };
-  auto store = [&](const Step &s, int base, int buffer) {
-    char *kb = kbuf + buffer * TENSOR, *vb = vbuf + buffer * TENSOR;
-    const bool whole = s.there == ~0ull;
-    if (base < last_lo || base + kManyStep > first_hi) {  // some rows do not see some tokens
+  auto store = [&](const Step &s, Staged &staged, int base, int buffer) {
+    char *kb = lds + buffer * BUFFER, *vb = kb + TENSOR;
+    if (!plain(s, base)) {
       uint32_t odd = 0;
 #pragma unroll
-      for (int l = 0; l < NVL; ++l)
+      for (int l = 0; l < NVL; ++l) {
+        const uint32_t have =
+            VT ? (uint32_t)(s.there >> (8 * vgroup8)) & 0xFFu
+               : (uint32_t)(s.there >> (tid / CPR + l * (kManyThreads / CPR))) & 1u ? 0xFFu : 0u;
 #pragma unroll
         for (int w = 0; w < VLB / 4; ++w) {
-          odd |= not_finite<C>(vreg[l].w[w]);
-          vreg[l].w[w] = only_finite<C>(vreg[l].w[w]);
+          uint32_t keep;
+          if constexpr (!VT) keep = have ? ~0u : 0u;
+          else if constexpr (E == 2)
+            keep = ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
+                   ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
+          else
+            keep = ((have >> (4 * w)) & 1 ? 0xFFu : 0u) | ((have >> (4 * w)) & 2 ? 0xFF00u : 0u) |
+                   ((have >> (4 * w)) & 4 ? 0xFF0000u : 0u) |
+                   ((have >> (4 * w)) & 8 ? 0xFF000000u : 0u);
+          const uint32_t x = staged.v[l].w[w] & keep;
+          odd |= not_finite<C>(x);
+          staged.v[l].w[w] = only_finite<C>(x);
         }
+      }
       if (odd != 0) *infinities = 1;
     }
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
       const int at = tid / CPR + l * (kManyThreads / CPR);
-      Raw<16> x = kreg[l];
-      if (D != DP && !inside) x = Raw<16>{};
-      put(kb + at * ROW, key_swap<DP>(at), x);
+      put(kb + at * ROW, key_swap<DP>(at), D != DP && !kinside ? Raw<16>{} : staged.k[l]);
     }
     if constexpr (VT) {
-      const uint32_t have = (uint32_t)(s.there >> (8 * (tid % 8))) & 0xFFu;
 #pragma unroll
       for (int l = 0; l < NVL; ++l) {
-        const int e = tid / 8 + 32 * l;
         u32x4 o;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          if constexpr (kFp8) o[w] = widen<IO, C>(vreg[l].w[w / 2], w % 2);
-          else o[w] = vreg[l].w[w];
-          if (!whole)
-            o[w] &= ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
-                    ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u);
+          if constexpr (kFp8) o[w] = widen<IO, C>(staged.v[l].w[w / 2], w % 2);
+          else o[w] = staged.v[l].w[w];
         }
-        const int swap = (e / 2) % 16;
-        if (swap & 1) o = u32x4{o[2], o[3], o[0], o[1]};
-        *reinterpret_cast<u32x4 *>(vb + e * (kManyStep * 2) + 16 * ((tid % 8) ^ (swap / 2))) = o;
+        *reinterpret_cast<u32x4 *>(vb + 16 * (tid + l * kManyThreads)) = o;
       }
     } else {
 #pragma unroll
       for (int l = 0; l < NL; ++l) {
         const int at = tid / CPR + l * (kManyThreads / CPR);
-        Raw<16> x = vreg[l];
-        if (!whole && !((s.there >> at) & 1)) x = Raw<16>{};
-        put(vb + at * ROW, value_swap<DP>(at), x);
+        put(vb + at * ROW, value_swap<DP>(at), staged.v[l]);
       }
     }
     if constexpr (INDEXED) {
@@ -316,22 +352,28 @@ attention_many_kernel(AttentionArgs a) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x16{};
 
-  auto step = [&](const Step &now, int base, int buffer) {
+  auto step = [&](const Step &now, int base, int buffer, const lds_char *cur) {
     if (base >= any_hi || base + kManyStep <= any_lo || now.there == 0) return;
-    const char *kb = kbuf + buffer * TENSOR + c * ROW;
-    f32x16 s[2];
+    // Rows start at multiples of their length, so that the permutation is an
+    // exclusive or of the address.
+    const int kb = c * ROW + 16 * (h ^ key_swap<DP>(c));
+    f32x16 s[2] = {};
+    {
+      // The two halves in turn: their sums do not wait for each other.
+      auto key = [&](int i) -> Frag {
+        const u32x4 x = lds_read<u32x4>(cur + (kb ^ (32 * (i / 2))) + (i % 2) * 32 * ROW);
+        return {{x[0], x[1], x[2], x[3]}};
+      };
+      Frag k[kAhead];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = f32x16{};
+      for (int i = 0; i < kAhead; ++i) k[i] = key(i);
 #pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const u32x4 x = *reinterpret_cast<const u32x4 *>(kb + b * 32 * ROW +
-                                                         16 * ((2 * i + h) ^ key_swap<DP>(c)));
-        Frag k;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) k.w[w] = x[w];
-        s[b] = mma<IO>(k, q[i], s[b]);
+      for (int i = 0; i < 2 * KC; ++i) {
+        __builtin_amdgcn_sched_barrier(kMayCross);
+        s[i % 2] = mma<IO>(k[i % kAhead], q[i / 2], s[i % 2]);
+        if (i + kAhead < 2 * KC) k[i % kAhead] = key(i + kAhead);
       }
+      __builtin_amdgcn_sched_barrier(kMayCross);
     }
     const bool whole = now.there == ~0ull && base >= all_lo && base + kManyStep <= all_hi;
     float top = -INFINITY;
@@ -410,36 +452,46 @@ attention_many_kernel(AttentionArgs a) {
       for (int i = 0; i < 8; ++i)
         w[2 * b + i / 4].w[i % 4] = pair_of<IO>(s[b][2 * i], s[b][2 * i + 1]);
     }
-    const char *vb = vbuf + buffer * TENSOR;
     // Values of 16 tokens (in the weights' order) of element 32 j + c.
+    const int li = lane % 16;
+    const lds_char *values_at = cur + TENSOR;
+    const int vb = VT ? c * (kManyStep * 2) + 8 * h + 16 * ((c / 2) % 8)
+                      : (4 * h + li / 4) * ROW + 8 * (li % 2) +
+                            16 * ((2 * ((lane / 16) % 2) + (li % 4) / 2) ^ value_swap<DP>(li / 4));
     auto values = [&](int kk, int j) -> Frag {
       Frag f;
-      if constexpr (VT) {
-        // units of 4 tokens, permuted by the element
-        const char *line = vb + (32 * j + c) * (kManyStep * 2);
-        const int swap = (c / 2) % 16;
-        const u32x2 x = *reinterpret_cast<const u32x2 *>(line + 8 * ((4 * kk + h) ^ swap));
-        const u32x2 y = *reinterpret_cast<const u32x2 *>(line + 8 * ((4 * kk + 2 + h) ^ swap));
-        f.w[0] = x[0];
-        f.w[1] = x[1];
-        f.w[2] = y[0];
-        f.w[3] = y[1];
+      u32x2 x, y;
+      if constexpr (VT) {  // chunks of 8 tokens, permuted by the element
+        x = lds_read<u32x2>(values_at + (vb ^ (32 * kk)) + 32 * j * (kManyStep * 2));
+        y = lds_read<u32x2>(values_at + (vb ^ (32 * kk + 16)) + 32 * j * (kManyStep * 2));
       } else {
-        const int i = lane % 16, token = 16 * kk + 4 * h + i / 4;
-        const int piece = (4 * j + 2 * ((lane / 16) % 2) + (i % 4) / 2) ^ value_swap<DP>(i / 4);
-        const char *p = vb + token * ROW + 16 * piece + 8 * (i % 2);
-        const u32x2 x = lds_transposed(p), y = lds_transposed(p + 8 * ROW);
-        f.w[0] = x[0];
-        f.w[1] = x[1];
-        f.w[2] = y[0];
-        f.w[3] = y[1];
+        x = lds_transposed(values_at + (vb ^ (64 * j)) + 16 * kk * ROW);
+        y = lds_transposed(values_at + (vb ^ (64 * j)) + (16 * kk + 8) * ROW);
       }
+      f.w[0] = x[0];
+      f.w[1] = x[1];
+      f.w[2] = y[0];
+      f.w[3] = y[1];
       return f;
     };
+    Frag v[kAhead];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
+    for (int i = 0; i < kAhead; ++i) v[i] = values(i / NJ, i % NJ);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[j] = mma<IO>(values(kk, j), w[kk], acc[j]);
+    for (int i = 0; i < 4 * NJ; ++i) {
+      __builtin_amdgcn_sched_barrier(kMayCross);
+      acc[i % NJ] = mma<IO>(v[i % kAhead], w[i / NJ], acc[i % NJ]);
+      if (i + kAhead < 4 * NJ) v[i % kAhead] = values((i + kAhead) / NJ, (i + kAhead) % NJ);
+    }
+    __builtin_amdgcn_sched_barrier(kMayCross);
+  };
+
+  // The two buffers are told apart by the parameters' __restrict__: a transposing
+  // read would else wait for the loads into the other buffer.
+  auto turn = [&](const lds_char *__restrict__ cur, lds_char *__restrict__ other, const Step &now,
+                  const Step &next, int base, int buffer, bool direct) {
+    if (direct) load_lds(next, other);
+    step(now, base, buffer, cur);
   };
 
   if (tid == 0) *infinities = 0;
@@ -447,24 +499,29 @@ attention_many_kernel(AttentionArgs a) {
   if (from < to) {
     TokenEntry ahead = entries(from), after = entries(from + kManyStep);
     Step now = resolve(from, ahead);
-    load(now);
+    Staged staged = load(now);
     Step next = resolve(from + kManyStep, after);  // nothing there past `to`
-    store(now, from, 0);
+    store(now, staged, from, 0);
     __syncthreads();
     int buffer = 0;
     for (int base = from;; base += kManyStep) {
       const bool more = base + kManyStep < to;
+      const bool direct = !kFp8 && D == DP && plain(next, base + kManyStep);
       if (more) {
         ahead = entries(base + 2 * kManyStep);
-        load(next);
+        if constexpr (kFp8) staged = load(next);
       }
-      step(now, base, buffer);
+      turn((lds_char *)lds + buffer * BUFFER, (lds_char *)lds + (buffer ^ 1) * BUFFER, now, next,
+           base, buffer, direct && more);
       if (!more) break;
-      if constexpr (NB == 1) __syncthreads();
-      else buffer ^= 1;
-      store(next, base + kManyStep, buffer);
+      buffer ^= 1;
+      if (!direct) {
+        if constexpr (!kFp8) staged = load(next);
+        store(next, staged, base + kManyStep, buffer);
+      }
       now = next;
       next = resolve(base + 2 * kManyStep, ahead);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what went straight into LDS
       __syncthreads();
     }
   }
@@ -525,8 +582,13 @@ void launch_many(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hi
   auto go = [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
     constexpr int kDim = decltype(dp)::value;
     constexpr bool kIndexed = decltype(indexed_)::value;
-    attention_many_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed, decltype(grouped_)::value>
-        <<<b, kManyThreads, many_lds<kDim, kIndexed>(), s>>>(a);
+    constexpr size_t kLds = many_lds<kDim, kIndexed>();
+    const auto kernel =
+        attention_many_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed, decltype(grouped_)::value>;
+    if (kLds > 65536)  // more than a kernel has unasked
+      (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
+    kernel<<<b, kManyThreads, kLds, s>>>(a);
   };
   auto by_dim = [&](auto vt_, auto indexed_, auto grouped_) {
     if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_, grouped_);
