@@ -172,6 +172,57 @@ __device__ __forceinline__ uint64_t address_of_lane(uint64_t x, int lane) {
          (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), lane) << 32;
 }
 
+// K and V rows of kv head `kvh` for the tokens that a wave's lanes look up, one
+// each: every token of a step, or (blocks that hold whole groups of 16) the
+// first of a group, whose other rows follow from it.  Tokens that are not there
+// get another's rows, so that loads need no conditions.
+struct LaneRows {
+  uint64_t k, v;
+  uint64_t held;  // bit per lane whose token is there; none: k and v cannot be read
+  float ks, vs;   // block-indexed scales
+};
+
+template <bool INDEXED>
+__device__ __forceinline__ LaneRows lane_rows(const AttentionArgs &a, const TokenEntry &entry,
+                                              int at, bool looks, int kvh) {
+  LaneRows r{0, 0, 0, 1.0f, 1.0f};
+  TokenRows x{nullptr, nullptr, 0};
+  const bool held = looks && token_rows(a, entry, at, &x);
+  if (held) {
+    r.k = reinterpret_cast<uint64_t>(x.k + kvh * a.gk.s_head);
+    r.v = reinterpret_cast<uint64_t>(x.v + kvh * a.gv.s_head);
+    if constexpr (INDEXED) {
+      r.ks = scale_of(a.ks, x.block, kvh);
+      r.vs = scale_of(a.vs, x.block, kvh);
+    }
+  }
+  r.held = __ballot(held);
+  if (r.held != 0 && r.held != ~0ull) {
+    const int first = 4 * __builtin_ctzll(r.held);
+    const uint64_t k = from_lane(r.k, first), v = from_lane(r.v, first);
+    if (!held) {
+      r.k = k;
+      r.v = v;
+    }
+  }
+  return r;
+}
+
+// Bits [from - base, to - base) of a mask of tokens from `base` on, n <= 64 of them.
+__device__ __forceinline__ uint64_t tokens_between(int from, int to, int base, int n) {
+  const int lo = from > base ? from - base : 0, hi = to < base + n ? to - base : n;
+  if (lo >= hi) return 0;
+  const uint64_t below = hi >= 64 ? ~0ull : (1ull << hi) - 1;
+  return below & ~((1ull << lo) - 1);
+}
+
+// A bit for each of 4 groups of 16 tokens, as a bit for each token.
+__device__ __forceinline__ uint64_t group_tokens(uint32_t groups) {
+  return ((groups & 1) | (uint64_t)(groups & 2) << 15 | (uint64_t)(groups & 4) << 30 |
+          (uint64_t)(groups & 8) << 45) *
+         0xFFFFull;
+}
+
 // B bytes of global memory at an address that went through another lane, and so
 // is not known to be global.  A uniform address and a 32-bit offset make the
 // scalar form of the load, without a vector operation for the address.  NT:

@@ -123,7 +123,6 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     const int d0 = VT ? 16 * i + c : c * NV + i * (VLB / E), d = d0 < D ? d0 : 0;
     voff[i] = (d / a.gv.pack) * (int32_t)a.gv.s_piece + (d % a.gv.pack) * (int32_t)a.gv.s_inner;
   }
-  const int64_t khead = kvh * a.gk.s_head, vhead = kvh * a.gv.s_head;
   float ks = 1.0f, vs = 1.0f;
   if constexpr (kFp8 && !INDEXED) {
     ks = scale_of(a.ks, 0, kvh);
@@ -141,52 +140,45 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   const uint32_t krow = (uint32_t)(c * (int)a.gk.s_off);
   const uint32_t vrow = (uint32_t)(4 * g * (int)a.gv.s_off);
 
-  struct Step {
-    uint64_t k, v;      // rows of token `lane` (one that is not there: of another)
-    uint32_t there;     // bit per token that some row may see
-    bool some;          // k and v can be read
-    float ks, vs;
+  constexpr int kStride = kFewWaves * kFewStep;
+  // GROUPED: lane 2 i + b looks up the first token of half b of the wave's i-th
+  // step, so that one look serves 32 steps; else lane i looks up token i of one.
+  constexpr int kSteps = GROUPED ? 32 : 1;
+  auto token_of_lane = [&](int base) {
+    return GROUPED ? base + (lane / 2) * kStride + 16 * (lane % 2) : base + lane;
   };
-  // A step's table entries are loaded two steps ahead and looked at one step
-  // later.
+  auto looks = [&](int base) {
+    return token_of_lane(base) < to && (GROUPED || lane < kFewStep);
+  };
+  // Table entries are loaded one look ahead of their use.
   auto entries = [&](int base) -> TokenEntry {
     TokenEntry e{0, 0};
-    if (lane < kFewStep && base + lane < to) e = token_entry(a, t, base + lane);
+    if (looks(base)) e = token_entry(a, t, token_of_lane(base));
     return e;
   };
-  auto resolve = [&](int base, const TokenEntry &entry) -> Step {
-    Step s{0, 0, 0, false, 1.0f, 1.0f};
-    TokenRows r{nullptr, nullptr, 0};
-    const int at = base + lane;
-    const bool held = lane < kFewStep && at < to && token_rows(a, entry, at, &r);
-    if (held) {
-      s.k = reinterpret_cast<uint64_t>(r.k + khead);
-      s.v = reinterpret_cast<uint64_t>(r.v + vhead);
-      if constexpr (INDEXED) {
-        s.ks = scale_of(a.ks, r.block, kvh);
-        s.vs = scale_of(a.vs, r.block, kvh);
-      }
-    }
-    const uint64_t all = __ballot(held);
-    s.some = all != 0;
-    if (s.some && all != 0xFFFFFFFFull) {
-      // Tokens that are not there read another's rows, so that loads need no
-      // conditions.
-      const int first = 4 * __builtin_ctzll(all);
-      const uint64_t k = from_lane(s.k, first), v = from_lane(s.v, first);
-      if (!held) {
-        s.k = k;
-        s.v = v;
-      }
-    }
+  struct Step {
+    LaneRows rows;
+    int lane0;       // GROUPED: the lane of its first half
+    uint32_t there;  // bit per token that some row may see
+  };
+  auto step_at = [&](const LaneRows &rows, int base, int lane0) -> Step {
     // Tokens in front of a window are of the block, but nobody's: they may hold
     // anything.
-    s.there = (uint32_t)__ballot(held && at >= lo);
-    return s;
+    const uint32_t in = (uint32_t)tokens_between(lo, to, base, kFewStep);
+    const uint32_t held =
+        GROUPED ? (uint32_t)group_tokens((uint32_t)(rows.held >> lane0) & 3u) : (uint32_t)rows.held;
+    return {rows, lane0, held & in};
+  };
+  auto look = [&](int base, const TokenEntry &entry) {
+    return lane_rows<INDEXED>(a, entry, token_of_lane(base), looks(base), kvh);
+  };
+  // A token's scale, of the eight that the lane has.
+  auto token_scale = [&](const Step &s, float x, int e) {
+    return GROUPED ? from_lane(x, 4 * (s.lane0 + e / 4)) : from_lane(x, 16 * g + 4 * place_of(e));
   };
   uint32_t kw[2][KL][4];
   auto load_keys = [&](const Step &s) {
-    if (!s.some) return;
+    if (s.rows.held == 0) return;
     auto one = [&](int b, uint64_t p, uint32_t row) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
@@ -197,21 +189,23 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     };
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      if constexpr (GROUPED) one(b, address_of_lane(s.k, 16 * b), krow);
-      else one(b, from_lane(s.k, 4 * c + 64 * b), 0);
+      if constexpr (GROUPED) one(b, address_of_lane(s.rows.k, s.lane0 + b), krow);
+      else one(b, from_lane(s.rows.k, 4 * c + 64 * b), 0);
     }
   };
   // Rows: [token e][dword]; VT: [half b][element j][dword].
   uint32_t vw[VT ? 2 * NV : 8][VT ? E : VW];
   auto load_values = [&](const Step &s) {
-    if (!s.some) return;
+    if (s.rows.held == 0) return;
     if constexpr (VT) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const uint64_t p = from_lane(s.v, 16 * g + 64 * b);
+        uint64_t p;
+        if constexpr (GROUPED) p = address_of_lane(s.rows.v, s.lane0 + b);
+        else p = from_lane(s.rows.v, 16 * g + 64 * b);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const Raw<VLB> r = global_load<VLB, true>(p, voff[j]);
+          const Raw<VLB> r = global_load<VLB, true>(p, (GROUPED ? 4 * g * E : 0) + voff[j]);
 #pragma unroll
           for (int w = 0; w < E; ++w) vw[b * NV + j][w] = r.w[w];
         }
@@ -228,8 +222,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (GROUPED)
-          one(e, address_of_lane(s.v, 4 * (e - e % 4)) + (e % 4) * a.gv.s_off, vrow);
-        else one(e, from_lane(s.v, 16 * g + 4 * place_of(e)), 0);
+          one(e, address_of_lane(s.rows.v, s.lane0 + e / 4) + (e % 4) * a.gv.s_off, vrow);
+        else one(e, from_lane(s.rows.v, 16 * g + 4 * place_of(e)), 0);
       }
     }
   };
@@ -261,13 +255,24 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   };
 
   int base = from + wave * kFewStep;
-  constexpr int kStride = kFewWaves * kFewStep;
   if (base < to) {
-    TokenEntry ahead = entries(base), after = entries(base + kStride);
-    Step now = resolve(base, ahead);
+    // The step after this one, from rows that serve kSteps steps; past `to`
+    // nothing is there.
+    LaneRows rows = look(base, entries(base));
+    Step now = step_at(rows, base, 0);
     load_keys(now);
     load_values(now);
-    Step next = resolve(base + kStride, after);  // nothing there past `to`
+    TokenEntry ahead = entries(base + kSteps * kStride);
+    int count = 0;
+    auto advance = [&](int at) -> Step {
+      count = (count + 1) % kSteps;
+      if (count == 0) {
+        rows = look(at, ahead);
+        ahead = entries(at + kSteps * kStride);
+      }
+      return step_at(rows, at, 2 * count);
+    };
+    Step next = advance(base + kStride);
     for (;;) {
       if (D != DP) {  // pieces past the head's end
 #pragma unroll
@@ -300,17 +305,14 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         }
       }
       const bool more = base + kStride < to;
-      if (more) {
-        ahead = entries(base + 2 * kStride);
-        load_keys(next);
-      }
+      if (more) load_keys(next);
 
       const bool whole = now.there == 0xFFFFFFFFu && base >= last_lo && base + kFewStep <= first_hi;
       float x[8], p[8], top = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[e] = s[e / 4][e % 4];
-        if constexpr (INDEXED) x[e] *= from_lane(now.ks, 16 * g + 4 * place_of(e));
+        if constexpr (INDEXED) x[e] *= token_scale(now, now.rows.ks, e);
       }
       if (a.cap != 0.0f) {
 #pragma unroll
@@ -347,7 +349,10 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       if constexpr (INDEXED) {
         // Values stay codes; weights carry the tokens' scales, relative to the
         // largest so far, so that they stay in the type's range.
-        float mine = lane < kFewStep && ((now.there >> lane) & 1) ? fabsf(now.vs) : 0.0f;
+        const int in = GROUPED ? lane - now.lane0 : lane;
+        const bool mine_there = in >= 0 && in < (GROUPED ? 2 : kFewStep) &&
+                                ((now.rows.held >> lane) & 1);
+        float mine = mine_there ? fabsf(now.rows.vs) : 0.0f;
 #pragma unroll
         for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
         if (mine > vref) {
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         const float inv = vref > 0.0f ? 1.0f / vref : 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          p[e] *= from_lane(now.vs, 16 * g + 4 * place_of(e)) * inv;
+          p[e] *= token_scale(now, now.rows.vs, e) * inv;
       }
       Frag w;
 #pragma unroll
@@ -412,7 +417,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       load_values(next);
       now = next;
       base += kStride;
-      next = resolve(base + kStride, ahead);
+      next = advance(base + kStride);
     }
   }
   l += __shfl_xor(l, 16);

@@ -174,7 +174,6 @@ attention_many_kernel(AttentionArgs a) {
   } else {
     voff[0] = (vd / a.gv.pack) * (int32_t)a.gv.s_piece + (vd % a.gv.pack) * E;
   }
-  const int64_t khead = kvh * a.gk.s_head, vhead = kvh * a.gv.s_head;
   float ks = 1.0f, vs = 1.0f;
   if constexpr (kFp8 && !INDEXED) {
     ks = scale_of(a.ks, 0, kvh);
@@ -182,44 +181,29 @@ attention_many_kernel(AttentionArgs a) {
   }
   const float scale = positive_scale<IO>(a, ks, q);
 
-  struct Step {
-    uint64_t k, v;  // rows of token `lane` (one that is not there: of another)
-    uint64_t there;
-    float ks, vs;
-    bool some;
-  };
-  // A step's table entries are loaded two steps ahead and looked at one step
-  // later.
+  // GROUPED: lane i looks up the first token of the i-th group of 16, so that one
+  // look serves 16 steps; else lane i looks up token i of one step.
+  constexpr int kSteps = GROUPED ? 16 : 1;
+  auto token_of_lane = [&](int base) { return base + (GROUPED ? 16 * lane : lane); };
+  // Table entries are loaded one look ahead of their use.
   auto entries = [&](int base) -> TokenEntry {
     TokenEntry e{0, 0};
-    if (base + lane < to) e = token_entry(a, t, base + lane);
+    if (token_of_lane(base) < to) e = token_entry(a, t, token_of_lane(base));
     return e;
   };
-  auto resolve = [&](int base, const TokenEntry &entry) -> Step {
-    Step s{0, 0, 0, 1.0f, 1.0f, false};
-    TokenRows x{nullptr, nullptr, 0};
-    const int at = base + lane;
-    const bool held = at < to && token_rows(a, entry, at, &x);
-    if (held) {
-      s.k = reinterpret_cast<uint64_t>(x.k + khead);
-      s.v = reinterpret_cast<uint64_t>(x.v + vhead);
-      if constexpr (INDEXED) {
-        s.ks = scale_of(a.ks, x.block, kvh);
-        s.vs = scale_of(a.vs, x.block, kvh);
-      }
-    }
-    const uint64_t all = __ballot(held);
-    s.some = all != 0;
-    if (s.some && all != ~0ull) {  // tokens that are not there read another's rows
-      const int first = 4 * __builtin_ctzll(all);
-      const uint64_t k = from_lane(s.k, first), v = from_lane(s.v, first);
-      if (!held) {
-        s.k = k;
-        s.v = v;
-      }
-    }
-    s.there = __ballot(held && at >= lo);  // slots in front of a window hold anything
-    return s;
+  struct Step {
+    LaneRows rows;
+    int lane0;       // GROUPED: the lane of its first group
+    uint64_t there;  // bit per token that some row may see
+  };
+  auto step_at = [&](const LaneRows &rows, int base, int lane0) -> Step {
+    // slots in front of a window hold anything
+    const uint64_t held = GROUPED ? group_tokens((uint32_t)(rows.held >> lane0) & 15u) : rows.held;
+    return {rows, lane0, held & tokens_between(lo, to, base, kManyStep)};
+  };
+  auto look = [&](int base, const TokenEntry &entry) {
+    const int at = token_of_lane(base);
+    return lane_rows<INDEXED>(a, entry, at, at < to, kvh);
   };
 
   // GROUPED: a wave's load takes kGroup tokens of one block, from one scalar
@@ -228,28 +212,32 @@ attention_many_kernel(AttentionArgs a) {
   const uint32_t kgroup = koff + (uint32_t)((lane / CPR) * (int)a.gk.s_off);
   const uint32_t vgroup = voff[0] + (uint32_t)((lane / CPR) * (int)a.gv.s_off);
   // f(l, address, offset) for this thread's key and value loads.
-  auto each_key = [&](const Step &s, auto f) {
+  auto each_row = [&](const Step &s, uint64_t rows, int64_t s_off, uint32_t in_group,
+                      uint32_t alone, auto f) {
 #pragma unroll
     for (int l = 0; l < NL; ++l) {
+      constexpr int kLoad = kManyThreads / CPR;  // tokens of the workgroup's load
+      const int at = wave * kGroup + l * kLoad;  // the wave's first
       if constexpr (GROUPED)
-        f(l, address_of_lane(s.k, wave * kGroup + l * (kManyThreads / CPR)), kgroup);
+        f(l, address_of_lane(rows, s.lane0 + at / 16) + (at % 16) * s_off, in_group);
       else
-        f(l, from_lane(s.k, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), koff);
+        f(l, from_lane(rows, 4 * (at + lane / CPR)), alone);
     }
+  };
+  auto each_key = [&](const Step &s, auto f) {
+    each_row(s, s.rows.k, a.gk.s_off, kgroup, koff, f);
   };
   auto each_value = [&](const Step &s, auto f) {
     if constexpr (VT) {
-      const uint64_t p = from_lane(s.v, 32 * vgroup8);
+      uint64_t p;
+      if constexpr (GROUPED)
+        p = from_lane(s.rows.v, 4 * (s.lane0 + vgroup8 / 2)) + (vgroup8 % 2) * (8 * E);
+      else
+        p = from_lane(s.rows.v, 32 * vgroup8);
 #pragma unroll
       for (int l = 0; l < NVL; ++l) f(l, p, voff[l]);
     } else {
-#pragma unroll
-      for (int l = 0; l < NL; ++l) {
-        if constexpr (GROUPED)
-          f(l, address_of_lane(s.v, wave * kGroup + l * (kManyThreads / CPR)), vgroup);
-        else
-          f(l, from_lane(s.v, 4 * (tid / CPR) + l * (4 * kManyThreads / CPR)), voff[0]);
-      }
+      each_row(s, s.rows.v, a.gv.s_off, vgroup, voff[0], f);
     }
   };
   struct Staged {
@@ -258,7 +246,7 @@ attention_many_kernel(AttentionArgs a) {
   };
   auto load = [&](const Step &s) -> Staged {
     Staged x{};
-    if (!s.some) return x;
+    if (s.rows.held == 0) return x;
     each_key(s, [&](int l, uint64_t p, uint32_t o) { x.k[l] = global_load<16, false>(p, o); });
     each_value(s, [&](int l, uint64_t p, uint32_t o) { x.v[l] = global_load<VLB, false>(p, o); });
     return x;
@@ -339,10 +327,10 @@ attention_many_kernel(AttentionArgs a) {
         put(vb + at * ROW, value_swap<DP>(at), staged.v[l]);
       }
     }
-    if constexpr (INDEXED) {
+    if constexpr (INDEXED && !GROUPED) {
       if (wave == 0) {
-        scales[(2 * buffer) * kManyStep + lane] = s.ks;
-        scales[(2 * buffer + 1) * kManyStep + lane] = s.vs;
+        scales[(2 * buffer) * kManyStep + lane] = s.rows.ks;
+        scales[(2 * buffer + 1) * kManyStep + lane] = s.rows.vs;
       }
     }
   };
@@ -352,6 +340,17 @@ attention_many_kernel(AttentionArgs a) {
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x16{};
 
+  // The scales of tokens 32 b + 8 i + 4 h .. + 3 of a step.
+  auto token_scales = [&](const Step &s, float x, int buffer, int which, int b, int i) -> f32x4 {
+    if constexpr (GROUPED) {
+      const float y = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(x),
+                                                                  s.lane0 + 2 * b + i / 2));
+      return f32x4{y, y, y, y};
+    } else {
+      return *reinterpret_cast<const f32x4 *>(scales + (2 * buffer + which) * kManyStep + 32 * b +
+                                              8 * i + 4 * h);
+    }
+  };
   auto step = [&](const Step &now, int base, int buffer, const lds_char *cur) {
     if (base >= any_hi || base + kManyStep <= any_lo || now.there == 0) return;
     // Rows start at multiples of their length, so that the permutation is an
@@ -382,8 +381,7 @@ attention_many_kernel(AttentionArgs a) {
       if constexpr (INDEXED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4 *>(
-              scales + 2 * buffer * kManyStep + 32 * b + 8 * i + 4 * h);
+          const f32x4 x = token_scales(now, now.rows.ks, buffer, 0, b, i);
 #pragma unroll
           for (int w = 0; w < 4; ++w) s[b][4 * i + w] *= x[w];
         }
@@ -417,7 +415,10 @@ attention_many_kernel(AttentionArgs a) {
     const float shift = m == -INFINITY ? 0.0f : m;
     float inv = 1.0f;
     if constexpr (INDEXED) {
-      float mine = (now.there >> lane) & 1 ? fabsf(now.vs) : 0.0f;
+      const int in = GROUPED ? lane - now.lane0 : lane;
+      const bool mine_there =
+          in >= 0 && in < (GROUPED ? 4 : kManyStep) && ((now.rows.held >> lane) & 1);
+      float mine = mine_there ? fabsf(now.rows.vs) : 0.0f;
 #pragma unroll
       for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
       if (mine > vref) {
@@ -442,8 +443,7 @@ attention_many_kernel(AttentionArgs a) {
       if constexpr (INDEXED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4 *>(
-              scales + (2 * buffer + 1) * kManyStep + 32 * b + 8 * i + 4 * h);
+          const f32x4 x = token_scales(now, now.rows.vs, buffer, 1, b, i);
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[b][4 * i + k] *= x[k] * inv;
         }
@@ -497,18 +497,29 @@ attention_many_kernel(AttentionArgs a) {
   if (tid == 0) *infinities = 0;
   __syncthreads();
   if (from < to) {
-    TokenEntry ahead = entries(from), after = entries(from + kManyStep);
-    Step now = resolve(from, ahead);
+    // The step after this one, from rows that serve kSteps steps; past `to`
+    // nothing is there.
+    LaneRows rows = look(from, entries(from));
+    Step now = step_at(rows, from, 0);
     Staged staged = load(now);
-    Step next = resolve(from + kManyStep, after);  // nothing there past `to`
+    TokenEntry ahead = entries(from + kSteps * kManyStep);
+    int count = 0;
+    auto advance = [&](int at) -> Step {
+      count = (count + 1) % kSteps;
+      if (count == 0) {
+        rows = look(at, ahead);
+        ahead = entries(at + kSteps * kManyStep);
+      }
+      return step_at(rows, at, 4 * count);
+    };
     store(now, staged, from, 0);
+    Step next = advance(from + kManyStep);
     __syncthreads();
     int buffer = 0;
     for (int base = from;; base += kManyStep) {
       const bool more = base + kManyStep < to;
       const bool direct = !kFp8 && D == DP && plain(next, base + kManyStep);
       if (more) {
-        ahead = entries(base + 2 * kManyStep);
         if constexpr (kFp8) staged = load(next);
       }
       turn((lds_char *)lds + buffer * BUFFER, (lds_char *)lds + (buffer ^ 1) * BUFFER, now, next,
@@ -520,7 +531,7 @@ attention_many_kernel(AttentionArgs a) {
         store(next, staged, base + kManyStep, buffer);
       }
       now = next;
-      next = resolve(base + 2 * kManyStep, ahead);
+      next = advance(base + 2 * kManyStep);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // what went straight into LDS
       __syncthreads();
     }
