@@ -5,11 +5,13 @@
 // Rows.  A kv head's query rows are its `group` query heads at each new token.
 // A workgroup takes a tile of them: `tile_tokens` tokens by `tile_heads` heads
 // (the group, or a part of one wider than the tile), all of which read the
-// same keys and values.  Tiles are numbered without knowing each sequence's
-// length on the host: sequence s starts at tile begin(s) / tile_tokens + s,
-// begin(s) its first row.  That leaves every sequence room for its
-// ceil(n / tile_tokens) tiles, at most one of them unused.  A kernel that takes
-// only sequences of a few rows gives each sequence the same number of tiles.
+// same keys and values.  The host knows only how many tiles there can be; each
+// workgroup counts those of the sequences before its own (of the sequences that
+// its kernel takes), so that the ones that are left over lie together.
+// Scattered among the others they would cost far more than their own time:
+// workgroups go round the machine in order, and a part of it would get all of
+// them and run empty (64 sequences of 4 drafts at
+// 2048 tokens: 155 us instead of 99).
 //
 // Splits.  Where the tiles alone do not fill the machine, a tile's tokens are
 // divided among `splits` workgroups.  Each writes its unnormalised sum, its
@@ -62,7 +64,6 @@ struct AttentionArgs {
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
   int32_t splits;
   int32_t split_steps;  // least steps of 64 tokens in a split
-  int32_t seq_tiles;  // tiles of every sequence; 0: numbered as above
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
   float *part_ml;     // the same without head_dim: (maximum, sum of weights)
@@ -106,6 +107,54 @@ __device__ __forceinline__ int last_sequence(int seqs, const F &before) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// The sequence and rows of a tile, or false behind the last one.  A lane counts
+// the tiles of four sequences, whose sums the wave scans.
+__device__ __forceinline__ bool find_rows(const AttentionArgs &a, int tile, QueryTile *t) {
+  constexpr int kEach = 4;
+  const int lane = (int)(threadIdx.x % kWave);
+  int left = tile;  // behind the tiles counted so far
+  for (int s0 = 0; s0 < a.seqs; s0 += kEach * kWave) {
+    const int s = s0 + kEach * lane;
+    int64_t begin[kEach + 1];
+    int count[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i <= kEach; ++i) begin[i] = query_begin(a, min(s + i, a.seqs));
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int64_t n = begin[i + 1] - begin[i];
+      const bool mine = n > 0 && n >= a.least_rows && n <= a.most_rows;
+      count[i] = mine ? (int)((uint32_t)(n + a.tile_tokens - 1) / (uint32_t)a.tile_tokens) : 0;
+      sum += count[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+      const int x = __shfl_up(upto, d);
+      upto += lane >= d ? x : 0;
+    }
+    const int from = __builtin_amdgcn_readfirstlane(__popcll(__ballot(upto <= left)));
+    if (from < kWave) {
+      left -= __builtin_amdgcn_readlane(upto - sum, from);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int c = __builtin_amdgcn_readlane(count[i], from);
+        if (left < c) {
+          const int b = __builtin_amdgcn_readlane((int)begin[i], from);
+          t->seq = s0 + kEach * from + i;
+          t->begin = b;
+          t->rows = __builtin_amdgcn_readlane((int)begin[i + 1], from) - b;
+          t->first = left * a.tile_tokens;
+          t->count = min(a.tile_tokens, t->rows - t->first);
+          return true;
+        }
+        left -= c;
+      }
+    }
+    left -= __builtin_amdgcn_readlane(upto, kWave - 1);
+  }
+  return false;
+}
+
 // The tile with number `tile`, or false where it has no rows or another
 // kernel takes its sequence.  Uniform over the wave, all of whose lanes call.
 __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, QueryTile *t) {
@@ -115,19 +164,8 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
     t->count = 1;
     t->begin = tile;
     t->rows = 1;
-  } else {
-    const int lo = a.seq_tiles > 0 ? tile / a.seq_tiles : last_sequence(a.seqs, [&](int q) {
-      return query_begin(a, q) / a.tile_tokens + q <= (int64_t)tile;
-    });
-    const int64_t b = query_begin(a, lo), e = query_begin(a, lo + 1);
-    const int64_t j = tile - (a.seq_tiles > 0 ? (int64_t)lo * a.seq_tiles : b / a.tile_tokens + lo);
-    const int64_t n = e > b ? e - b : 0;
-    if (j < 0 || j * a.tile_tokens >= n || n < a.least_rows || n > a.most_rows) return false;
-    t->seq = lo;
-    t->begin = b;
-    t->rows = (int32_t)n;
-    t->first = (int32_t)j * a.tile_tokens;
-    t->count = min(a.tile_tokens, t->rows - t->first);
+  } else if (!find_rows(a, tile, t)) {
+    return false;
   }
   t->length = index_at(a.lens, a.lens64, t->seq);
   int64_t hold, first;

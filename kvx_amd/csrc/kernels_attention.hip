@@ -2,6 +2,8 @@
 // joins the splits of a tile.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "attention.h"
 #include "kvx_internal.h"
 
@@ -9,7 +11,7 @@ namespace kvx {
 namespace dev {
 namespace {
 
-constexpr int kJoinThreads = 256;
+constexpr int kMostSplits = 256;
 
 // Rows that have partial sums.
 __host__ __device__ __forceinline__ int64_t join_rows(const AttentionArgs &a) {
@@ -18,16 +20,18 @@ __host__ __device__ __forceinline__ int64_t join_rows(const AttentionArgs &a) {
 
 // Adds up the splits of one row and head: with M the largest maximum,
 //   out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
-// One wave has a row and head; the splits' partial sums are adjacent.
-template <int IO>
+// A workgroup has a row and head.  Its threads weigh one split each, then take
+// VEC elements of every G-th split, G as many as fit beside each other, and add
+// the G sums up through LDS: loads of many splits are in flight at once.
+template <int IO, int VEC, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionArgs a) {
-  const int lane = (int)(threadIdx.x % kWave);
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+  __shared__ float weights[kJoinThreads];  // of the splits; < 0: nothing was written for it
+  __shared__ float waves[2][kJoinThreads / kWave];
+  __shared__ float sums[kJoinThreads * VEC];
+  const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int hq = a.heads * a.group;
-  const int64_t unit = (int64_t)blockIdx.x * (kJoinThreads / kWave) + wave;
-  if (unit >= join_rows(a) * hq) return;
-  const int64_t part = unit / hq;
-  const int head = (int)(unit - part * hq);
+  const int64_t part = blockIdx.x / (uint32_t)hq;
+  const int head = (int)(blockIdx.x % (uint32_t)hq);
   int64_t row = part;
   if (a.qptr != nullptr) {
     const int s = a.part_rows > 0 ? (int)(part / a.part_rows)
@@ -39,32 +43,58 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionA
     if (row < b || row >= b + n || n < a.least_rows || n > a.most_rows) return;
   }
   const int64_t at = (part * hq + head) * a.splits;
-  float top = -INFINITY;
-  for (int z = lane; z < a.splits; z += kWave) top = fmaxf(top, a.part_ml[2 * (at + z)]);
+  const bool split = tid < a.splits;
+  const float m = split ? a.part_ml[2 * (at + tid)] : -INFINITY;
+  const float l = split ? a.part_ml[2 * (at + tid) + 1] : 0.0f;
+  float top = m;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float total = 0.0f, sum[8] = {};
-  for (int z = 0; z < a.splits; ++z) {
-    const float l = a.part_ml[2 * (at + z) + 1];
-    if (l == 0.0f) continue;  // nothing was written for it
-    const float w = exp2f(a.part_ml[2 * (at + z)] - base);
-    total += w * l;
+  if (lane == 0) waves[0][wave] = top;
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int d = lane + j * kWave;
-      if (d < a.head_dim) sum[j] = fmaf(w, a.part_o[(at + z) * a.head_dim + d], sum[j]);
-    }
-  }
+  for (int i = 0; i < kJoinThreads / kWave; ++i) top = fmaxf(top, waves[0][i]);
+  const float w = l == 0.0f ? -1.0f : exp2f(m - (top == -INFINITY ? 0.0f : top));
+  weights[tid] = w;
+  float total = l == 0.0f ? 0.0f : w * l;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) total += __shfl_xor(total, d);
+  if (lane == 0) waves[1][wave] = total;
+  __syncthreads();
+  total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / kWave; ++i) total += waves[1][i];
   const bool none = top == -INFINITY && total == 0.0f;
+
+  const int columns = a.head_dim / VEC;
+  int across = 1;  // threads of a split
+  while (across < columns && across < kJoinThreads) across *= 2;
+  const int g = tid / across, groups = kJoinThreads / across;
+  for (int c0 = 0; c0 < columns; c0 += across) {
+    const int c = c0 + tid % across;
+    float sum[VEC] = {};
+    if (c < columns) {
+#pragma unroll 4
+      for (int z = g; z < a.splits; z += groups) {
+        const float by = weights[z];
+        const Raw<4 * VEC> x =
+            ld<4 * VEC>(reinterpret_cast<const char *>(a.part_o + (at + z) * a.head_dim + c * VEC));
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int d = lane + j * kWave;
-    if (d < a.head_dim)
-      store_out<IO>(a.out + row * a.o_tok + head * a.o_head + (int64_t)d * bytes_of_type<IO>(),
-                    none ? 0.0f : sum[j] / total);
+        for (int j = 0; j < VEC; ++j) sum[j] = by < 0.0f ? sum[j] : fmaf(by, __uint_as_float(x.w[j]), sum[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sums[tid * VEC + j] = sum[j];
+    __syncthreads();
+    for (int d = tid; d < across * VEC && c0 * VEC + d < a.head_dim; d += kJoinThreads) {
+      float x = 0.0f;
+      for (int i = 0; i < groups; ++i) x += sums[i * across * VEC + d];
+      store_out<IO>(a.out + row * a.o_tok + head * a.o_head +
+                        (int64_t)(c0 * VEC + d) * bytes_of_type<IO>(),
+                    none ? 0.0f : x / total);
+    }
+    __syncthreads();
   }
-  if (lane == 0 && a.lse != nullptr)
+  if (tid == 0 && a.lse != nullptr)
     a.lse[row * hq + head] = none ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
@@ -101,30 +131,41 @@ void tile_rows(AttentionArgs *a, int rows) {
   a->tile_heads = a->group < rows ? a->group : rows;
   a->head_tiles = (a->group + a->tile_heads - 1) / a->tile_heads;
   a->tile_tokens = rows / a->tile_heads;
-  a->seq_tiles = 0;
   a->tiles = a->qptr != nullptr ? a->tokens / a->tile_tokens + a->seqs : a->seqs;
 }
 
-// Workgroups that share a tile's tokens, so that about `target` workgroups
-// run, each with at least `least` tokens of the longest sequence.
+enum Kind { kRows, kFew, kMany };
+
+// Workgroups that share a tile's tokens.  The machine holds about 512 at once;
+// with fewer tiles, each is divided until they fill it, into four parts or more
+// of `least` tokens: starting a workgroup and joining its sums takes as long.
+// With many rows the sums are large, and parts are short only where there are
+// few tiles (8 kv heads, us, whole and in parts of 128: one chunk of 100 tokens
+// at 1000 tokens 37 and 25, of 512 at 512 24 and 35).
+// Sequences of different lengths even out over a few rounds of workgroups, so
+// that parts of 2048 tokens at least are made for up to 3072 of them (5
+// sequences of 16384 to 32768 tokens: 97 us at 512 workgroups, 86 at 640).
 // `rows`: rows of partial sums per query head.
-void split_tokens(const AttentionPlan &p, AttentionArgs *a, int64_t target, int64_t least,
-                  int64_t rows) {
-  const int64_t tiles = a->qptr == nullptr ? a->seqs
-                        : a->seq_tiles > 0 ? (int64_t)a->seqs * a->seq_tiles
-                                           : (a->tokens + a->tile_tokens - 1) / a->tile_tokens;
-  const int64_t units = tiles * a->heads * a->head_tiles;
-  const int64_t tokens = longest(p);
-  int64_t n = target / (units > 0 ? units : 1);
-  if (n > tokens / least) n = tokens / least;
+void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t rows) {
+  // about as many tiles as there are: sequences that another kernel takes are
+  // the short ones where `least_rows` says so
+  int64_t tiles = a->qptr == nullptr ? a->seqs : a->tokens / a->tile_tokens;
+  if (a->least_rows == 0) tiles = std::max<int64_t>(tiles, a->seqs);
+  tiles = std::min<int64_t>(tiles, a->tiles);
+  const int64_t units = std::max<int64_t>(tiles * a->heads * a->head_tiles, 1);
+  int64_t tokens = longest(p);  // that a tile sees
+  if (a->causal && a->window > 0)
+    tokens = std::min(tokens, (int64_t)a->window + a->tile_tokens);
+  const int64_t least =
+      kind == kMany ? std::min<int64_t>(std::max<int64_t>(4 * units, 128), 512) : 256;
+  int64_t n = tokens < 4 * least ? 1 : std::min(512 / units, tokens / least);
+  if (kind != kMany) n = std::max(n, std::min(3072 / units, tokens / 2048));
   // partial sums of at most 1 GiB
   const int64_t each = rows * a->heads * a->group * (a->head_dim + 2) * 4;
   if (n * each > ((int64_t)1 << 30)) n = ((int64_t)1 << 30) / each;
-  a->splits = (int)(n < 1 ? 1 : n > 256 ? 256 : n);
+  a->splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
   a->split_steps = (int)((tokens + 64 * (int64_t)a->splits - 1) / (64 * (int64_t)a->splits));
 }
-
-enum Kind { kRows, kFew, kMany };
 
 // Up to two launches: sequences of few and of many new tokens.
 struct Plan {
@@ -259,24 +300,24 @@ Plan make_plan(const AttentionPlan &p) {
     AttentionArgs &x = add(kRows, a);
     tile_rows(&x, kRowTile);
     x.chunk_k = chunks(p, g.gk, g.src_k, 4);
-    split_tokens(p, &x, 1024, 256, x.tokens);
+    split_tokens(p, &x, kRows, x.tokens);
   } else if (all_few || !many_ok) {
     AttentionArgs &x = add(kFew, a);
     tile_rows(&x, kRowTile);
-    split_tokens(p, &x, 3072, 512, x.tokens);
+    split_tokens(p, &x, kFew, x.tokens);
   } else {
     AttentionArgs &x = add(kMany, a);
     tile_rows(&x, kManyRowTile);
     if (!all_many) x.least_rows = few + 1;
-    split_tokens(p, &x, 512, 512, x.tokens);
+    split_tokens(p, &x, kMany, x.tokens);
     if (!all_many) {
       AttentionArgs &y = add(kFew, a);
       tile_rows(&y, kRowTile);
       y.most_rows = few;
       y.part_rows = few;
-      y.seq_tiles = (few + y.tile_tokens - 1) / y.tile_tokens;
-      y.tiles = y.seqs * y.seq_tiles;
-      split_tokens(p, &y, 3072, 512, (int64_t)y.seqs * few);
+      const int64_t most = (int64_t)y.seqs * ((few + y.tile_tokens - 1) / y.tile_tokens);
+      y.tiles = (int)std::min<int64_t>(y.tiles, most);
+      split_tokens(p, &y, kFew, (int64_t)y.seqs * few);
     }
   }
   for (int i = 0; i < r.parts; ++i) {
@@ -290,11 +331,17 @@ Plan make_plan(const AttentionPlan &p) {
   return r;
 }
 
+// Few splits are joined by one wave a row and head, many by four.
 template <int IO>
 void launch_join(const AttentionArgs &a, hipStream_t s) {
-  const int64_t units = join_rows(a) * a.heads * a.group;
-  const int64_t waves = kJoinThreads / kWave;
-  attention_join_kernel<IO><<<dim3((uint32_t)((units + waves - 1) / waves)), kJoinThreads, 0, s>>>(a);
+  const dim3 units((uint32_t)(join_rows(a) * a.heads * a.group));
+  auto go = [&](auto vec) {
+    constexpr int kVec = decltype(vec)::value;
+    if (a.splits <= 16) attention_join_kernel<IO, kVec, 64><<<units, 64, 0, s>>>(a);
+    else attention_join_kernel<IO, kVec, kMostSplits><<<units, kMostSplits, 0, s>>>(a);
+  };
+  if (a.head_dim % 4 == 0) go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 1>{});
 }
 
 int64_t workgroups(const AttentionArgs &a) {
@@ -304,7 +351,7 @@ int64_t workgroups(const AttentionArgs &a) {
 bool launchable(const Plan &p) {
   for (int i = 0; i < p.parts; ++i) {
     const AttentionArgs &a = p.part[i].a;
-    if (join_rows(a) * a.heads * a.group * kWave > 0xFFFFFF00ll) return false;
+    if (a.splits > 1 && join_rows(a) * a.heads * a.group * kMostSplits > 0xFFFFFF00ll) return false;
     if (workgroups(a) * 256 > 0xFFFFFFFFll) return false;
     if (p.part[i].kind == kRows && (int64_t)a.heads * a.head_tiles > 65535) return false;
   }

@@ -366,6 +366,7 @@ attention_many_kernel(AttentionArgs a) {
       Frag k[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) k[i] = key(i);
+      __builtin_amdgcn_s_setprio(1);  // products go before the other wave's weights
 #pragma unroll
       for (int i = 0; i < 2 * KC; ++i) {
         __builtin_amdgcn_sched_barrier(kMayCross);
@@ -373,6 +374,7 @@ attention_many_kernel(AttentionArgs a) {
         if (i + kAhead < 2 * KC) k[i % kAhead] = key(i + kAhead);
       }
       __builtin_amdgcn_sched_barrier(kMayCross);
+      __builtin_amdgcn_s_setprio(0);
     }
     const bool whole = now.there == ~0ull && base >= all_lo && base + kManyStep <= all_hi;
     float top = -INFINITY;
@@ -477,6 +479,7 @@ attention_many_kernel(AttentionArgs a) {
     Frag v[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) v[i] = values(i / NJ, i % NJ);
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < 4 * NJ; ++i) {
       __builtin_amdgcn_sched_barrier(kMayCross);
@@ -484,6 +487,7 @@ attention_many_kernel(AttentionArgs a) {
       if (i + kAhead < 4 * NJ) v[i % kAhead] = values((i + kAhead) / NJ, (i + kAhead) % NJ);
     }
     __builtin_amdgcn_sched_barrier(kMayCross);
+    __builtin_amdgcn_s_setprio(0);
   };
 
   // The two buffers are told apart by the parameters' __restrict__: a transposing
