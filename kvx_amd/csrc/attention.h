@@ -317,9 +317,15 @@ void run_attention_few_bf16_e4m3(const AttentionArgs &a, bool vt, bool grouped, 
                         hipStream_t s);
 void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
                         hipStream_t s);
+void run_attention_few_f32(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
 void run_attention_few_f16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
                         hipStream_t s);
+void run_attention_few_f32_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
 void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                        hipStream_t s);
+void run_attention_few_f32_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
                         hipStream_t s);
 void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
                         hipStream_t s);

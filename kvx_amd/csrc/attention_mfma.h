@@ -43,6 +43,11 @@ __device__ __forceinline__ Acc mma(const Frag &a, const Frag &b, Acc c) {
   }
 }
 
+// c + a b: v_mfma_f32_16x16x4_f32.
+__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
 // Two f32 to two 16-bit elements, to nearest even.
 template <int IO>
 __device__ __forceinline__ uint32_t pair_of(float a, float b) {
@@ -73,10 +78,19 @@ __device__ __forceinline__ uint32_t widen(uint32_t w, bool hi) {
   }
 }
 
+// FP8 code number i of w.
+template <int C>
+__device__ __forceinline__ float code(uint32_t w, int i) {
+  if constexpr (bytes_of_type<C>() == 1)
+    return decode_pair<C == KVX_DTYPE_F8_E5M2>((int)w, i >= 2)[i & 1];
+  else return 0.0f;
+}
+
 // An element of w that is NaN or infinite.
 template <int C>
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  if constexpr (C == KVX_DTYPE_BF16) return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
+  if constexpr (C == KVX_DTYPE_F32) return ((w & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+  else if constexpr (C == KVX_DTYPE_BF16) return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
   else if constexpr (C == KVX_DTYPE_F16) return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
   else if constexpr (C == KVX_DTYPE_F8_E4M3)
     return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
@@ -122,7 +136,7 @@ __device__ __forceinline__ void add_infinities(const AttentionArgs &a, const Que
             float *p = a.part_o + (part_index(a, t, t.first + i, head) * a.splits + z) * a.head_dim;
             p[d] += x;
           } else {
-            char *p = a.out + (t.begin + t.first + i) * a.o_tok + head * a.o_head + 2 * d;
+            char *p = a.out + (t.begin + t.first + i) * a.o_tok + head * a.o_head + d * bytes_of_type<IO>();
             store_out<IO>(p, value_at<IO>(p) + x);
           }
         }
@@ -146,7 +160,9 @@ template <int IO, int N>
 __device__ __forceinline__ float positive_scale(const AttentionArgs &a, float ks, Frag (&q)[N]) {
   if (a.cap != 0.0f) return 1.0f;
   const float scale = a.scale_log2 * ks;
-  const uint32_t keep = scale == 0.0f ? 0u : ~0u, flip = scale < 0.0f ? 0x80008000u : 0u;
+  const uint32_t keep = scale == 0.0f ? 0u : ~0u, flip = scale >= 0.0f             ? 0u
+                                                            : IO == KVX_DTYPE_F32 ? 0x80000000u
+                                                                                  : 0x80008000u;
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll

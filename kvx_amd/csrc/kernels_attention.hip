@@ -201,22 +201,23 @@ bool near(const AttentionPlan &p, const Geom &g) {
          (pieces * g.s_piece + (int64_t)g.pack * g.s_inner) * e < most;
 }
 
-// The matrix-core kernels read queries and write outputs 8 elements at a time
-// and keys 16 bytes at a time.
+// The matrix-core kernels read queries and keys 16 bytes at a time and write 8
+// elements of the output at a time.
 bool matrix_cores(const AttentionPlan &p) {
   const int D = p.g.head_dim, e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
-  if (p.g.io_dtype == KVX_DTYPE_F32 || D % 8 != 0 || D > 256) return false;
-  if (((p.q_tok | p.q_head | p.o_tok | p.o_head) % 8) != 0 ||
+  if (D % 8 != 0 || D > 256) return false;
+  const int n = 16 / dtype_size((kvx_dtype_t)p.g.io_dtype);
+  if (((p.q_tok | p.q_head | p.o_tok | p.o_head) % n) != 0 ||
       (uintptr_t)p.query % 16 != 0 || (uintptr_t)p.out % 16 != 0)
     return false;
   return near(p, p.g.gk) && near(p, p.g.gv) && chunks(p, p.g.gk, p.g.src_k, 16 / e);
 }
 
-// Values: DP / 16 elements at a time (few rows) or 16 bytes (many); with the
-// token axis innermost 4 tokens or 8 (vt).
+// Values: DP / 16 elements at a time, or 16 bytes of more (few rows), or 16 bytes
+// (many); with the token axis innermost 4 tokens or 8 (vt).
 bool values_fit(const AttentionPlan &p, Kind kind, bool *vt) {
   const int D = p.g.head_dim, e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
-  const int n = kind == kMany || D > 128 ? 16 / e : D <= 64 ? 4 : 8;
+  const int n = kind == kMany || D > 128 || e == 4 ? 16 / e : D <= 64 ? 4 : 8;
   *vt = !chunks(p, p.g.gv, p.g.src_v, n);
   return !*vt || tokens_inner(p, kind == kMany ? 8 : 4);
 }
@@ -280,9 +281,11 @@ Plan make_plan(const AttentionPlan &p) {
     return r.part[r.parts++].a;
   };
   const bool cores = matrix_cores(p);
-  // Sequences of at most `few` new tokens go to the kernel for few rows: about
-  // two of its tiles.  How many new tokens each has is known here where there
-  // is one sequence, one token each, or a hint that bounds all; else both
+  // Sequences of at most `few` new tokens go to the kernel for few rows: two of
+  // its tiles (8 sequences of 7 tokens at 8192, groups of 4: 91 us, with the
+  // other kernel 122; 64 of them at 2048: 164 and 145; with three tiles, 12
+  // tokens, 236 and 139).  How many new tokens each has is known here where
+  // there is one sequence, one token each, or a hint that bounds all; else both
   // kernels run and each takes its own.
   const int few = a.group >= 2 * kRowTile ? 1 : 2 * kRowTile / a.group;
   const bool all_few = a.qptr == nullptr || a.tokens <= few ||
@@ -295,7 +298,7 @@ Plan make_plan(const AttentionPlan &p) {
               steps_fit(g.gv);
   const bool few_ok = cores && values_fit(p, kFew, &r.vt);
   bool vt_many = false;
-  const bool many_ok = few_ok && values_fit(p, kMany, &vt_many) && vt_many == r.vt;
+  const bool many_ok = few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) && vt_many == r.vt;
   if (!few_ok) {
     AttentionArgs &x = add(kRows, a);
     tile_rows(&x, kRowTile);
@@ -363,6 +366,9 @@ void run_part(const Plan::Part &p, bool vt, bool grouped, int io, int cache, hip
   const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
   if (p.kind == kRows)
     run_attention_rows(p.a, io, cache, s);
+  else if (p.kind == kFew && io == KVX_DTYPE_F32)
+    (e4 ? run_attention_few_f32_e4m3 : e5 ? run_attention_few_f32_e5m2
+                                          : run_attention_few_f32)(p.a, vt, grouped, grid, s);
   else if (p.kind == kFew && io == KVX_DTYPE_BF16)
     (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
                                            : run_attention_few_bf16)(p.a, vt, grouped, grid, s);

@@ -24,6 +24,20 @@
 //                 cache whose token axis is innermost it loads four tokens of
 //                 one element, as they are.
 //
+// F32: v_mfma_f32_16x16x4, lane l has A[row c][g] and B[g][column c].  Element
+// 16 i + 4 g + w of a key is the w-th of the lane's i-th load, and takes part in
+// the product 4 i + w with the query's element of that place; values need no
+// transposition, a product takes tokens 4 g + i of the four groups.  Wide F32
+// rows take steps of 16 tokens, so that two waves a SIMD have registers (heads
+// of 128, 16 sequences of 4096 tokens: 102 us, 111 with 32 tokens and one wave;
+// of 256: 242, and 584 with 32 tokens, for which there are no registers).
+//
+// Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16
+// 96 us (5.6 TB/s), FP8 59 us (4.5 TB/s), F32 188 us (5.7 TB/s).  More waves a
+// SIMD in fewer registers spill: BF16 at three 142 us.  Sequences whose rows need
+// two tiles read their keys and values twice, from L2 the second time: with 8
+// tokens each 165 us.
+//
 // Maximum and sum are one register each, as a lane has one row; the maximum
 // is shared over the four lane groups, the sum only at the end.  Weights are
 // rounded to the queries' type for the product (half a step of 2^-8 or 2^-11
@@ -37,7 +51,6 @@ namespace dev {
 
 constexpr int kFewWaves = 4;
 constexpr int kFewThreads = kFewWaves * kWave;
-constexpr int kFewStep = 32;  // tokens
 
 // Token e of a lane's eight in a step, from its group's first.
 __device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12 + e; }
@@ -46,13 +59,17 @@ __device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12
 // rounded up to 64, 128 or 256; VT: values with the token axis innermost;
 // INDEXED: scales by block.
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
-__global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_kernel(AttentionArgs a) {
-  constexpr bool kFp8 = C != IO;
-  constexpr int E = kFp8 ? 1 : 2;
-  constexpr int KC = DP / 32;          // products of a half step's logits
+__global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
+    attention_few_kernel(AttentionArgs a) {
+  constexpr bool kFp8 = C != IO, kF32 = IO == KVX_DTYPE_F32;
+  constexpr int E = bytes_of_type<C>();
+  constexpr int KC = kF32 ? DP / 16 : DP / 32;  // operands of a half step's logits
   constexpr int KL = DP * E / 64;      // 16-byte key loads of a token and lane group
   constexpr int NV = DP / 16;          // products of a step's sums; elements a lane loads
   constexpr int VB = NV * E;           // bytes of them
+  constexpr int HALVES = DP * E >= 512 ? 1 : 2;  // groups of 16 tokens in a step: registers
+  constexpr int kFewStep = 16 * HALVES;           // tokens
+  constexpr uint32_t kAll = 0xFFFFFFFFu >> (32 - kFewStep);
   constexpr int VW = VB / 4;           // dwords (VT: of four tokens)
   __shared__ float sums[2][kRowTile][DP + 4];
   __shared__ float states[kFewWaves][2][kRowTile];
@@ -97,11 +114,13 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   Frag q[KC];
 #pragma unroll
   for (int i = 0; i < KC; ++i) {
-    // FP8: two products share a 16-byte load of 16 elements
-    const int d = kFp8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+    // FP8: two (F32: four) operands share a 16-byte load of 16 elements
+    constexpr int N = kF32 ? 4 : 8, kShare = kFp8 ? 16 / N : 1;
+    const int d = N * (4 * kShare * (i / kShare) + kShare * g + i % kShare);
     Raw<16> r{};
     if (row && d < D)
-      r = ld<16>(a.q + (t.begin + t.first + tok) * a.q_tok + (int64_t)qh * a.q_head + 2 * d);
+      r = ld<16>(a.q + (t.begin + t.first + tok) * a.q_tok + (int64_t)qh * a.q_head +
+                 d * bytes_of_type<IO>());
 #pragma unroll
     for (int j = 0; j < 4; ++j) q[i].w[j] = r.w[j];
   }
@@ -141,11 +160,12 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   const uint32_t vrow = (uint32_t)(4 * g * (int)a.gv.s_off);
 
   constexpr int kStride = kFewWaves * kFewStep;
-  // GROUPED: lane 2 i + b looks up the first token of half b of the wave's i-th
-  // step, so that one look serves 32 steps; else lane i looks up token i of one.
-  constexpr int kSteps = GROUPED ? 32 : 1;
+  // GROUPED: lane HALVES i + b looks up the first token of half b of the wave's
+  // i-th step, so that one look serves 32 steps; else lane i looks up token i of
+  // one.
+  constexpr int kSteps = GROUPED ? kWave / HALVES : 1;
   auto token_of_lane = [&](int base) {
-    return GROUPED ? base + (lane / 2) * kStride + 16 * (lane % 2) : base + lane;
+    return GROUPED ? base + (lane / HALVES) * kStride + 16 * (lane % HALVES) : base + lane;
   };
   auto looks = [&](int base) {
     return token_of_lane(base) < to && (GROUPED || lane < kFewStep);
@@ -166,7 +186,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
     // anything.
     const uint32_t in = (uint32_t)tokens_between(lo, to, base, kFewStep);
     const uint32_t held =
-        GROUPED ? (uint32_t)group_tokens((uint32_t)(rows.held >> lane0) & 3u) : (uint32_t)rows.held;
+        GROUPED ? (uint32_t)group_tokens((uint32_t)(rows.held >> lane0) & (2u * HALVES - 1))
+                : (uint32_t)rows.held;
     return {rows, lane0, held & in};
   };
   auto look = [&](int base, const TokenEntry &entry) {
@@ -176,7 +197,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   auto token_scale = [&](const Step &s, float x, int e) {
     return GROUPED ? from_lane(x, 4 * (s.lane0 + e / 4)) : from_lane(x, 16 * g + 4 * place_of(e));
   };
-  uint32_t kw[2][KL][4];
+  uint32_t kw[HALVES][KL][4];
   auto load_keys = [&](const Step &s) {
     if (s.rows.held == 0) return;
     auto one = [&](int b, uint64_t p, uint32_t row) {
@@ -188,18 +209,18 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       }
     };
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < HALVES; ++b) {
       if constexpr (GROUPED) one(b, address_of_lane(s.rows.k, s.lane0 + b), krow);
       else one(b, from_lane(s.rows.k, 4 * c + 64 * b), 0);
     }
   };
   // Rows: [token e][dword]; VT: [half b][element j][dword].
-  uint32_t vw[VT ? 2 * NV : 8][VT ? E : VW];
+  uint32_t vw[VT ? HALVES * NV : 4 * HALVES][VT ? E : VW];
   auto load_values = [&](const Step &s) {
     if (s.rows.held == 0) return;
     if constexpr (VT) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < HALVES; ++b) {
         uint64_t p;
         if constexpr (GROUPED) p = address_of_lane(s.rows.v, s.lane0 + b);
         else p = from_lane(s.rows.v, 16 * g + 64 * b);
@@ -220,7 +241,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         }
       };
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4 * HALVES; ++e) {
         if constexpr (GROUPED)
           one(e, address_of_lane(s.rows.v, s.lane0 + e / 4) + (e % 4) * a.gv.s_off, vrow);
         else one(e, from_lane(s.rows.v, 16 * g + 4 * place_of(e)), 0);
@@ -231,12 +252,13 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
   auto clear_values = [&](uint32_t there) {
     if constexpr (VT) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < HALVES; ++b) {
         const uint32_t have = (there >> (4 * g)) >> (16 * b);
 #pragma unroll
         for (int w = 0; w < E; ++w) {
           const uint32_t keep =
-              E == 2 ? ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
+              E == 4   ? (have >> w) & 1 ? ~0u : 0u
+              : E == 2 ? ((have >> (2 * w)) & 1 ? 0xFFFFu : 0u) |
                            ((have >> (2 * w + 1)) & 1 ? 0xFFFF0000u : 0u)
                      : (have & 1 ? 0xFFu : 0u) | (have & 2 ? 0xFF00u : 0u) |
                            (have & 4 ? 0xFF0000u : 0u) | (have & 8 ? 0xFF000000u : 0u);
@@ -246,7 +268,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4 * HALVES; ++e) {
         const uint32_t keep = ((there >> (4 * g)) >> place_of(e)) & 1 ? ~0u : 0u;
 #pragma unroll
         for (int w = 0; w < VW; ++w) vw[e][w] &= keep;
@@ -270,7 +292,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         rows = look(at, ahead);
         ahead = entries(at + kSteps * kStride);
       }
-      return step_at(rows, at, 2 * count);
+      return step_at(rows, at, HALVES * count);
     };
     Step next = advance(base + kStride);
     for (;;) {
@@ -279,21 +301,32 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         for (int i = 0; i < KL; ++i) {
           const uint32_t keep = (i * 64 + g * 16) / E < D ? ~0u : 0u;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            kw[0][i][j] &= keep;
-            kw[1][i][j] &= keep;
-          }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int b = 0; b < HALVES; ++b) kw[b][i][j] &= keep;
         }
       }
       // Logits: lane c has its row's tokens base + 16 b + 4 g + i.
-      f32x4 s[2];
+      f32x4 s[HALVES] = {};
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        s[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int b = 0; b < HALVES; ++b) {
 #pragma unroll
         for (int i = 0; i < KC; ++i) {
           Frag k;
-          if constexpr (kFp8) {
+          if constexpr (kF32) {
+            // the halves in turn, whose sums do not wait for each other
+            if (b == 1) continue;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+#pragma unroll
+              for (int half = 0; half < HALVES; ++half) {
+                const float x = kFp8 ? code<C>(kw[half][i / 4][i % 4], w)
+                                     : bits_f32(kw[half][kFp8 ? 0 : i][w]);
+                s[half] = mma4(x, bits_f32(q[i].w[w]), s[half]);
+              }
+            }
+            continue;
+          } else if constexpr (kFp8) {
 #pragma unroll
             for (int w = 0; w < 4; ++w)
               k.w[w] = widen<IO, C>(kw[b][i / 2][2 * (i % 2) + w / 2], w % 2);
@@ -307,29 +340,29 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       const bool more = base + kStride < to;
       if (more) load_keys(next);
 
-      const bool whole = now.there == 0xFFFFFFFFu && base >= last_lo && base + kFewStep <= first_hi;
-      float x[8], p[8], top = -INFINITY;
+      const bool whole = now.there == kAll && base >= last_lo && base + kFewStep <= first_hi;
+      float x[4 * HALVES], p[4 * HALVES], top = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4 * HALVES; ++e) {
         x[e] = s[e / 4][e % 4];
         if constexpr (INDEXED) x[e] *= token_scale(now, now.rows.ks, e);
       }
       if (a.cap != 0.0f) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = capped(a, x[e] * ks);
+        for (int e = 0; e < 4 * HALVES; ++e) x[e] = capped(a, x[e] * ks);
       }
       if (!whole) {
         const uint32_t there = now.there >> (4 * g);
         const int start = base + 4 * g;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4 * HALVES; ++e) {
           const int at = start + place_of(e);
           const bool seen = ((there >> place_of(e)) & 1) & (at >= rlo) & (at < rhi);
           x[e] = seen ? x[e] : -INFINITY;
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);  // NaN does not move it
+      for (int e = 0; e < 4 * HALVES; ++e) top = fmaxf(top, x[e]);  // NaN does not move it
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32)) * scale;
       top = fmaxf(top, m);
@@ -342,7 +375,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
       }
       m = top;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4 * HALVES; ++e) {
         p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], scale, -shift));
         l += p[e];
       }
@@ -350,7 +383,7 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         // Values stay codes; weights carry the tokens' scales, relative to the
         // largest so far, so that they stay in the type's range.
         const int in = GROUPED ? lane - now.lane0 : lane;
-        const bool mine_there = in >= 0 && in < (GROUPED ? 2 : kFewStep) &&
+        const bool mine_there = in >= 0 && in < (GROUPED ? HALVES : kFewStep) &&
                                 ((now.rows.held >> lane) & 1);
         float mine = mine_there ? fabsf(now.rows.vs) : 0.0f;
 #pragma unroll
@@ -363,18 +396,14 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         }
         const float inv = vref > 0.0f ? 1.0f / vref : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 4 * HALVES; ++e)
           p[e] *= token_scale(now, now.rows.vs, e) * inv;
       }
-      Frag w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w.w[i] = pair_of<IO>(p[2 * i], p[2 * i + 1]);
-
-      if (now.there != 0xFFFFFFFFu) clear_values(now.there);
+      if (now.there != kAll) clear_values(now.there);
       if (t.count > 1 && (base < last_lo || base + kFewStep > first_hi)) {
         uint32_t odd = 0;  // some rows do not see some tokens
 #pragma unroll
-        for (int e = 0; e < (VT ? 2 * NV : 8); ++e)
+        for (int e = 0; e < (VT ? HALVES * NV : 4 * HALVES); ++e)
 #pragma unroll
           for (int i = 0; i < (VT ? E : VW); ++i) {
             odd |= not_finite<C>(vw[e][i]);
@@ -382,36 +411,54 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
           }
         if (odd != 0) infinities = 1;
       }
-      // Values by element: v[j], token order of the weights.
-      auto by_element = [&](int d, Frag *v) {  // v[2 d] and v[2 d + 1]
+      if constexpr (kF32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (VT) {
+        for (int e = 0; e < 4 * HALVES; ++e)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int at = (i / 2) * NV + 2 * d + k;
-              v[k].w[i] = kFp8 ? widen<IO, C>(vw[at][0], i % 2) : vw[at][kFp8 ? 0 : i % 2];
-            }
-          } else {
-            uint32_t t0, t1;
-            if constexpr (kFp8) {
-              t0 = widen<IO, C>(vw[2 * i][d / 2], d % 2);
-              t1 = widen<IO, C>(vw[2 * i + 1][d / 2], d % 2);
-            } else {
-              t0 = vw[2 * i][d];
-              t1 = vw[2 * i + 1][d];
-            }
-            v[0].w[i] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
-            v[1].w[i] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+          for (int j = 0; j < NV; ++j) {
+            float x;
+            if constexpr (VT)
+              x = kFp8 ? code<C>(vw[(e / 4) * NV + j][0], e % 4)
+                       : bits_f32(vw[(e / 4) * NV + j][kFp8 ? 0 : e % 4]);
+            else
+              x = kFp8 ? code<C>(vw[e][j / 4], j % 4) : bits_f32(vw[e][kFp8 ? 0 : j]);
+            acc[j] = mma4(x, p[e], acc[j]);
           }
-        }
-      };
+      } else {
+        Frag w;
 #pragma unroll
-      for (int d = 0; d < NV / 2; ++d) {
-        Frag v[2];
-        by_element(d, v);
-        acc[2 * d] = mma<IO>(v[0], w, acc[2 * d]);
-        acc[2 * d + 1] = mma<IO>(v[1], w, acc[2 * d + 1]);
+        for (int i = 0; i < 4; ++i) w.w[i] = pair_of<IO>(p[2 * i], p[2 * i + 1]);
+        // Values by element: v[j], token order of the weights.
+        auto by_element = [&](int d, Frag *v) {  // v[2 d] and v[2 d + 1]
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (VT) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int at = (i / 2) * NV + 2 * d + k;
+                v[k].w[i] = kFp8 ? widen<IO, C>(vw[at][0], i % 2) : vw[at][kFp8 ? 0 : i % 2];
+              }
+            } else {
+              uint32_t t0, t1;
+              if constexpr (kFp8) {
+                t0 = widen<IO, C>(vw[2 * i][d / 2], d % 2);
+                t1 = widen<IO, C>(vw[2 * i + 1][d / 2], d % 2);
+              } else {
+                t0 = vw[2 * i][d];
+                t1 = vw[2 * i + 1][d];
+              }
+              v[0].w[i] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+              v[1].w[i] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+            }
+          }
+        };
+#pragma unroll
+        for (int d = 0; d < NV / 2; ++d) {
+          Frag v[2];
+          by_element(d, v);
+          acc[2 * d] = mma<IO>(v[0], w, acc[2 * d]);
+          acc[2 * d + 1] = mma<IO>(v[1], w, acc[2 * d + 1]);
+        }
       }
       if (!more) break;
       load_values(next);
@@ -500,10 +547,21 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) attention_few_
         *reinterpret_cast<f32x4 *>(o) = f32x4{x[0], x[1], x[2], x[3]};
         *reinterpret_cast<f32x4 *>(o + 4) = f32x4{x[4], x[5], x[6], x[7]};
       } else {
+        char *to_row =
+            a.out + out_row * a.o_tok + (int64_t)head * a.o_head + d * bytes_of_type<IO>();
         Raw<16> o;
+        if constexpr (kF32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o.w[i] = pack_pair<IO>(f32x2{x[2 * i], x[2 * i + 1]});
-        st<16>(a.out + out_row * a.o_tok + (int64_t)head * a.o_head + 2 * d, o);
+          for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o.w[i] = f32_bits(x[4 * b + i]);
+            st<16>(to_row + 16 * b, o);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o.w[i] = pack_pair<IO>(f32x2{x[2 * i], x[2 * i + 1]});
+          st<16>(to_row, o);
+        }
       }
     }
   }

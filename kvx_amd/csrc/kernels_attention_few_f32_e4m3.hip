@@ -1,0 +1,13 @@
+// Attention of few rows: F32 queries over an E4M3 cache.
+#include "kernels_attention_few.h"
+
+namespace kvx {
+namespace dev {
+
+void run_attention_few_f32_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
+                                 hipStream_t s) {
+  launch_few<KVX_DTYPE_F32, KVX_DTYPE_F8_E4M3>(a, vt, grouped, grid, s);
+}
+
+}  // namespace dev
+}  // namespace kvx
