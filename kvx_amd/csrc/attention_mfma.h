@@ -196,17 +196,24 @@ struct LaneRows {
   uint64_t k, v;
   uint64_t held;  // bit per lane whose token is there; none: k and v cannot be read
   float ks, vs;   // block-indexed scales
+  bool apart;     // a value load's tokens are not all of one block
 };
 
-template <bool INDEXED>
+// VN: values with the token axis innermost, VN tokens a load from the lane of the
+// first.  Only a RAGGED table can name different blocks for them; v is the row
+// of the load's first token in the lane's own block then.
+template <bool INDEXED, int VN = 0>
 __device__ __forceinline__ LaneRows lane_rows(const AttentionArgs &a, const TokenEntry &entry,
                                               int at, bool looks, int kvh) {
-  LaneRows r{0, 0, 0, 1.0f, 1.0f};
+  LaneRows r{0, 0, 0, 1.0f, 1.0f, false};
   TokenRows x{nullptr, nullptr, 0};
   const bool held = looks && token_rows(a, entry, at, &x);
   if (held) {
     r.k = reinterpret_cast<uint64_t>(x.k + kvh * a.gk.s_head);
     r.v = reinterpret_cast<uint64_t>(x.v + kvh * a.gv.s_head);
+    if constexpr (VN > 0) {
+      if (a.format == KVX_BLOCK_TABLE_RAGGED) r.v -= (at % VN) * a.gv.s_off;
+    }
     if constexpr (INDEXED) {
       r.ks = scale_of(a.ks, x.block, kvh);
       r.vs = scale_of(a.vs, x.block, kvh);
@@ -219,6 +226,13 @@ __device__ __forceinline__ LaneRows lane_rows(const AttentionArgs &a, const Toke
     if (!held) {
       r.k = k;
       r.v = v;
+    }
+  }
+  if constexpr (VN > 0) {
+    if (a.format == KVX_BLOCK_TABLE_RAGGED && r.held != 0) {
+      const int first = (int)(threadIdx.x % kWave) / VN * VN;
+      const bool same = from_lane(r.v, 4 * first) == r.v && ((r.held >> first) & 1);
+      r.apart = __any(held && !same);
     }
   }
   return r;
@@ -237,6 +251,14 @@ __device__ __forceinline__ uint64_t group_tokens(uint32_t groups) {
   return ((groups & 1) | (uint64_t)(groups & 2) << 15 | (uint64_t)(groups & 4) << 30 |
           (uint64_t)(groups & 8) << 45) *
          0xFFFFull;
+}
+
+// Bits of token `at` of a load of tokens, in its dword w.
+template <int E>
+__device__ __forceinline__ uint32_t token_bits(int at, int w) {
+  constexpr int kEach = 4 / E;  // tokens of a dword
+  const uint32_t one = E == 4 ? ~0u : (1u << (8 * E % 32)) - 1;
+  return at / kEach == w ? one << (8 * E * (at % kEach) % 32) : 0u;
 }
 
 // B bytes of global memory at an address that went through another lane, and so

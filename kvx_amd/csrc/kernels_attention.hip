@@ -183,7 +183,7 @@ struct Plan {
 bool tokens_inner(const AttentionPlan &p, int n) {
   const Geom &g = p.g.gv;
   const int e = dtype_size((kvx_dtype_t)p.g.cache_dtype);
-  if (g.s_off != 1 || p.g.block_size % n != 0 || p.g.format == KVX_BLOCK_TABLE_RAGGED) return false;
+  if (g.s_off != 1 || p.g.block_size % n != 0) return false;
   uint64_t low = (uint64_t)((g.s_inner | g.s_head | g.s_piece) * e);
   if (p.g.format == KVX_BLOCK_TABLE_KV_OFFSETS)
     low |= (uint64_t)(uintptr_t)p.g.pool[0] | (uint64_t)(uintptr_t)p.g.pool[1] |

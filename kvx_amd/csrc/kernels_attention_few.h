@@ -67,8 +67,9 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
   constexpr int KL = DP * E / 64;      // 16-byte key loads of a token and lane group
   constexpr int NV = DP / 16;          // products of a step's sums; elements a lane loads
   constexpr int VB = NV * E;           // bytes of them
-  constexpr int HALVES = DP * E >= 512 ? 1 : 2;  // groups of 16 tokens in a step: registers
-  constexpr int kFewStep = 16 * HALVES;           // tokens
+  // groups of 16 tokens in a step
+  constexpr int HALVES = kF32 && DP * E >= 512 ? 1 : 2;
+  constexpr int kFewStep = 16 * HALVES;  // tokens
   constexpr uint32_t kAll = 0xFFFFFFFFu >> (32 - kFewStep);
   constexpr int VW = VB / 4;           // dwords (VT: of four tokens)
   __shared__ float sums[2][kRowTile][DP + 4];
@@ -191,7 +192,8 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
     return {rows, lane0, held & in};
   };
   auto look = [&](int base, const TokenEntry &entry) {
-    return lane_rows<INDEXED>(a, entry, token_of_lane(base), looks(base), kvh);
+    return lane_rows<INDEXED, VT && !GROUPED ? 4 : 0>(a, entry, token_of_lane(base), looks(base),
+                                                      kvh);
   };
   // A token's scale, of the eight that the lane has.
   auto token_scale = [&](const Step &s, float x, int e) {
@@ -218,6 +220,26 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
   uint32_t vw[VT ? HALVES * NV : 4 * HALVES][VT ? E : VW];
   auto load_values = [&](const Step &s) {
     if (s.rows.held == 0) return;
+    if constexpr (VT && !GROUPED) {
+      if (s.rows.apart) {  // each token's block in turn
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int b = 0; b < HALVES; ++b) {
+            const uint64_t p = from_lane(s.rows.v, 16 * g + 64 * b + 4 * e);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+              const Raw<VLB> r = global_load<VLB, true>(p, voff[j]);
+#pragma unroll
+              for (int w = 0; w < E; ++w) {
+                const uint32_t mine = token_bits<E>(e, w);
+                vw[b * NV + j][w] = (vw[b * NV + j][w] & ~mine) | (r.w[w] & mine);
+              }
+            }
+          }
+        return;
+      }
+    }
     if constexpr (VT) {
 #pragma unroll
       for (int b = 0; b < HALVES; ++b) {

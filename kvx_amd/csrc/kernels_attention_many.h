@@ -203,7 +203,7 @@ attention_many_kernel(AttentionArgs a) {
   };
   auto look = [&](int base, const TokenEntry &entry) {
     const int at = token_of_lane(base);
-    return lane_rows<INDEXED>(a, entry, at, at < to, kvh);
+    return lane_rows<INDEXED, VT && !GROUPED ? 8 : 0>(a, entry, at, at < to, kvh);
   };
 
   // GROUPED: a wave's load takes kGroup tokens of one block, from one scalar
@@ -248,6 +248,24 @@ attention_many_kernel(AttentionArgs a) {
     Staged x{};
     if (s.rows.held == 0) return x;
     each_key(s, [&](int l, uint64_t p, uint32_t o) { x.k[l] = global_load<16, false>(p, o); });
+    if constexpr (VT && !GROUPED) {
+      if (s.rows.apart) {  // each token's block in turn
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t p = from_lane(s.rows.v, 32 * vgroup8 + 4 * e);
+#pragma unroll
+          for (int l = 0; l < NVL; ++l) {
+            const Raw<VLB> r = global_load<VLB, false>(p, voff[l]);
+#pragma unroll
+            for (int w = 0; w < VLB / 4; ++w) {
+              const uint32_t mine = token_bits<E>(e, w);
+              x.v[l].w[w] = (x.v[l].w[w] & ~mine) | (r.w[w] & mine);
+            }
+          }
+        }
+        return x;
+      }
+    }
     each_value(s, [&](int l, uint64_t p, uint32_t o) { x.v[l] = global_load<VLB, false>(p, o); });
     return x;
   };
@@ -522,7 +540,8 @@ attention_many_kernel(AttentionArgs a) {
     int buffer = 0;
     for (int base = from;; base += kManyStep) {
       const bool more = base + kManyStep < to;
-      const bool direct = !kFp8 && D == DP && plain(next, base + kManyStep);
+      const bool direct =
+          !kFp8 && D == DP && plain(next, base + kManyStep) && !(VT && next.rows.apart);
       if (more) {
         if constexpr (kFp8) staged = load(next);
       }

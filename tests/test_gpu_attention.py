@@ -119,6 +119,34 @@ def test_blocks_that_are_not_there(io, cache, table):
        holes=[(0, 1), (1, 2), (2, 0), (3, 0), (3, 5), (3, 12)])
 
 
+@pytest.mark.parametrize("layout", ["nhd", "vllm"])
+@pytest.mark.parametrize("io,cache,D", [("bf16", None, 128), ("f16", "e4m3", 64), ("f32", None, 64),
+                                        ("f32", "e5m2", 80), ("bf16", None, 256)])
+@pytest.mark.parametrize("share", [0.0, 0.1, 1.0])
+def test_ragged_tables_whose_tokens_lie_apart(io, cache, D, layout, share):
+    """A RAGGED table names each token's block: `share` of them are moved to
+    other blocks, or to none, so that neighbours lie apart."""
+    c = AttentionCase(io=io, cache=cache, layout=layout, table="ragged", lens=[70, 5, 200, 131],
+                      new=[1, 2, 70, 40], D=D, H=2, G=2)
+    ids = c.table.indices.cpu().clone()
+    g = torch.Generator().manual_seed(5)
+    moved = torch.rand(ids.shape, generator=g) < share
+    ids[moved] = torch.randint(-1, c.nb + 1, ids.shape, generator=g).to(ids.dtype)[moved]
+    c.table = paged.RaggedTable(ids.to("cuda"), c.table.indptr)
+    ptr = c.table.indptr.tolist()
+
+    def rows_of(s):
+        b = ids[ptr[s]: ptr[s + 1]].long()
+        o = torch.arange(b.numel()) % c.bs
+        there = (b >= 0) & (b < c.nb)
+        b = b.clamp(0, c.nb - 1)
+        return c.exact[0][b, o], c.exact[1][b, o], there
+
+    c.rows_of = rows_of
+    assert c.run() == Status.OK
+    c.check()
+
+
 def test_lengths_past_the_table():
     """A length beyond what the table holds: the missing tokens are not
     attended to, positions count from the length."""
