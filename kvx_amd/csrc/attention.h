@@ -308,39 +308,37 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-void run_attention_rows(const AttentionArgs &a, int io, int cache, hipStream_t s);
+// A launch of one of the kernels.
+struct AttentionPart {
+  AttentionArgs a;
+  uint32_t grid;  // workgroups
+};
+
+void run_attention_rows(const AttentionPart &p, int io, int cache, hipStream_t s);
 // vt: values with the token axis innermost; grouped: blocks hold whole groups of
 // the tokens that a wave loads together, whose rows follow from the first's
-void run_attention_few_bf16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_bf16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_bf16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f32(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f32_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f32_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_few_f16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_bf16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_bf16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_bf16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_f16(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_f16_e4m3(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
-void run_attention_many_f16_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                        hipStream_t s);
+void run_attention_few_f32(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_f32_e4m3(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_f32_e5m2(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_bf16(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_bf16_e4m3(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_bf16_e5m2(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_f16(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_f16_e4m3(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+void run_attention_few_f16_e5m2(const AttentionPart &p, bool vt, bool grouped, hipStream_t s);
+// few: sequences of few new tokens in the same launch, or null
+void run_attention_many_bf16(const AttentionPart &p, const AttentionPart *few, bool vt,
+                             bool grouped, hipStream_t s);
+void run_attention_many_bf16_e4m3(const AttentionPart &p, const AttentionPart *few, bool vt,
+                                  bool grouped, hipStream_t s);
+void run_attention_many_bf16_e5m2(const AttentionPart &p, const AttentionPart *few, bool vt,
+                                  bool grouped, hipStream_t s);
+void run_attention_many_f16(const AttentionPart &p, const AttentionPart *few, bool vt,
+                            bool grouped, hipStream_t s);
+void run_attention_many_f16_e4m3(const AttentionPart &p, const AttentionPart *few, bool vt,
+                                 bool grouped, hipStream_t s);
+void run_attention_many_f16_e5m2(const AttentionPart &p, const AttentionPart *few, bool vt,
+                                 bool grouped, hipStream_t s);
 
 }  // namespace dev
 }  // namespace kvx

@@ -24,14 +24,14 @@ __host__ __device__ __forceinline__ int64_t join_rows(const AttentionArgs &a) {
 // VEC elements of every G-th split, G as many as fit beside each other, and add
 // the G sums up through LDS: loads of many splits are in flight at once.
 template <int IO, int VEC, int kJoinThreads>
-__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionArgs a) {
+__device__ __forceinline__ void join_splits(const AttentionArgs &a, uint32_t unit) {
   __shared__ float weights[kJoinThreads];  // of the splits; < 0: nothing was written for it
   __shared__ float waves[2][kJoinThreads / kWave];
   __shared__ float sums[kJoinThreads * VEC];
   const int tid = (int)threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int hq = a.heads * a.group;
-  const int64_t part = blockIdx.x / (uint32_t)hq;
-  const int head = (int)(blockIdx.x % (uint32_t)hq);
+  const int64_t part = unit / (uint32_t)hq;
+  const int head = (int)(unit % (uint32_t)hq);
   int64_t row = part;
   if (a.qptr != nullptr) {
     const int s = a.part_rows > 0 ? (int)(part / a.part_rows)
@@ -96,6 +96,18 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(AttentionA
   }
   if (tid == 0 && a.lse != nullptr)
     a.lse[row * hq + head] = none ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+// Up to two parts' sums: of the sequences of many new tokens and of few.
+struct JoinArgs {
+  AttentionArgs part[2];
+  uint32_t units;  // rows and heads of the first
+};
+
+template <int IO, int VEC, int kJoinThreads>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(JoinArgs j) {
+  if (blockIdx.x < j.units) join_splits<IO, VEC, kJoinThreads>(j.part[0], blockIdx.x);
+  else join_splits<IO, VEC, kJoinThreads>(j.part[1], blockIdx.x - j.units);
 }
 
 GeomBytes bytes_of(const Geom &g, int esize) {
@@ -167,13 +179,11 @@ void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t r
   a->split_steps = (int)((tokens + 64 * (int64_t)a->splits - 1) / (64 * (int64_t)a->splits));
 }
 
-// Up to two launches: sequences of few and of many new tokens.
+// Up to two parts: sequences of many new tokens, and of few beside them.
 struct Plan {
-  struct Part {
-    AttentionArgs a;
-    Kind kind;
-  } part[2];
+  AttentionPart part[2];
   int parts;
+  Kind kind;  // of the first; a second one is kFew
   bool vt;
   bool grouped;
   uint64_t workspace;
@@ -276,8 +286,8 @@ Plan make_plan(const AttentionPlan &p) {
   a.most_rows = 0x7FFFFFFF;
   Plan r{};
   auto add = [&](Kind kind, const AttentionArgs &x) -> AttentionArgs & {
+    if (r.parts == 0) r.kind = kind;
     r.part[r.parts].a = x;
-    r.part[r.parts].kind = kind;
     return r.part[r.parts++].a;
   };
   const bool cores = matrix_cores(p);
@@ -285,8 +295,8 @@ Plan make_plan(const AttentionPlan &p) {
   // its tiles (8 sequences of 7 tokens at 8192, groups of 4: 91 us, with the
   // other kernel 122; 64 of them at 2048: 164 and 145; with three tiles, 12
   // tokens, 236 and 139).  How many new tokens each has is known here where
-  // there is one sequence, one token each, or a hint that bounds all; else both
-  // kernels run and each takes its own.
+  // there is one sequence, one token each, or a hint that bounds all; else one
+  // launch has workgroups of both kinds and each kind takes its own.
   const int few = a.group >= 2 * kRowTile ? 1 : 2 * kRowTile / a.group;
   const bool all_few = a.qptr == nullptr || a.tokens <= few ||
                        (p.max_query_len > 0 && p.max_query_len <= few);
@@ -336,14 +346,24 @@ Plan make_plan(const AttentionPlan &p) {
 
 // Few splits are joined by one wave a row and head, many by four.
 template <int IO>
-void launch_join(const AttentionArgs &a, hipStream_t s) {
-  const dim3 units((uint32_t)(join_rows(a) * a.heads * a.group));
+void launch_join(const Plan &p, hipStream_t s) {
+  JoinArgs j{};
+  uint32_t units = 0;
+  int splits = 1;
+  for (int i = 0; i < p.parts; ++i) {
+    const AttentionArgs &a = p.part[i].a;
+    j.part[i] = a;
+    splits = std::max(splits, a.splits);
+    if (a.splits > 1) units += (uint32_t)(join_rows(a) * a.heads * a.group);
+    if (i == 0) j.units = units;
+  }
+  if (units == 0) return;
   auto go = [&](auto vec) {
     constexpr int kVec = decltype(vec)::value;
-    if (a.splits <= 16) attention_join_kernel<IO, kVec, 64><<<units, 64, 0, s>>>(a);
-    else attention_join_kernel<IO, kVec, kMostSplits><<<units, kMostSplits, 0, s>>>(a);
+    if (splits <= 16) attention_join_kernel<IO, kVec, 64><<<dim3(units), 64, 0, s>>>(j);
+    else attention_join_kernel<IO, kVec, kMostSplits><<<dim3(units), kMostSplits, 0, s>>>(j);
   };
-  if (a.head_dim % 4 == 0) go(std::integral_constant<int, 4>{});
+  if (p.part[0].a.head_dim % 4 == 0) go(std::integral_constant<int, 4>{});
   else go(std::integral_constant<int, 1>{});
 }
 
@@ -352,35 +372,37 @@ int64_t workgroups(const AttentionArgs &a) {
 }
 
 bool launchable(const Plan &p) {
+  int64_t grid = 0, units = 0;
   for (int i = 0; i < p.parts; ++i) {
     const AttentionArgs &a = p.part[i].a;
-    if (a.splits > 1 && join_rows(a) * a.heads * a.group * kMostSplits > 0xFFFFFF00ll) return false;
-    if (workgroups(a) * 256 > 0xFFFFFFFFll) return false;
-    if (p.part[i].kind == kRows && (int64_t)a.heads * a.head_tiles > 65535) return false;
+    if (a.splits > 1) units += join_rows(a) * a.heads * a.group;
+    grid += workgroups(a);
+    if (p.kind == kRows && (int64_t)a.heads * a.head_tiles > 65535) return false;
   }
-  return true;
+  return units * kMostSplits <= 0xFFFFFF00ll && grid * 256 <= 0xFFFFFFFFll;
 }
 
-void run_part(const Plan::Part &p, bool vt, bool grouped, int io, int cache, hipStream_t s) {
-  const int64_t grid = workgroups(p.a);
+void run_parts(Plan &p, int io, int cache, hipStream_t s) {
   const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
+  for (int i = 0; i < p.parts; ++i) p.part[i].grid = (uint32_t)workgroups(p.part[i].a);
+  const AttentionPart &a = p.part[0], *few = p.parts > 1 ? &p.part[1] : nullptr;
   if (p.kind == kRows)
-    run_attention_rows(p.a, io, cache, s);
+    run_attention_rows(a, io, cache, s);
   else if (p.kind == kFew && io == KVX_DTYPE_F32)
     (e4 ? run_attention_few_f32_e4m3 : e5 ? run_attention_few_f32_e5m2
-                                          : run_attention_few_f32)(p.a, vt, grouped, grid, s);
+                                          : run_attention_few_f32)(a, p.vt, p.grouped, s);
   else if (p.kind == kFew && io == KVX_DTYPE_BF16)
     (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
-                                           : run_attention_few_bf16)(p.a, vt, grouped, grid, s);
+                                           : run_attention_few_bf16)(a, p.vt, p.grouped, s);
   else if (p.kind == kFew)
     (e4 ? run_attention_few_f16_e4m3 : e5 ? run_attention_few_f16_e5m2
-                                          : run_attention_few_f16)(p.a, vt, grouped, grid, s);
+                                          : run_attention_few_f16)(a, p.vt, p.grouped, s);
   else if (io == KVX_DTYPE_BF16)
     (e4 ? run_attention_many_bf16_e4m3 : e5 ? run_attention_many_bf16_e5m2
-                                            : run_attention_many_bf16)(p.a, vt, grouped, grid, s);
+                                            : run_attention_many_bf16)(a, few, p.vt, p.grouped, s);
   else
     (e4 ? run_attention_many_f16_e4m3 : e5 ? run_attention_many_f16_e5m2
-                                           : run_attention_many_f16)(p.a, vt, grouped, grid, s);
+                                           : run_attention_many_f16)(a, few, p.vt, p.grouped, s);
 }
 
 }  // namespace
@@ -391,17 +413,13 @@ using namespace dev;
 uint64_t attention_workspace(const AttentionPlan &p) { return make_plan(p).workspace; }
 
 kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
-  const Plan plan = make_plan(p);
+  Plan plan = make_plan(p);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!launchable(plan)) return KVX_STATUS_UNSUPPORTED;
-  for (int i = 0; i < plan.parts; ++i) {
-    run_part(plan.part[i], plan.vt, plan.grouped, p.g.io_dtype, p.g.cache_dtype, s);
-    const AttentionArgs &a = plan.part[i].a;
-    if (a.splits == 1) continue;
-    if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(a, s);
-    else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(a, s);
-    else launch_join<KVX_DTYPE_BF16>(a, s);
-  }
+  run_parts(plan, p.g.io_dtype, p.g.cache_dtype, s);
+  if (p.g.io_dtype == KVX_DTYPE_F32) launch_join<KVX_DTYPE_F32>(plan, s);
+  else if (p.g.io_dtype == KVX_DTYPE_F16) launch_join<KVX_DTYPE_F16>(plan, s);
+  else launch_join<KVX_DTYPE_BF16>(plan, s);
   return hipGetLastError() == hipSuccess ? KVX_STATUS_OK : KVX_STATUS_INTERNAL_ERROR;
 }
 

@@ -55,12 +55,19 @@ constexpr int kFewThreads = kFewWaves * kWave;
 // Token e of a lane's eight in a step, from its group's first.
 __device__ __forceinline__ constexpr int place_of(int e) { return e < 4 ? e : 12 + e; }
 
-// IO: type of queries and of the products; C: the cache's type; DP: head_dim
-// rounded up to 64, 128 or 256; VT: values with the token axis innermost;
-// INDEXED: scales by block.
+template <int DP>
+struct FewShared {
+  float sums[2][kRowTile][DP + 4];
+  float states[kFewWaves][2][kRowTile];
+  int infinities;  // see add_infinities
+};
+
+// Workgroup `id` of its grid.  IO: type of queries and of the products; C: the
+// cache's type; DP: head_dim rounded up to 64, 128 or 256; VT: values with the
+// token axis innermost; INDEXED: scales by block.
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
-__global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
-    attention_few_kernel(AttentionArgs a) {
+__device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t id,
+                                              FewShared<DP> &shared) {
   constexpr bool kFp8 = C != IO, kF32 = IO == KVX_DTYPE_F32;
   constexpr int E = bytes_of_type<C>();
   constexpr int KC = kF32 ? DP / 16 : DP / 32;  // operands of a half step's logits
@@ -72,12 +79,11 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
   constexpr int kFewStep = 16 * HALVES;  // tokens
   constexpr uint32_t kAll = 0xFFFFFFFFu >> (32 - kFewStep);
   constexpr int VW = VB / 4;           // dwords (VT: of four tokens)
-  __shared__ float sums[2][kRowTile][DP + 4];
-  __shared__ float states[kFewWaves][2][kRowTile];
-  __shared__ int infinities;  // see add_infinities
+  auto &sums = shared.sums;
+  auto &states = shared.states;
+  int &infinities = shared.infinities;
 
   const int hh = a.heads * a.head_tiles;
-  uint32_t id = blockIdx.x;
   const int y = (int)(id % (uint32_t)hh);
   id /= (uint32_t)hh;
   const int z = (int)(id % (uint32_t)a.splits);
@@ -592,16 +598,17 @@ __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
   add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kFewStep);
 }
 
-template <int IO, int C>
-void launch_few(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hipStream_t s) {
-  const dim3 b((uint32_t)grid);
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
+__global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
+    attention_few_kernel(AttentionArgs a) {
+  __shared__ FewShared<DP> shared;
+  attention_few<IO, C, DP, VT, INDEXED, GROUPED>(a, blockIdx.x, shared);
+}
+
+// go(DP, VT, INDEXED, GROUPED) with the constants that a call needs.
+template <int IO, int C, typename F>
+void with_variant(const AttentionArgs &a, bool vt, bool grouped, const F &go) {
   const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
-  auto go = [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
-    constexpr int kDim = decltype(dp)::value;
-    constexpr bool kIndexed = decltype(indexed_)::value;
-    attention_few_kernel<IO, C, kDim, decltype(vt_)::value, kIndexed, decltype(grouped_)::value>
-        <<<b, kFewThreads, 0, s>>>(a);
-  };
   auto by_dim = [&](auto vt_, auto indexed_, auto grouped_) {
     if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_, grouped_);
     else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_, grouped_);
@@ -619,6 +626,15 @@ void launch_few(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hip
   };
   if (grouped) by_values(std::true_type{});
   else by_values(std::false_type{});
+}
+
+template <int IO, int C>
+void launch_few(const AttentionPart &p, bool vt, bool grouped, hipStream_t s) {
+  with_variant<IO, C>(p.a, vt, grouped, [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
+    attention_few_kernel<IO, C, decltype(dp)::value, decltype(vt_)::value,
+                         decltype(indexed_)::value, decltype(grouped_)::value>
+        <<<dim3(p.grid), kFewThreads, 0, s>>>(p.a);
+  });
 }
 
 }  // namespace dev

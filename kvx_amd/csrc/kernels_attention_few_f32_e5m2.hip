@@ -4,9 +4,8 @@
 namespace kvx {
 namespace dev {
 
-void run_attention_few_f32_e5m2(const AttentionArgs &a, bool vt, bool grouped, int64_t grid,
-                                 hipStream_t s) {
-  launch_few<KVX_DTYPE_F32, KVX_DTYPE_F8_E5M2>(a, vt, grouped, grid, s);
+void run_attention_few_f32_e5m2(const AttentionPart &p, bool vt, bool grouped, hipStream_t s) {
+  launch_few<KVX_DTYPE_F32, KVX_DTYPE_F8_E5M2>(p, vt, grouped, s);
 }
 
 }  // namespace dev

@@ -24,12 +24,18 @@
 //   each; it is put off until a maximum has grown by more than 8 (weights then
 //   reach 2^8, which changes neither their relative rounding nor the F32 sums).
 //
+// Measured: a chunk of 8192 tokens, 8 kv heads of 128, groups of 4, BF16: 583 us
+// (940 TFLOP/s); chunks of 2048 tokens at 4096 to 8192: 326 us (798 TFLOP/s).
+// Matrix and vector instructions of a SIMD's two waves add up to nearly all of
+// it: they overlap little.  The next step's products written between the weights
+// of this one ran slower (402 us for 340), and the products' priority gives 2 %.
+//
 // LDS rows are not padded; the 16-byte chunks of a row are permuted by the
 // token's number, so that the 8 lanes that read one element range of 8 keys
 // (and the 16 that transpose 4 values) meet all banks.
 #pragma once
 
-#include "attention_mfma.h"
+#include "kernels_attention_few.h"
 
 namespace kvx {
 namespace dev {
@@ -86,9 +92,9 @@ __device__ __forceinline__ u32x2 lds_transposed(const lds_char *at) {
                                        (__attribute__((address_space(3))) s16x4 *)(at)));
 }
 
+// Workgroup `id` of its grid.
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
-__global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : 2)
-attention_many_kernel(AttentionArgs a) {
+__device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t id, char *lds) {
   constexpr bool kFp8 = C != IO;
   constexpr int E = kFp8 ? 1 : 2;
   constexpr int KC = DP / 16;                   // products of 32 tokens' logits
@@ -100,7 +106,6 @@ attention_many_kernel(AttentionArgs a) {
   constexpr int NVL = VT ? DP / 32 : NL;        // value loads (VT: 8 tokens of an element)
   constexpr int VLB = VT ? 8 * E : 16;
   constexpr int TENSOR = kManyStep * ROW;
-  extern __shared__ __align__(1024) char lds[];
   constexpr int BUFFER = 2 * TENSOR;  // keys, then values
   float *const scales = reinterpret_cast<float *>(lds + NB * BUFFER);  // [buffer][k, v][64]
   int *const infinities =
@@ -108,7 +113,6 @@ attention_many_kernel(AttentionArgs a) {
 
   // The last tiles of a causal chunk see most tokens: they start first.
   const int hh = a.heads * a.head_tiles;
-  uint32_t id = blockIdx.x;
   const int y = (int)(id % (uint32_t)hh);
   id /= (uint32_t)hh;
   const int z = (int)(id % (uint32_t)a.splits);
@@ -609,11 +613,35 @@ attention_many_kernel(AttentionArgs a) {
     add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kManyStep);
 }
 
+// A batch's sequences of few new tokens, beside the ones of many: their
+// workgroups start first, and wait for memory while the others compute (12
+// sequences, 8 of 100 to 500 new tokens with a window of 1024, 4 kv heads of 64:
+// 55 us with the join, 64 as two launches; a chunk that is alone takes 1 to 4 %
+// longer for the code that it does not run).
+// Heads of 64: three waves a SIMD (10 chunks of 256 tokens at 2048, FP8: 90 us,
+// 126 with two).
+struct MixedArgs {
+  AttentionArgs many, few;
+  uint32_t few_grid;
+};
+
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
+__global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : DP == 128 ? 2 : 3)
+    attention_many_kernel(MixedArgs x) {
+  extern __shared__ __align__(1024) char lds[];
+  static_assert(sizeof(FewShared<DP>) <= many_lds<DP, INDEXED>() && kFewThreads == kManyThreads);
+  if (blockIdx.x < x.few_grid)
+    attention_few<IO, C, DP, VT, INDEXED, GROUPED>(x.few, blockIdx.x,
+                                                   *reinterpret_cast<FewShared<DP> *>(lds));
+  else
+    attention_many<IO, C, DP, VT, INDEXED, GROUPED>(x.many, blockIdx.x - x.few_grid, lds);
+}
+
+// few: null where no sequence can have few new tokens.
 template <int IO, int C>
-void launch_many(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hipStream_t s) {
-  const dim3 b((uint32_t)grid);
-  const bool indexed = C != IO && (a.ks.s_block != 0 || a.vs.s_block != 0);
-  auto go = [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
+void launch_many(const AttentionPart &p, const AttentionPart *few, bool vt, bool grouped,
+                 hipStream_t s) {
+  with_variant<IO, C>(p.a, vt, grouped, [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
     constexpr int kDim = decltype(dp)::value;
     constexpr bool kIndexed = decltype(indexed_)::value;
     constexpr size_t kLds = many_lds<kDim, kIndexed>();
@@ -622,25 +650,9 @@ void launch_many(const AttentionArgs &a, bool vt, bool grouped, int64_t grid, hi
     if (kLds > 65536)  // more than a kernel has unasked
       (void)hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)kLds);
-    kernel<<<b, kManyThreads, kLds, s>>>(a);
-  };
-  auto by_dim = [&](auto vt_, auto indexed_, auto grouped_) {
-    if (a.head_dim <= 64) go(std::integral_constant<int, 64>{}, vt_, indexed_, grouped_);
-    else if (a.head_dim <= 128) go(std::integral_constant<int, 128>{}, vt_, indexed_, grouped_);
-    else go(std::integral_constant<int, 256>{}, vt_, indexed_, grouped_);
-  };
-  auto by_scale = [&](auto vt_, auto grouped_) {
-    if constexpr (C != IO) {
-      if (indexed) return by_dim(vt_, std::true_type{}, grouped_);
-    }
-    by_dim(vt_, std::false_type{}, grouped_);
-  };
-  auto by_values = [&](auto grouped_) {
-    if (vt) by_scale(std::true_type{}, grouped_);
-    else by_scale(std::false_type{}, grouped_);
-  };
-  if (grouped) by_values(std::true_type{});
-  else by_values(std::false_type{});
+    const MixedArgs x{p.a, few ? few->a : p.a, few ? few->grid : 0};
+    kernel<<<dim3(p.grid + x.few_grid), kManyThreads, kLds, s>>>(x);
+  });
 }
 
 }  // namespace dev

@@ -255,7 +255,8 @@ void launch_rows_io(const AttentionArgs &a, int cache, hipStream_t s) {
 
 }  // namespace
 
-void run_attention_rows(const AttentionArgs &a, int io, int cache, hipStream_t s) {
+void run_attention_rows(const AttentionPart &p, int io, int cache, hipStream_t s) {
+  const AttentionArgs &a = p.a;
   if (io == KVX_DTYPE_F32) launch_rows_io<KVX_DTYPE_F32>(a, cache, s);
   else if (io == KVX_DTYPE_F16) launch_rows_io<KVX_DTYPE_F16>(a, cache, s);
   else launch_rows_io<KVX_DTYPE_BF16>(a, cache, s);
