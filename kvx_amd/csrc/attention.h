@@ -34,6 +34,8 @@ constexpr int kManyRowTile = 128;  // and of the one for many
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+constexpr int kDies = 8;  // that take workgroups in turn
+
 struct AttentionArgs {
   // cache and table
   const char *k, *v;
@@ -64,6 +66,7 @@ struct AttentionArgs {
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
   int32_t splits;
   int32_t split_steps;  // least steps of 64 tokens in a split
+  int32_t heads_near;  // the heads of a tile's part run on one die (few rows)
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
   float *part_ml;     // the same without head_dim: (maximum, sum of weights)

@@ -179,6 +179,12 @@ void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t r
   a->split_steps = (int)((tokens + 64 * (int64_t)a->splits - 1) / (64 * (int64_t)a->splits));
 }
 
+int64_t workgroups(const AttentionArgs &a) {
+  int64_t parts = (int64_t)a.tiles * a.splits;
+  if (a.heads_near) parts = (parts + kDies - 1) / kDies * kDies;
+  return parts * a.heads * a.head_tiles;
+}
+
 // Up to two parts: sequences of many new tokens, and of few beside them.
 struct Plan {
   AttentionPart part[2];
@@ -318,6 +324,19 @@ Plan make_plan(const AttentionPlan &p) {
     AttentionArgs &x = add(kFew, a);
     tile_rows(&x, kRowTile);
     split_tokens(p, &x, kFew, x.tokens);
+    // Heads that share 128-byte lines run on one die, or each die would read
+    // their lines (200 sequences of 1000 tokens, 8 FP8 heads of 64: 53 us, 74
+    // spread over the dies).  Heads of one line are better off together too
+    // where there are more workgroups than the machine holds (of 128: 89 and 99
+    // us; 16 sequences of 4096 tokens: 38 and 37), wider ones are not (BF16 of
+    // 128: 160 and 158).  Two tiles of a sequence would part instead (164 us
+    // become 201), so that this is for sequences of one.
+    const bool one = a.qptr == nullptr || (p.max_query_len > 0 && p.max_query_len <= x.tile_tokens);
+    const auto near_lines = [&](const GeomBytes &g) {
+      const int64_t s = g.s_head < 0 ? -g.s_head : g.s_head;
+      return s < 256 && (s % 128 != 0 || workgroups(x) > 512);
+    };
+    x.heads_near = one && a.heads > 1 && near_lines(a.gk) && near_lines(a.gv);
   } else {
     AttentionArgs &x = add(kMany, a);
     tile_rows(&x, kManyRowTile);
@@ -365,10 +384,6 @@ void launch_join(const Plan &p, hipStream_t s) {
   };
   if (p.part[0].a.head_dim % 4 == 0) go(std::integral_constant<int, 4>{});
   else go(std::integral_constant<int, 1>{});
-}
-
-int64_t workgroups(const AttentionArgs &a) {
-  return (int64_t)a.tiles * a.splits * a.heads * a.head_tiles;
 }
 
 bool launchable(const Plan &p) {

@@ -33,7 +33,8 @@
 // of 256: 242, and 584 with 32 tokens, for which there are no registers).
 //
 // Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16
-// 96 us (5.6 TB/s), FP8 59 us (4.5 TB/s), F32 188 us (5.7 TB/s).  More waves a
+// 97 us (5.5 TB/s), FP8 60 us (4.5 TB/s), F32 188 us (5.7 TB/s); 200 of 4000
+// tokens, FP8: 320 us (5.1 TB/s).  More waves a
 // SIMD in fewer registers spill: BF16 at three 142 us.  Sequences whose rows need
 // two tiles read their keys and values twice, from L2 the second time: with 8
 // tokens each 165 us.
@@ -83,12 +84,20 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
   auto &states = shared.states;
   int &infinities = shared.infinities;
 
-  const int hh = a.heads * a.head_tiles;
-  const int y = (int)(id % (uint32_t)hh);
-  id /= (uint32_t)hh;
+  // Heads in turn, or (heads_near) eight tiles' parts in turn: one for each die.
+  const uint32_t hh = (uint32_t)(a.heads * a.head_tiles);
+  int y;
+  if (a.heads_near) {
+    y = (int)(id / kDies % hh);
+    id = id / (kDies * hh) * kDies + id % kDies;
+  } else {
+    y = (int)(id % hh);
+    id /= hh;
+  }
   const int z = (int)(id % (uint32_t)a.splits);
+  const int tile = (int)(id / (uint32_t)a.splits);
   QueryTile t;
-  if (!find_tile(a, (int)(id / (uint32_t)a.splits), &t)) return;
+  if (tile >= a.tiles || !find_tile(a, tile, &t)) return;
   const int lane = (int)(threadIdx.x % kWave);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
   const int c = lane % 16, g = lane / 16;
