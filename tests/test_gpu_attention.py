@@ -371,6 +371,68 @@ def test_graph(new):
         d.check(out=c.out, lse=c.lse)
 
 
+@pytest.mark.parametrize("io,cache", [("bf16", None), ("f16", "e5m2"), ("f32", None)])
+def test_graph_of_wide_heads(io, cache):
+    """Heads of 256 elements, chunks and decoding sequences: the launch that
+    needs the most LDS, captured before any eager call of its kind."""
+    c = AttentionCase(io=io, cache=cache, lens=[300, 40, 2000], new=[90, 1, 3], D=256, H=1, G=4)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert c.run() == Status.OK
+    for _ in range(3):
+        c.out.fill_(7.0)
+        c.lse.fill_(7.0)
+        graph.replay()
+        c.check()
+
+
+@pytest.mark.parametrize("new", [None, [1, 30, 2]])
+@pytest.mark.parametrize("share", [1.0, 0.5])
+def test_pools_of_known_size(new, share):
+    """KV_OFFSETS with `pool_blocks`: entries past a pool's blocks are not
+    there."""
+    c = AttentionCase(io="bf16", table="offsets", lens=[70, 33, 200], new=new, D=64)
+    blocks = max(int(2 * c.nb * share) // 2 * 2, 2)
+
+    def rows_of(s):
+        n = c.lens[s]
+        b = c.tb[s].repeat_interleave(c.bs)[:n]
+        there = (b >= 0) & (2 * b + 1 < blocks)
+        o = torch.arange(n) % c.bs
+        b = b.clamp(0, c.nb - 1)
+        return c.exact[0][b, o], c.exact[1][b, o], there
+
+    c.rows_of = rows_of
+    assert c.run(pool_blocks=(blocks, 0)) == Status.OK
+    c.check()
+
+
+@pytest.mark.parametrize("seqs", [1, 7, 9, 200])
+@pytest.mark.parametrize("hint", [0, 1])
+def test_narrow_heads_of_many_sequences(seqs, hint):
+    """Heads that share lines run on one die: any number of sequences, with
+    and without the query offsets."""
+    lens = [1 + (37 * i) % 90 for i in range(seqs)]
+    c = AttentionCase(io="bf16", cache="e4m3", lens=lens, H=3, G=2, D=48, bs=16,
+                      new=[1] * seqs if hint else None)
+    assert c.run(max_query_len=hint) == Status.OK
+    c.check()
+    c = AttentionCase(io="f16", lens=lens, H=3, G=2, D=24, new=[1] * seqs if hint else None)
+    assert c.run(max_query_len=hint) == Status.OK
+    c.check()
+
+
+def test_more_sequences_than_one_scan():
+    """Tiles are numbered over 256 sequences at a time: chunks far behind many
+    short or empty ones."""
+    new = [(1, 0, 3, 20)[i % 4] for i in range(700)]
+    new[650] = 150
+    c = AttentionCase(io="bf16", lens=[n + i % 5 for i, n in enumerate(new)], new=new, H=1, G=2,
+                      D=64)
+    assert c.run() == Status.OK
+    c.check()
+
+
 def test_two_graphs_do_not_share_memory():
     a = AttentionCase(lens=[2500], D=128, H=1, seed=1)
     b = AttentionCase(lens=[2600], D=128, H=1, seed=2)
