@@ -315,6 +315,7 @@ __device__ __forceinline__ void wave_sync() {
 struct AttentionPart {
   AttentionArgs a;
   uint32_t grid;  // workgroups
+  bool stream;    // few rows: no two tiles read the same keys and values
 };
 
 void run_attention_rows(const AttentionPart &p, int io, int cache, hipStream_t s);

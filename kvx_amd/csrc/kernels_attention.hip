@@ -190,6 +190,7 @@ struct Plan {
   AttentionPart part[2];
   int parts;
   Kind kind;  // of the first; a second one is kFew
+  bool many;  // there is a kernel for many rows
   bool vt;
   bool grouped;
   uint64_t workspace;
@@ -299,7 +300,7 @@ Plan make_plan(const AttentionPlan &p) {
   const bool cores = matrix_cores(p);
   // Sequences of at most `few` new tokens go to the kernel for few rows: two of
   // its tiles (8 sequences of 7 tokens at 8192, groups of 4: 91 us, with the
-  // other kernel 122; 64 of them at 2048: 164 and 145; with three tiles, 12
+  // other kernel 122; 64 of them at 2048: 133 and 145; with three tiles, 12
   // tokens, 236 and 139).  How many new tokens each has is known here where
   // there is one sequence, one token each, or a hint that bounds all; else one
   // launch has workgroups of both kinds and each kind takes its own.
@@ -314,13 +315,14 @@ Plan make_plan(const AttentionPlan &p) {
               steps_fit(g.gv);
   const bool few_ok = cores && values_fit(p, kFew, &r.vt);
   bool vt_many = false;
-  const bool many_ok = few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) && vt_many == r.vt;
+  r.many = few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) &&
+           vt_many == r.vt;
   if (!few_ok) {
     AttentionArgs &x = add(kRows, a);
     tile_rows(&x, kRowTile);
     x.chunk_k = chunks(p, g.gk, g.src_k, 4);
     split_tokens(p, &x, kRows, x.tokens);
-  } else if (all_few || !many_ok) {
+  } else if (all_few || !r.many) {
     AttentionArgs &x = add(kFew, a);
     tile_rows(&x, kRowTile);
     split_tokens(p, &x, kFew, x.tokens);
@@ -331,7 +333,9 @@ Plan make_plan(const AttentionPlan &p) {
     // us; 16 sequences of 4096 tokens: 38 and 37), wider ones are not (BF16 of
     // 128: 160 and 158).  Two tiles of a sequence would part instead (164 us
     // become 201), so that this is for sequences of one.
-    const bool one = a.qptr == nullptr || (p.max_query_len > 0 && p.max_query_len <= x.tile_tokens);
+    const bool one = x.head_tiles == 1 && (x.qptr == nullptr || (p.max_query_len > 0 &&
+                                                                 p.max_query_len <= x.tile_tokens));
+    r.part[0].stream = one || !(r.many || g.io_dtype == KVX_DTYPE_F32);
     const auto near_lines = [&](const GeomBytes &g) {
       const int64_t s = g.s_head < 0 ? -g.s_head : g.s_head;
       return s < 256 && (s % 128 != 0 || workgroups(x) > 512);
@@ -400,16 +404,21 @@ bool launchable(const Plan &p) {
 void run_parts(Plan &p, int io, int cache, hipStream_t s) {
   const bool e4 = cache == KVX_DTYPE_F8_E4M3, e5 = cache == KVX_DTYPE_F8_E5M2;
   for (int i = 0; i < p.parts; ++i) p.part[i].grid = (uint32_t)workgroups(p.part[i].a);
-  const AttentionPart &a = p.part[0], *few = p.parts > 1 ? &p.part[1] : nullptr;
+  AttentionPart a = p.part[0];
+  const AttentionPart *few = p.parts > 1 ? &p.part[1] : nullptr;
+  if (p.kind == kFew && !a.stream && io != KVX_DTYPE_F32) {  // the unstreamed kernel is there
+    few = &p.part[0];
+    a.grid = 0;
+  }
   if (p.kind == kRows)
     run_attention_rows(a, io, cache, s);
   else if (p.kind == kFew && io == KVX_DTYPE_F32)
     (e4 ? run_attention_few_f32_e4m3 : e5 ? run_attention_few_f32_e5m2
                                           : run_attention_few_f32)(a, p.vt, p.grouped, s);
-  else if (p.kind == kFew && io == KVX_DTYPE_BF16)
+  else if (p.kind == kFew && p.part[0].stream && io == KVX_DTYPE_BF16)
     (e4 ? run_attention_few_bf16_e4m3 : e5 ? run_attention_few_bf16_e5m2
                                            : run_attention_few_bf16)(a, p.vt, p.grouped, s);
-  else if (p.kind == kFew)
+  else if (p.kind == kFew && p.part[0].stream)
     (e4 ? run_attention_few_f16_e4m3 : e5 ? run_attention_few_f16_e5m2
                                           : run_attention_few_f16)(a, p.vt, p.grouped, s);
   else if (io == KVX_DTYPE_BF16)

@@ -35,9 +35,12 @@
 // Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16
 // 97 us (5.5 TB/s), FP8 60 us (4.5 TB/s), F32 188 us (5.7 TB/s); 200 of 4000
 // tokens, FP8: 320 us (5.1 TB/s).  More waves a
-// SIMD in fewer registers spill: BF16 at three 142 us.  Sequences whose rows need
-// two tiles read their keys and values twice, from L2 the second time: with 8
-// tokens each 165 us.
+// SIMD in fewer registers spill: BF16 at three 142 us.
+//
+// Keys and values that one tile reads are streamed past the caches (5 sequences
+// of 16384 to 32768 tokens: 85 us, 94 without), unless a sequence may have two
+// tiles, whose second reads come from L2 then (64 sequences of 2048 with 8 new
+// tokens each: 133 us, 165 streamed).
 //
 // Maximum and sum are one register each, as a lane has one row; the maximum
 // is shared over the four lane groups, the sum only at the end.  Weights are
@@ -65,8 +68,9 @@ struct FewShared {
 
 // Workgroup `id` of its grid.  IO: type of queries and of the products; C: the
 // cache's type; DP: head_dim rounded up to 64, 128 or 256; VT: values with the
-// token axis innermost; INDEXED: scales by block.
-template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
+// token axis innermost; INDEXED: scales by block; GROUPED: blocks hold whole
+// groups of 16 tokens; STREAM: keys and values are read past the caches.
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED, bool STREAM>
 __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t id,
                                               FewShared<DP> &shared) {
   constexpr bool kFp8 = C != IO, kF32 = IO == KVX_DTYPE_F32;
@@ -220,7 +224,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
     auto one = [&](int b, uint64_t p, uint32_t row) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) {
-        const Raw<16> r = global_load<16, true>(p, row + koff[i]);
+        const Raw<16> r = global_load<16, STREAM>(p, row + koff[i]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) kw[b][i][j] = r.w[j];
       }
@@ -244,7 +248,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
             const uint64_t p = from_lane(s.rows.v, 16 * g + 64 * b + 4 * e);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-              const Raw<VLB> r = global_load<VLB, true>(p, voff[j]);
+              const Raw<VLB> r = global_load<VLB, STREAM>(p, voff[j]);
 #pragma unroll
               for (int w = 0; w < E; ++w) {
                 const uint32_t mine = token_bits<E>(e, w);
@@ -263,7 +267,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
         else p = from_lane(s.rows.v, 16 * g + 64 * b);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const Raw<VLB> r = global_load<VLB, true>(p, (GROUPED ? 4 * g * E : 0) + voff[j]);
+          const Raw<VLB> r = global_load<VLB, STREAM>(p, (GROUPED ? 4 * g * E : 0) + voff[j]);
 #pragma unroll
           for (int w = 0; w < E; ++w) vw[b * NV + j][w] = r.w[w];
         }
@@ -272,7 +276,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
       auto one = [&](int e, uint64_t p, uint32_t row) {
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-          const Raw<VLB> r = global_load<VLB, true>(p, row + voff[i]);
+          const Raw<VLB> r = global_load<VLB, STREAM>(p, row + voff[i]);
 #pragma unroll
           for (int w = 0; w < VLB / 4; ++w) vw[e][i * (VLB / 4) + w] = r.w[w];
         }
@@ -607,11 +611,11 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
   add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kFewStep);
 }
 
-template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
+template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED, bool STREAM>
 __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
     attention_few_kernel(AttentionArgs a) {
   __shared__ FewShared<DP> shared;
-  attention_few<IO, C, DP, VT, INDEXED, GROUPED>(a, blockIdx.x, shared);
+  attention_few<IO, C, DP, VT, INDEXED, GROUPED, STREAM>(a, blockIdx.x, shared);
 }
 
 // go(DP, VT, INDEXED, GROUPED) with the constants that a call needs.
@@ -640,8 +644,15 @@ void with_variant(const AttentionArgs &a, bool vt, bool grouped, const F &go) {
 template <int IO, int C>
 void launch_few(const AttentionPart &p, bool vt, bool grouped, hipStream_t s) {
   with_variant<IO, C>(p.a, vt, grouped, [&](auto dp, auto vt_, auto indexed_, auto grouped_) {
-    attention_few_kernel<IO, C, decltype(dp)::value, decltype(vt_)::value,
-                         decltype(indexed_)::value, decltype(grouped_)::value>
+    constexpr int kDim = decltype(dp)::value;
+    constexpr bool kVt = decltype(vt_)::value, kIndexed = decltype(indexed_)::value;
+    constexpr bool kGrouped = decltype(grouped_)::value;
+    if constexpr (IO == KVX_DTYPE_F32) {  // others: launch_many
+      if (!p.stream)
+        return attention_few_kernel<IO, C, kDim, kVt, kIndexed, kGrouped, false>
+            <<<dim3(p.grid), kFewThreads, 0, s>>>(p.a);
+    }
+    attention_few_kernel<IO, C, kDim, kVt, kIndexed, kGrouped, true>
         <<<dim3(p.grid), kFewThreads, 0, s>>>(p.a);
   });
 }

@@ -631,13 +631,14 @@ __global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : DP == 128 ? 2 : 
   extern __shared__ __align__(1024) char lds[];
   static_assert(sizeof(FewShared<DP>) <= many_lds<DP, INDEXED>() && kFewThreads == kManyThreads);
   if (blockIdx.x < x.few_grid)
-    attention_few<IO, C, DP, VT, INDEXED, GROUPED>(x.few, blockIdx.x,
-                                                   *reinterpret_cast<FewShared<DP> *>(lds));
+    attention_few<IO, C, DP, VT, INDEXED, GROUPED, false>(
+        x.few, blockIdx.x, *reinterpret_cast<FewShared<DP> *>(lds));
   else
     attention_many<IO, C, DP, VT, INDEXED, GROUPED>(x.many, blockIdx.x - x.few_grid, lds);
 }
 
-// few: null where no sequence can have few new tokens.
+// few: null where no sequence can have few new tokens; p.grid: 0 where none can
+// have many.
 template <int IO, int C>
 void launch_many(const AttentionPart &p, const AttentionPart *few, bool vt, bool grouped,
                  hipStream_t s) {
