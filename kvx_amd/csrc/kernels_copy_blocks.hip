@@ -7,6 +7,10 @@
 // kernel arguments, so that a fork's few pages cost one launch instead of one
 // for each layer.  Other blocks (padded axes, a block axis that is not
 // outermost) are copied element by element through their strides.
+//
+// Measured, 64 tensors (32 layers) of 32 KiB blocks: 400 pairs 318 us (5.3 TB/s;
+// a library copy of 2 GiB reaches 4.9), 2 pairs 3.4 us in the kernel and 10.7 us
+// a call, which the host's walk over the layers takes.
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"

@@ -16,6 +16,11 @@
 // position of a million still has its angle to 1e-9), whole turns dropped,
 // the rest split into f32 and a correction that enters by the first term of
 // the addition theorem: cosines and sines are right to about one unit of f32.
+//
+// Measured: 32768 tokens of 32 + 8 + 8 heads of 128, BF16, 163 us (4.9 TB/s);
+// 4 tokens 5.2 us, 251 into an FP8 cache 7.2 us, where a launch's latency is
+// nearly all.  With one query and one key head a token's angles cost more than
+// its bytes (90000 tokens into FP8: 82 us, 1.4 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"
