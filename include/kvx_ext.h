@@ -165,7 +165,7 @@ typedef struct kvx_attention_desc {
   kvx_tensor_desc_t query; /* [num_tokens, query_heads, head_dim], F16/BF16/F32, the
                               cache's dtype unless that is FP8; elements of a head
                               adjacent, any other strides */
-  kvx_tensor_desc_t out;   /* same shape and dtype */
+  kvx_tensor_desc_t out;   /* same shape and dtype; may be the query itself */
   float *lse;              /* F32 [num_tokens, query_heads], or NULL */
   const void *query_indptr; /* [seq_count + 1] row numbers, or NULL */
   kvx_dtype_t query_indptr_dtype; /* S32 or S64 */

@@ -239,7 +239,8 @@ bool values_fit(const AttentionPlan &p, Kind kind, bool *vt) {
   return !*vt || tokens_inner(p, kind == kMany ? 8 : 4);
 }
 
-Plan make_plan(const AttentionPlan &p) {
+// most: the kernel for the largest chunks that may be taken.
+Plan make_plan(const AttentionPlan &p, Kind most) {
   const GatherPlan &g = p.g;
   const int cs = dtype_size((kvx_dtype_t)g.cache_dtype), is = dtype_size((kvx_dtype_t)g.io_dtype);
   AttentionArgs a{};
@@ -313,9 +314,9 @@ Plan make_plan(const AttentionPlan &p) {
   auto steps_fit = [&](const Geom &x) { return x.s_off >= 0 && x.s_off * cs < (1 << 24); };
   r.grouped = g.block_size % 16 == 0 && g.format != KVX_BLOCK_TABLE_RAGGED && steps_fit(g.gk) &&
               steps_fit(g.gv);
-  const bool few_ok = cores && values_fit(p, kFew, &r.vt);
+  const bool few_ok = most != kRows && cores && values_fit(p, kFew, &r.vt);
   bool vt_many = false;
-  r.many = few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) &&
+  r.many = most == kMany && few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) &&
            vt_many == r.vt;
   if (!few_ok) {
     AttentionArgs &x = add(kRows, a);
@@ -434,10 +435,22 @@ void run_parts(Plan &p, int io, int cache, hipStream_t s) {
 
 using namespace dev;
 
-uint64_t attention_workspace(const AttentionPlan &p) { return make_plan(p).workspace; }
+uint64_t attention_workspace(const AttentionPlan &p) { return make_plan(p, kMany).workspace; }
+
+// Enough whatever kernels the alignment of the call's tensors allows.
+uint64_t attention_workspace_bound(const AttentionPlan &p) {
+  AttentionPlan x = p;  // as if everything were aligned: all pointers null
+  x.query = nullptr;
+  x.out = nullptr;
+  x.g.src_k = x.g.src_v = nullptr;
+  x.g.pool[0] = x.g.pool[1] = nullptr;
+  uint64_t bytes = 0;
+  for (const Kind most : {kRows, kFew, kMany}) bytes = std::max(bytes, make_plan(x, most).workspace);
+  return bytes;
+}
 
 kvx_status_t enqueue_attention(const AttentionPlan &p, void *stream) {
-  Plan plan = make_plan(p);
+  Plan plan = make_plan(p, kMany);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (!launchable(plan)) return KVX_STATUS_UNSUPPORTED;
   run_parts(plan, p.g.io_dtype, p.g.cache_dtype, s);

@@ -169,6 +169,7 @@ kvx_status_t enqueue_copy_blocks(const CopyTensor *tensors, int64_t count, const
 // Bytes of workspace that enqueue_attention uses for the plan (its pointers
 // are not read).
 uint64_t attention_workspace(const AttentionPlan &plan);
+uint64_t attention_workspace_bound(const AttentionPlan &p);  // for any alignment
 
 // Checks and conversions that the entry points share (launch.cpp).
 bool is_io_float(kvx_dtype_t dt);

@@ -4,6 +4,7 @@
 // checks itself.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <vector>
 
 #include "kvx_ext.h"
@@ -175,7 +176,7 @@ static kvx_status_t plan_attention(const kvx_cache_desc_t *cache, const kvx_atte
   if (a->flags & ~(uint32_t)KVX_ATTENTION_CAUSAL) return KVX_STATUS_INVALID_ARGUMENT;
   const bool causal = (a->flags & KVX_ATTENTION_CAUSAL) != 0;
   if (a->window > kMost32 || (a->window > 0 && !causal)) return KVX_STATUS_INVALID_ARGUMENT;
-  if (!(a->softcap >= 0.0f) || a->max_seq_len > kMost32 || a->max_query_len > kMost32)
+  if (!(a->softcap >= 0.0f) || std::isinf(a->softcap) || a->max_seq_len > kMost32 || a->max_query_len > kMost32)
     return KVX_STATUS_INVALID_ARGUMENT;
   if (D > 512) return KVX_STATUS_UNSUPPORTED;
   GatherPlan &g = p->g;
@@ -312,7 +313,7 @@ KVX_API kvx_status_t kvx_attention_workspace_size(const kvx_cache_desc_t *cache,
   bool empty = false;
   const kvx_status_t st = kvx::plan_attention(cache, attention, false, &p, &empty);
   if (st != KVX_STATUS_OK) return st;
-  *out_bytes = empty ? 0 : kvx::attention_workspace(p);
+  *out_bytes = empty ? 0 : kvx::attention_workspace_bound(p);
   return KVX_STATUS_OK;
 }
 

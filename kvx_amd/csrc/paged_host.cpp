@@ -372,6 +372,13 @@ bool is_index(const at::Tensor &t) {
          t.is_contiguous();
 }
 
+// Scales (null: none) that kernels can read.
+bool are_scales(std::initializer_list<const at::Tensor *> scales) {
+  for (const at::Tensor *t : scales)
+    if (t != nullptr && t->scalar_type() != at::ScalarType::Float) return false;
+  return here(scales);
+}
+
 bool is_line(const at::Tensor &t, int64_t n) { return is_index(t) && t.dim() == 1 && t.size(0) == n; }
 
 // The cache's tensors, which come next among the arguments.
@@ -406,7 +413,7 @@ PyObject *host_rope_write(Args a) {
   const at::Tensor *vs = a.tensor_or_none();
   const int64_t vg = a.number();
   if (!a.ok || a.at != a.n || (q == nullptr) != (o == nullptr) ||
-      !here({q, o, key, value, pos, inv, slots}) || key->dim() != 3 || value->dim() != 3 ||
+      !here({q, o, key, value, pos, inv, slots}) || !are_scales({ks, vs}) || key->dim() != 3 || value->dim() != 3 ||
       (q != nullptr && (q->dim() != 3 || o->dim() != 3)) || !is_line(*pos, key->size(0)) ||
       !is_line(*slots, key->size(0)) || inv->scalar_type() != at::ScalarType::Float ||
       !inv->is_contiguous() || !fits32(key->size(0)) || !fits32(key->size(1)) ||
@@ -480,6 +487,7 @@ PyObject *host_attention(Args a) {
   const at::Tensor *workspace = a.tensor_or_none();
   if (!a.ok || a.at != a.n ||
       !here({q, o, table, indptr, primary, secondary, lens, rows, lse, workspace}) ||
+      !are_scales({ks, vs}) ||
       q->dim() != 3 || o->dim() != 3 || !is_index(*table) || !is_index(*lens) ||
       (indptr != nullptr && !is_index(*indptr)))
     Py_RETURN_NONE;

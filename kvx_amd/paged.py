@@ -546,6 +546,17 @@ def _indices(name: str, t: torch.Tensor, shape: tuple | None = None) -> torch.Te
     return t
 
 
+def _check_scales(device: torch.device, **scales) -> None:
+    for name, scale in scales.items():
+        t = scale.values if isinstance(scale, Scales) else scale
+        if t is None:
+            continue
+        if t.dtype != torch.float32:
+            raise ValueError(f"{name} is {t.dtype}, not float32")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+
+
 def _row_tensor(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dim() != 3:
         raise ValueError(f"{name} is not [tokens, heads, head_dim]")
@@ -596,6 +607,7 @@ def rope_write_kv(cache: PagedCache, query: torch.Tensor | None, key: torch.Tens
     device = _on_one_gpu(cache.key_cache, value_cache=cache.value_cache, query=query, key=key,
                          value=value, positions=positions, inv_freq=rope.inv_freq,
                          slot_mapping=slot_mapping, query_out=query_out)
+    _check_scales(device, k_scale=k_scale, v_scale=v_scale)
     T = _row_tensor("key", key).shape[0]
     _row_tensor("value", value)
     if query is not None:
@@ -629,7 +641,7 @@ def build_attention(query: torch.Tensor, out: torch.Tensor, block_table, seq_len
         d.query_indptr = query_indptr.data_ptr()
         d.query_indptr_dtype = int(dtype_code(query_indptr))
     d.window = window
-    d.scale = query.shape[-1] ** -0.5 if scale is None else scale
+    d.scale = max(query.shape[-1], 1) ** -0.5 if scale is None else scale
     d.softcap = softcap
     d.max_seq_len = max_seq_len
     d.max_query_len = max_query_len
@@ -656,7 +668,7 @@ def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_t
     seq_lens[s] cached tokens, the new ones last.  A row at position p attends
     to the tokens up to p (`causal`; else to all), with a `window` only to the
     last `window` of them.  softmax(scale * q.k) v goes to `out` (like
-    `query`), the natural logarithm of the weights' sum to `lse` (float32 [T,
+    `query`, or the query itself), the natural logarithm of the weights' sum to `lse` (float32 [T,
     Hq], or None); `scale` is 1 / sqrt(D) unless given; `softcap` > 0 turns a
     logit x into softcap * tanh(x / softcap).  Hq is a multiple of the cache's
     heads.  Rows that attend to nothing are 0 with lse -inf; rows behind the
@@ -669,14 +681,16 @@ def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_t
     may run at the same time; None allocates it.  kvx_launch_attention."""
     lib = abi.load()
     host = _host()
+    if scale is None:
+        scale = max(_row_tensor("query", query).shape[2], 1) ** -0.5
     if host and type(cache) is PagedCache and pool_blocks is None:
         code = host.attention(
             _address(lib, "kvx_launch_attention"),
             _address(lib, "kvx_attention_workspace_size"),
             None if stream is None else _stream_handle(stream), *_cache_args(cache), query, out,
             *_table_args(block_table), seq_lens, query_indptr, 1 if causal else 0,
-            query.shape[-1] ** -0.5 if scale is None else scale, window, softcap, lse,
-            max_seq_len, max_query_len, *_scale_args(k_scale), *_scale_args(v_scale), workspace)
+            scale, window, softcap, lse, max_seq_len, max_query_len, *_scale_args(k_scale),
+            *_scale_args(v_scale), workspace)
         if code is not None:
             return _STATUS[code]
     # what the native builder leaves to the descriptor helpers
@@ -690,10 +704,11 @@ def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_t
         table_tensors = {"block_table": _indices("block_table", block_table)}
         if block_table.dim() != 2:
             raise ValueError("block_table is not [sequences, blocks]")
+    _row_tensor("query", query)
     device = _on_one_gpu(cache.key_cache, value_cache=cache.value_cache, query=query, out=out,
                          seq_lens=seq_lens, query_indptr=query_indptr, lse=lse,
                          workspace=workspace, **table_tensors)
-    _row_tensor("query", query)
+    _check_scales(device, k_scale=k_scale, v_scale=v_scale)
     _row_tensor("out", out)
     cd = gather_cache_desc(cache, block_table)
     d = build_attention(query, out, block_table, seq_lens, query_indptr, causal=causal,

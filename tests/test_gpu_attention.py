@@ -455,6 +455,43 @@ def test_two_graphs_do_not_share_memory():
         b.check()
 
 
+@pytest.mark.parametrize("io,cache", [("bf16", None), ("f32", None), ("f16", "e4m3")])
+@pytest.mark.parametrize("new", [None, [7, 1, 90]])
+def test_output_in_place_of_the_query(io, cache, new):
+    c = AttentionCase(io=io, cache=cache, lens=[3000, 200, 90], new=new, D=64, H=1)
+    assert c.run(q=c.q_dev, out=c.q_dev) == Status.OK
+    c.check(out=c.q_dev)
+
+
+@pytest.mark.parametrize("new", [None, [1, 90]])
+def test_workspace_size_holds_for_any_alignment(new):
+    """The size is asked for with aligned tensors; the call's lie otherwise and
+    take other kernels."""
+    c = AttentionCase(lens=[5000, 900], new=new, D=128, H=1, G=2)
+    size = paged.attention_workspace_size(c.cache, c.q_dev, c.table, c.lens_t, c.indptr,
+                                          max_seq_len=5000, max_query_len=max(c.new))
+    w = torch.empty(size, dtype=torch.uint8, device="cuda")
+    flat = torch.full((c.out.numel() + 1,), 7.0, dtype=c.out.dtype, device="cuda")
+    out = flat[1:].view(c.out.shape)
+    assert c.run(out=out, workspace=w) == Status.OK
+    c.check(out=out)
+
+
+def test_refused_scales():
+    c = AttentionCase(io="bf16", cache="e4m3", lens=[40, 30], D=64)
+    good = torch.ones(1, device="cuda")
+    for bad in (good.cpu(), good.half(), good.double()):
+        for kw in (dict(k_scale=bad, v_scale=good), dict(k_scale=good, v_scale=bad)):
+            with pytest.raises(ValueError):
+                c.run(**kw)
+            with pytest.raises(ValueError):
+                x = c.q_dev[:, :2].contiguous()
+                i = torch.zeros(2, dtype=torch.int64, device="cuda")
+                paged.rope_write_kv(c.cache, None, x, x, i,
+                                    paged.Rope(torch.ones(32, device="cuda")), i, **kw)
+    assert (c.out == 7.0).all()
+
+
 def test_refusals_on_device():
     c = AttentionCase(lens=[40, 30], D=64)
     with pytest.raises(ValueError):

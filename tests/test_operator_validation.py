@@ -105,6 +105,11 @@ def test_attention_arguments(kvx_lib):
     assert A(L, c, attn()) == UNS
 
 
+def test_attention_softcap_is_finite(kvx_lib):
+    assert A(kvx_lib, cache(), attn(softcap=math.inf)) == INV
+    assert A(kvx_lib, cache(), attn(softcap=3e38)) == OK
+
+
 def test_attention_tables(kvx_lib):
     L = kvx_lib
     a = attn()
