@@ -155,7 +155,7 @@ enum Kind { kRows, kFew, kMany };
 // few tiles (8 kv heads, us, whole and in parts of 128: one chunk of 100 tokens
 // at 1000 tokens 37 and 25, of 512 at 512 24 and 35).
 // Sequences of different lengths even out over a few rounds of workgroups, so
-// that parts of 2048 tokens at least are made for up to 3072 of them (5
+// that parts of 2048 tokens at least are made for up to 3200 of them (5
 // sequences of 16384 to 32768 tokens: 97 us at 512 workgroups, 86 at 640).
 // `rows`: rows of partial sums per query head.
 void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t rows) {
@@ -171,7 +171,7 @@ void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t r
   const int64_t least =
       kind == kMany ? std::min<int64_t>(std::max<int64_t>(4 * units, 128), 512) : 256;
   int64_t n = tokens < 4 * least ? 1 : std::min(512 / units, tokens / least);
-  if (kind != kMany) n = std::max(n, std::min(3072 / units, tokens / 2048));
+  if (kind != kMany) n = std::max(n, std::min(3200 / units, tokens / 2048));
   // partial sums of at most 1 GiB
   const int64_t each = rows * a->heads * a->group * (a->head_dim + 2) * 4;
   if (n * each > ((int64_t)1 << 30)) n = ((int64_t)1 << 30) / each;
