@@ -10,8 +10,12 @@
 // its kernel takes), so that the ones that are left over lie together.
 // Scattered among the others they would cost far more than their own time:
 // workgroups go round the machine in order, and a part of it would get all of
-// them and run empty (64 sequences of 4 drafts at
-// 2048 tokens: 155 us instead of 99).
+// them and run empty (64 sequences of 4 drafts at 2048 tokens: 155 us instead of
+// 99).  Counting many sequences takes time as well: where they are said to have
+// one tile each, or are more than 256 and have few rows, the first tile of each
+// has the sequence's number and only further ones are counted (1024 sequences
+// of one token at 200: 223 us instead of 291, without the hint 252 instead of
+// 307).
 //
 // Splits.  Where the tiles alone do not fill the machine, a tile's tokens are
 // divided among `splits` workgroups.  Each writes its unnormalised sum, its
@@ -66,6 +70,7 @@ struct AttentionArgs {
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
   int32_t splits;
   int32_t split_steps;  // least steps of 64 tokens in a split
+  int32_t first_tiles; // each sequence's first tile has its number, others follow
   int32_t heads_near;  // the heads of a tile's part run on one die (few rows)
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
@@ -111,22 +116,45 @@ __device__ __forceinline__ int last_sequence(int seqs, const F &before) {
 }
 
 // The sequence and rows of a tile, or false behind the last one.  A lane counts
-// the tiles of four sequences, whose sums the wave scans.
-__device__ __forceinline__ bool find_rows(const AttentionArgs &a, int tile, QueryTile *t) {
-  constexpr int kEach = 4;
+// the tiles of kEach sequences, without the first `skip` of each, and the wave
+// scans the sums.
+template <int kEach>
+__device__ __forceinline__ bool find_rows(const AttentionArgs &a, int tile, int skip,
+                                          QueryTile *t) {
   const int lane = (int)(threadIdx.x % kWave);
   int left = tile;  // behind the tiles counted so far
   for (int s0 = 0; s0 < a.seqs; s0 += kEach * kWave) {
     const int s = s0 + kEach * lane;
     int64_t begin[kEach + 1];
     int count[kEach], sum = 0;
+    if (kEach > 4 && s + kEach <= a.seqs) {
+      // 16 bytes a load: a lane's numbers one by one would be a line each
+      const int bytes = a.qptr64 ? 8 : 4;
+      const char *p = static_cast<const char *>(a.qptr) + (int64_t)s * bytes;
 #pragma unroll
-    for (int i = 0; i <= kEach; ++i) begin[i] = query_begin(a, min(s + i, a.seqs));
+      for (int i = 0; i < kEach; i += 4) {
+        Raw<16> lo, hi{};
+        __builtin_memcpy(&lo, p + i * bytes, 16);
+        if (a.qptr64) __builtin_memcpy(&hi, p + i * bytes + 16, 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const Raw<16> &r = k < 2 ? lo : hi;
+          const int64_t x = a.qptr64 ? (int64_t)((uint64_t)r.w[k % 2 * 2 + 1] << 32 | r.w[k % 2 * 2])
+                                     : (int64_t)(int32_t)lo.w[k];
+          begin[i + k] = x < 0 ? 0 : x > a.tokens ? a.tokens : x;
+        }
+      }
+      begin[kEach] = query_begin(a, s + kEach);
+    } else {
+#pragma unroll
+      for (int i = 0; i <= kEach; ++i) begin[i] = query_begin(a, min(s + i, a.seqs));
+    }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int64_t n = begin[i + 1] - begin[i];
       const bool mine = n > 0 && n >= a.least_rows && n <= a.most_rows;
-      count[i] = mine ? (int)((uint32_t)(n + a.tile_tokens - 1) / (uint32_t)a.tile_tokens) : 0;
+      count[i] =
+          mine ? (int)((uint32_t)(n + a.tile_tokens - 1) / (uint32_t)a.tile_tokens) - skip : 0;
       sum += count[i];
     }
     int upto = sum;
@@ -146,7 +174,7 @@ __device__ __forceinline__ bool find_rows(const AttentionArgs &a, int tile, Quer
           t->seq = s0 + kEach * from + i;
           t->begin = b;
           t->rows = __builtin_amdgcn_readlane((int)begin[i + 1], from) - b;
-          t->first = left * a.tile_tokens;
+          t->first = (left + skip) * a.tile_tokens;
           t->count = min(a.tile_tokens, t->rows - t->first);
           return true;
         }
@@ -167,8 +195,18 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
     t->count = 1;
     t->begin = tile;
     t->rows = 1;
-  } else if (!find_rows(a, tile, t)) {
-    return false;
+  } else if (a.first_tiles && tile < a.seqs) {
+    const int64_t b = query_begin(a, tile), n = query_begin(a, tile + 1) - b;
+    if (n <= 0 || n < a.least_rows || n > a.most_rows) return false;
+    t->seq = tile;
+    t->first = 0;
+    t->count = (int32_t)min(n, (int64_t)a.tile_tokens);
+    t->begin = b;
+    t->rows = (int32_t)n;
+  } else {
+    const int skip = a.first_tiles ? 1 : 0, left = tile - skip * a.seqs;
+    if (a.seqs <= 4 * kWave ? !find_rows<4>(a, left, skip, t) : !find_rows<16>(a, left, skip, t))
+      return false;
   }
   t->length = index_at(a.lens, a.lens64, t->seq);
   int64_t hold, first;

@@ -159,10 +159,11 @@ enum Kind { kRows, kFew, kMany };
 // sequences of 16384 to 32768 tokens: 97 us at 512 workgroups, 86 at 640).
 // `rows`: rows of partial sums per query head.
 void split_tokens(const AttentionPlan &p, AttentionArgs *a, Kind kind, int64_t rows) {
-  // about as many tiles as there are: sequences that another kernel takes are
-  // the short ones where `least_rows` says so
+  // about as many tiles as there are: of many rows, between full ones and a part
+  // of one in each sequence
   int64_t tiles = a->qptr == nullptr ? a->seqs : a->tokens / a->tile_tokens;
-  if (a->least_rows == 0) tiles = std::max<int64_t>(tiles, a->seqs);
+  if (a->least_rows > 0) tiles = (tiles + a->tiles) / 2;
+  else tiles = std::max<int64_t>(tiles, a->seqs);
   tiles = std::min<int64_t>(tiles, a->tiles);
   const int64_t units = std::max<int64_t>(tiles * a->heads * a->head_tiles, 1);
   int64_t tokens = longest(p);  // that a tile sees
@@ -341,11 +342,16 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
       const int64_t s = g.s_head < 0 ? -g.s_head : g.s_head;
       return s < 256 && (s % 128 != 0 || workgroups(x) > 512);
     };
+    x.first_tiles = one;
     x.heads_near = one && a.heads > 1 && near_lines(a.gk) && near_lines(a.gv);
   } else {
     AttentionArgs &x = add(kMany, a);
     tile_rows(&x, kManyRowTile);
-    if (!all_many) x.least_rows = few + 1;
+    if (!all_many) {
+      x.least_rows = few + 1;
+      // no more sequences than that have so many tokens
+      x.tiles = x.tokens / x.tile_tokens + std::min(x.seqs, x.tokens / x.least_rows);
+    }
     split_tokens(p, &x, kMany, x.tokens);
     if (!all_many) {
       AttentionArgs &y = add(kFew, a);
@@ -354,6 +360,7 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
       y.part_rows = few;
       const int64_t most = (int64_t)y.seqs * ((few + y.tile_tokens - 1) / y.tile_tokens);
       y.tiles = (int)std::min<int64_t>(y.tiles, most);
+      y.first_tiles = y.seqs > 256;
       split_tokens(p, &y, kFew, (int64_t)y.seqs * few);
     }
   }

@@ -455,6 +455,19 @@ def test_two_graphs_do_not_share_memory():
         b.check()
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("seqs", [255, 257, 1030])
+@pytest.mark.parametrize("most", [1, 12])
+def test_tiles_of_many_sequences(seqs, most, dtype):
+    """However tiles are numbered, also with a hint that is too small."""
+    new = [(i * 7 + i // 3) % (most + 1) for i in range(seqs)]
+    for hint in (0, most, 1):
+        c = AttentionCase(io="bf16", lens=[n + i % 4 for i, n in enumerate(new)], new=new, H=1,
+                          G=4, D=32, index=dtype, indptr_dtype=dtype, extra_rows=3)
+        assert c.run(max_query_len=hint) == Status.OK
+        c.check()
+
+
 @pytest.mark.parametrize("io,cache", [("bf16", None), ("f32", None), ("f16", "e4m3")])
 @pytest.mark.parametrize("new", [None, [7, 1, 90]])
 def test_output_in_place_of_the_query(io, cache, new):
