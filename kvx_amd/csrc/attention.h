@@ -14,7 +14,7 @@
 // 99).  Counting many sequences takes time as well: where they are said to have
 // one tile each, or are more than 256 and have few rows, the first tile of each
 // has the sequence's number and only further ones are counted (1024 sequences
-// of one token at 200: 223 us instead of 291, without the hint 252 instead of
+// of one token at 200: 226 us instead of 291, without the hint 252 instead of
 // 307).
 //
 // Splits.  Where the tiles alone do not fill the machine, a tile's tokens are
@@ -65,6 +65,7 @@ struct AttentionArgs {
   int32_t causal, window;
   float scale_log2;  // scale * log2 e
   float cap, cap_in; // softcap * log2 e and scale / softcap; cap 0: none
+  float scale_rest, cap_rest;  // what rounding left of scale_log2 and cap
   // tiles
   int32_t tile_heads, head_tiles, tile_tokens, tiles;
   int32_t least_rows, most_rows;  // new tokens of the sequences this kernel takes
@@ -116,39 +117,19 @@ __device__ __forceinline__ int last_sequence(int seqs, const F &before) {
 }
 
 // The sequence and rows of a tile, or false behind the last one.  A lane counts
-// the tiles of kEach sequences, without the first `skip` of each, and the wave
+// the tiles of four sequences, without the first `skip` of each, and the wave
 // scans the sums.
-template <int kEach>
 __device__ __forceinline__ bool find_rows(const AttentionArgs &a, int tile, int skip,
                                           QueryTile *t) {
+  constexpr int kEach = 4;
   const int lane = (int)(threadIdx.x % kWave);
   int left = tile;  // behind the tiles counted so far
   for (int s0 = 0; s0 < a.seqs; s0 += kEach * kWave) {
     const int s = s0 + kEach * lane;
     int64_t begin[kEach + 1];
     int count[kEach], sum = 0;
-    if (kEach > 4 && s + kEach <= a.seqs) {
-      // 16 bytes a load: a lane's numbers one by one would be a line each
-      const int bytes = a.qptr64 ? 8 : 4;
-      const char *p = static_cast<const char *>(a.qptr) + (int64_t)s * bytes;
 #pragma unroll
-      for (int i = 0; i < kEach; i += 4) {
-        Raw<16> lo, hi{};
-        __builtin_memcpy(&lo, p + i * bytes, 16);
-        if (a.qptr64) __builtin_memcpy(&hi, p + i * bytes + 16, 16);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const Raw<16> &r = k < 2 ? lo : hi;
-          const int64_t x = a.qptr64 ? (int64_t)((uint64_t)r.w[k % 2 * 2 + 1] << 32 | r.w[k % 2 * 2])
-                                     : (int64_t)(int32_t)lo.w[k];
-          begin[i + k] = x < 0 ? 0 : x > a.tokens ? a.tokens : x;
-        }
-      }
-      begin[kEach] = query_begin(a, s + kEach);
-    } else {
-#pragma unroll
-      for (int i = 0; i <= kEach; ++i) begin[i] = query_begin(a, min(s + i, a.seqs));
-    }
+    for (int i = 0; i <= kEach; ++i) begin[i] = query_begin(a, min(s + i, a.seqs));
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int64_t n = begin[i + 1] - begin[i];
@@ -204,9 +185,8 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs &a, int tile, Quer
     t->begin = b;
     t->rows = (int32_t)n;
   } else {
-    const int skip = a.first_tiles ? 1 : 0, left = tile - skip * a.seqs;
-    if (a.seqs <= 4 * kWave ? !find_rows<4>(a, left, skip, t) : !find_rows<16>(a, left, skip, t))
-      return false;
+    const int skip = a.first_tiles ? 1 : 0;
+    if (!find_rows(a, tile - skip * a.seqs, skip, t)) return false;
   }
   t->length = index_at(a.lens, a.lens64, t->seq);
   int64_t hold, first;

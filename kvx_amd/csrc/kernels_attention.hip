@@ -12,6 +12,7 @@ namespace dev {
 namespace {
 
 constexpr int kMostSplits = 256;
+constexpr double kLog2eWide = 1.44269504088896340736;
 
 // Rows that have partial sums.
 __host__ __device__ __forceinline__ int64_t join_rows(const AttentionArgs &a) {
@@ -290,6 +291,8 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
   a.window = p.window;
   a.scale_log2 = p.scale * kLog2e;
   a.cap = p.softcap * kLog2e;
+  a.scale_rest = (float)((double)p.scale * kLog2eWide - (double)a.scale_log2);
+  a.cap_rest = (float)((double)p.softcap * kLog2eWide - (double)a.cap);
   a.cap_in = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
   a.least_rows = 0;
   a.most_rows = 0x7FFFFFFF;

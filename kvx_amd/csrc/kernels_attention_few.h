@@ -29,11 +29,11 @@
 // the product 4 i + w with the query's element of that place; values need no
 // transposition, a product takes tokens 4 g + i of the four groups.  Wide F32
 // rows take steps of 16 tokens, so that two waves a SIMD have registers (heads
-// of 128, 16 sequences of 4096 tokens: 102 us, 111 with 32 tokens and one wave;
+// of 128, 16 sequences of 4096 tokens: 107 us, 111 with 32 tokens and one wave;
 // of 256: 242, and 584 with 32 tokens, for which there are no registers).
 //
 // Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16
-// 97 us (5.5 TB/s), FP8 60 us (4.5 TB/s), F32 188 us (5.7 TB/s); 200 of 4000
+// 97 us (5.5 TB/s), FP8 60 us (4.5 TB/s), F32 196 us (5.5 TB/s); 200 of 4000
 // tokens, FP8: 320 us (5.1 TB/s).  More waves a
 // SIMD in fewer registers spill: BF16 at three 142 us.
 //
@@ -168,7 +168,17 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
     vs = scale_of(a.vs, 0, kvh);
   }
 
-  const float scale = positive_scale<IO>(a, ks, q);
+  // F32: the factor's rest too, or all logits would be off by its rounding.
+  float scale = positive_scale<IO>(a, ks, q), scale_rest = 0.0f;
+  if constexpr (kF32) {
+    const float hi = a.cap != 0.0f ? a.cap : a.scale_log2, by = a.cap != 0.0f ? 1.0f : ks;
+    const float product = hi * by;
+    if (product != 0.0f) {
+      scale = fabsf(product);
+      scale_rest = fmaf(hi, by, -product) + (a.cap != 0.0f ? a.cap_rest : a.scale_rest) * by;
+      scale_rest = product < 0.0f ? -scale_rest : scale_rest;
+    }
+  }
   float m = -INFINITY, l = 0.0f, vref = 0.0f;
   f32x4 acc[NV];
 #pragma unroll
@@ -390,7 +400,8 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
       }
       if (a.cap != 0.0f) {
 #pragma unroll
-        for (int e = 0; e < 4 * HALVES; ++e) x[e] = capped(a, x[e] * ks);
+        for (int e = 0; e < 4 * HALVES; ++e)
+          x[e] = kF32 ? tanhf(x[e] * ks * a.cap_in) : capped(a, x[e] * ks);
       }
       if (!whole) {
         const uint32_t there = now.there >> (4 * g);
@@ -417,7 +428,9 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
       m = top;
 #pragma unroll
       for (int e = 0; e < 4 * HALVES; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(x[e], scale, -shift));
+        float y = fmaf(x[e], scale, -shift);
+        if constexpr (kF32) y += fmaxf(x[e], -3e38f) * scale_rest;  // no infinity by 0
+        p[e] = __builtin_amdgcn_exp2f(y);
         l += p[e];
       }
       if constexpr (INDEXED) {

@@ -9,7 +9,7 @@
 // weights a token from LDS, again broadcasts.  Each key or value element is
 // used 16 times per load, in F32 throughout; LDS and the vector unit bound it
 // (16 sequences of 4096 tokens, 8 kv heads of 100 F32: 336 us, 1.2 TB/s; where
-// the matrix cores can be used, heads of 128 take 102).
+// the matrix cores can be used, heads of 128 take 107).
 #include <hip/hip_runtime.h>
 
 #include "attention.h"
