@@ -25,7 +25,7 @@
 //   reach 2^8, which changes neither their relative rounding nor the F32 sums).
 //
 // Measured: a chunk of 8192 tokens, 8 kv heads of 128, groups of 4, BF16: 583 us
-// (940 TFLOP/s); chunks of 2048 tokens at 4096 to 8192: 326 us (798 TFLOP/s).
+// (940 TFLOP/s); chunks of 2048 tokens at 4096 to 8192: 323 us (805 TFLOP/s).
 // Matrix and vector instructions of a SIMD's two waves add up to nearly all of
 // it: they overlap little.  The next step's products written between the weights
 // of this one ran slower (402 us for 340), and the products' priority gives 2 %.
