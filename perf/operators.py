@@ -447,8 +447,8 @@ def _rope_inputs(case, seed):
     # The pool holds each sequence's last pages, and as many others.
     bs = case["block"]
     first = (positions[nth == 0] // bs)
-    table, pool = _block_table(case, [int(n) - int(f) * bs for n, f in zip(lens, first)], seed)
-    blocks = max(pool, 2 * int((table >= 0).sum()))
+    table, _ = _block_table(case, [int(n) - int(f) * bs for n, f in zip(lens, first)], seed)
+    blocks = 2 * int((table >= 0).sum())
     slots = table[seq, positions // bs - first[seq]] * bs + positions % bs
     pad = torch.randperm(total, generator=torch.Generator().manual_seed(case["lens_seed"]))
     slots[pad[: case["padded"]]] = -1
