@@ -302,6 +302,9 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
   auto store = [&](const Step &s, Staged &staged, int base, int buffer) {
     char *kb = lds + buffer * BUFFER, *vb = kb + TENSOR;
     if (!plain(s, base)) {
+      // the steps that add_infinities looks at again: missing tokens alone are no
+      // reason to take anything out of the others
+      const bool partly = base < last_lo || base + kManyStep > first_hi;
       uint32_t odd = 0;
 #pragma unroll
       for (int l = 0; l < NVL; ++l) {
@@ -320,8 +323,8 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
                    ((have >> (4 * w)) & 4 ? 0xFF0000u : 0u) |
                    ((have >> (4 * w)) & 8 ? 0xFF000000u : 0u);
           const uint32_t x = staged.v[l].w[w] & keep;
-          odd |= not_finite<C>(x);
-          staged.v[l].w[w] = only_finite<C>(x);
+          odd |= partly ? not_finite<C>(x) : 0u;
+          staged.v[l].w[w] = partly ? only_finite<C>(x) : x;
         }
       }
       if (odd != 0) *infinities = 1;
