@@ -48,6 +48,12 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Block-indexed scales of values multiply the weights, which the products take in
+// the queries' type.  BF16 and F32 have the range for that; F16 weights carry
+// them relative to a reference, from this one on (values of so small a scale are
+// 0 in an F16 output: 2^-64 * 57344).
+constexpr float kLeastScale = 0x1p-64f;
+
 // Two f32 to two 16-bit elements, to nearest even.
 template <int IO>
 __device__ __forceinline__ uint32_t pair_of(float a, float b) {

@@ -75,6 +75,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
                                               FewShared<DP> &shared) {
   constexpr bool kFp8 = C != IO, kF32 = IO == KVX_DTYPE_F32;
   constexpr int E = bytes_of_type<C>();
+  constexpr bool kRelative = INDEXED && IO == KVX_DTYPE_F16;  // see kLeastScale
   constexpr int KC = kF32 ? DP / 16 : DP / 32;  // operands of a half step's logits
   constexpr int KL = DP * E / 64;      // 16-byte key loads of a token and lane group
   constexpr int NV = DP / 16;          // products of a step's sums; elements a lane loads
@@ -179,7 +180,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
       scale_rest = product < 0.0f ? -scale_rest : scale_rest;
     }
   }
-  float m = -INFINITY, l = 0.0f, vref = 0.0f;
+  float m = -INFINITY, l = 0.0f, vref = kLeastScale;
   f32x4 acc[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -403,6 +404,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
         for (int e = 0; e < 4 * HALVES; ++e)
           x[e] = kF32 ? tanhf(x[e] * ks * a.cap_in) : capped(a, x[e] * ks);
       }
+      uint32_t hidden = 0;  // bit e: this lane's row does not see its token e
       if (!whole) {
         const uint32_t there = now.there >> (4 * g);
         const int start = base + 4 * g;
@@ -411,6 +413,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
           const int at = start + place_of(e);
           const bool seen = ((there >> place_of(e)) & 1) & (at >= rlo) & (at < rhi);
           x[e] = seen ? x[e] : -INFINITY;
+          hidden |= seen ? 0u : 1u << e;
         }
       }
 #pragma unroll
@@ -434,24 +437,35 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
         l += p[e];
       }
       if constexpr (INDEXED) {
-        // Values stay codes; weights carry the tokens' scales, relative to the
-        // largest so far, so that they stay in the type's range.
-        const int in = GROUPED ? lane - now.lane0 : lane;
-        const bool mine_there = in >= 0 && in < (GROUPED ? HALVES : kFewStep) &&
-                                ((now.rows.held >> lane) & 1);
-        float mine = mine_there ? fabsf(now.rows.vs) : 0.0f;
+        // Values stay codes; weights carry the tokens' scales.  A page in front of
+        // the window may have slid out of it and its scale be anything: one that
+        // the row does not see counts as 0, by selection.  F16 weights carry them
+        // relative to the largest that the row saw, so that they stay in the
+        // type's range.
+        float by[4 * HALVES];
 #pragma unroll
-        for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
-        if (mine > vref) {
-          const float ratio = vref / mine;
-#pragma unroll
-          for (int j = 0; j < NV; ++j) acc[j] *= ratio;
-          vref = mine;
+        for (int e = 0; e < 4 * HALVES; ++e) {
+          by[e] = token_scale(now, now.rows.vs, e);
+          by[e] = (hidden >> e) & 1 ? 0.0f : by[e];
         }
-        const float inv = vref > 0.0f ? 1.0f / vref : 0.0f;
+        if constexpr (kRelative) {
+          float most = vref;
 #pragma unroll
-        for (int e = 0; e < 4 * HALVES; ++e)
-          p[e] *= token_scale(now, now.rows.vs, e) * inv;
+          for (int e = 0; e < 4 * HALVES; ++e) most = fmaxf(most, fabsf(by[e]));
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          if (__any(most > vref)) {
+            const float ratio = vref / most;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) acc[j] *= ratio;
+            vref = most;
+          }
+          const float inv = 1.0f / vref;
+#pragma unroll
+          for (int e = 0; e < 4 * HALVES; ++e) by[e] *= inv;
+        }
+#pragma unroll
+        for (int e = 0; e < 4 * HALVES; ++e) p[e] *= by[e];
       }
       if (now.there != kAll) clear_values(now.there);
       if (t.count > 1 && (base < last_lo || base + kFewStep > first_hi)) {
@@ -523,7 +537,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
-  if constexpr (INDEXED) {
+  if constexpr (kRelative) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) acc[j] *= vref;
   }

@@ -96,6 +96,7 @@ __device__ __forceinline__ u32x2 lds_transposed(const lds_char *at) {
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
 __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t id, char *lds) {
   constexpr bool kFp8 = C != IO;
+  constexpr bool kRelative = INDEXED && IO == KVX_DTYPE_F16;  // see kLeastScale
   constexpr int E = kFp8 ? 1 : 2;
   constexpr int KC = DP / 16;                   // products of 32 tokens' logits
   constexpr int NJ = DP / 32;                   // blocks of elements of the sums
@@ -360,7 +361,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
     }
   };
 
-  float m = -INFINITY, l = 0.0f, vref = 0.0f;
+  float m = -INFINITY, l = 0.0f, vref = kLeastScale;
   f32x16 acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x16{};
@@ -403,6 +404,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
     }
     const bool whole = now.there == ~0ull && base >= all_lo && base + kManyStep <= all_hi;
     float top = -INFINITY;
+    uint32_t hidden = 0;  // bit 16 b + i: this lane's row does not see its token i of half b
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       if constexpr (INDEXED) {
@@ -425,6 +427,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
           const int at = 8 * (i / 4) + i % 4;
           const bool seen = ((there >> at) & 1) & (start + at >= rlo) & (start + at < rhi);
           s[b][i] = seen ? s[b][i] : -INFINITY;
+          hidden |= seen ? 0u : 1u << (16 * b + i);
         }
       }
 #pragma unroll
@@ -440,21 +443,32 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
       for (int j = 0; j < NJ; ++j) acc[j] *= alpha;
     }
     const float shift = m == -INFINITY ? 0.0f : m;
-    float inv = 1.0f;
-    if constexpr (INDEXED) {
-      const int in = GROUPED ? lane - now.lane0 : lane;
-      const bool mine_there =
-          in >= 0 && in < (GROUPED ? 4 : kManyStep) && ((now.rows.held >> lane) & 1);
-      float mine = mine_there ? fabsf(now.rows.vs) : 0.0f;
+    // Scales of values by block: see the few-row kernel.
+    auto value_scale = [&](int b, int i) -> f32x4 {
+      f32x4 x = token_scales(now, now.rows.vs, buffer, 1, b, i);
 #pragma unroll
-      for (int d = 1; d < kWave; d *= 2) mine = fmaxf(mine, __shfl_xor(mine, d));
-      if (mine > vref) {
-        const float ratio = vref / mine;
+      for (int k = 0; k < 4; ++k) x[k] = (hidden >> (16 * b + 4 * i + k)) & 1 ? 0.0f : x[k];
+      return x;
+    };
+    float inv = 1.0f;
+    if constexpr (kRelative) {
+      float most = vref;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = value_scale(b, i);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[k]));
+        }
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (__any(most > vref)) {
+        const float ratio = vref / most;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[j] *= ratio;
-        vref = mine;
+        vref = most;
       }
-      inv = vref > 0.0f ? 1.0f / vref : 0.0f;
+      inv = 1.0f / vref;
     }
     Frag w[4];
 #pragma unroll
@@ -470,9 +484,9 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
       if constexpr (INDEXED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = token_scales(now, now.rows.vs, buffer, 1, b, i);
+          const f32x4 x = value_scale(b, i);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[b][4 * i + k] *= x[k] * inv;
+          for (int k = 0; k < 4; ++k) s[b][4 * i + k] *= kRelative ? x[k] * inv : x[k];
         }
       }
 #pragma unroll
@@ -567,7 +581,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
     }
   }
   l += __shfl_xor(l, 32);
-  if constexpr (INDEXED) {
+  if constexpr (kRelative) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] *= vref;
   }

@@ -138,7 +138,8 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(AttentionA
       l[r] = l[r] * alpha + wave_sum(p);
 #pragma unroll
       for (int j = 0; j < DJ; ++j) acc[r][j] *= alpha;
-      pw[lane * kRowTile + r] = p * vs;
+      // a page that the row does not see may have any scale
+      pw[lane * kRowTile + r] = seen ? p * vs : 0.0f;
     }
     wave_sync();
     const int count = min(kWave, to - base);

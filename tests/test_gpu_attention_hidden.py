@@ -1,4 +1,5 @@
-"""What a row of the attention must see, and what it must not: NaN and
+"""What a row of the attention must not see, and what it must: scales of pages
+in front of its window or of nobody, scales that only other rows see, NaN and
 infinities beside missing blocks.  Bounds: operator_helpers.attention_reference."""
 import math
 
@@ -10,6 +11,98 @@ from kvx_amd.abi import Status
 from operator_helpers import AttentionCase, set_rows
 
 pytestmark = pytest.mark.gpu
+
+POISON = (math.nan, math.inf, -math.inf, 1e30)
+
+
+def seen_blocks(c, window):
+    """Blocks with a token that some row attends to."""
+    live = torch.zeros(c.nb, dtype=torch.bool)
+    for s, (n, m) in enumerate(zip(c.lens, c.new)):
+        first = max(n - m + 1 - window, 0) if window else 0
+        live[c.tb[s, first // c.bs: -(-n // c.bs)]] = True
+    return live
+
+
+@pytest.mark.parametrize("table,bs,layout,D", [("packed", 8, "nhd", 64), ("packed", 16, "nhd", 128),
+                                               ("packed", 32, "vllm", 64), ("packed", 16, "hnd", 256),
+                                               ("ragged", 16, "nhd", 64), ("ragged", 8, "vllm", 128),
+                                               ("packed", 8, "nhd", 20)])
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("window", [17, 100])
+@pytest.mark.parametrize("lens,new", [([100, 35, 2600], None), ([200, 35, 2600], [90, 3, 70])])
+def test_scales_of_hidden_pages(lens, new, window, io, table, bs, layout, D):
+    """Pages that slid out of the window, and pages of nobody, have scales that
+    were never written."""
+    for kind in ("block", "block_head"):
+        c = AttentionCase(io=io, cache="e4m3", scales=kind, layout=layout, table=table, bs=bs, H=2,
+                          G=2, D=D, lens=lens, new=new, window=window)
+        dead = (~seen_blocks(c, window)).nonzero()[:, 0]
+        assert dead.numel() > 3
+        for s in c.kv_scales:
+            for i, b in enumerate(dead.tolist()):
+                s.values[b] = POISON[(i + b) % 4]
+        assert c.run() == Status.OK
+        c.check()
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf, 1e30])
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("new", [None, [40, 70]])
+def test_one_kind_of_hidden_scale(io, new, poison):
+    c = AttentionCase(io=io, cache="e5m2", scales="block", H=1, G=4, D=64, lens=[100, 300], new=new,
+                      window=33)
+    dead = ~seen_blocks(c, 33)
+    for s in c.kv_scales:
+        s.values[dead.to("cuda")] = poison
+    assert c.run() == Status.OK
+    c.check()
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("table", ["packed", "ragged"])
+@pytest.mark.parametrize("new,D", [([44], 64), ([7], 128), ([44], 20)])
+def test_scales_that_some_rows_see(new, D, table, io, which, poison):
+    """One page's scale is not finite: rows that attend to a token of it turn
+    so, the others stay what they are.  An infinite scale of keys makes a negative
+    product a logit of -infinity: a token that does not count."""
+    window = 50
+    for block in (11, 8):  # of the new tokens, and leaving the window
+        c = AttentionCase(io=io, cache="e4m3", scales="block", H=2, G=2, D=D, lens=[190], new=new,
+                          window=window, table=table)
+        page = int(c.tb[0, block])
+        c.kv_scales[which].values[page] = poison
+        assert c.run() == Status.OK
+        torch.cuda.synchronize()
+        ref = list(c.reference())
+        rows_of = c.rows_of
+        c.rows_of = lambda s: (*rows_of(s)[:2], torch.arange(190) // 16 != block)
+        without = c.reference()
+        out, lse = c.out.cpu().double(), c.lse.cpu()
+        sees = 0
+        for i in range(new[0]):
+            p = 190 - new[0] + i
+            t = torch.arange(16 * block, 16 * block + 16)
+            t = t[(t <= p) & (t > p - window)] % 16
+            if t.numel() == 0:
+                continue
+            sees += 1
+            for h in range(4):
+                dots = c.rows[0][page, t, h // 2].double() @ c.q[i, h].double()
+                if which == 0 and poison == math.inf and (dots < 0).all():
+                    for x, y in zip(ref, without):
+                        x[i, h] = y[i, h]
+                    continue
+                assert not torch.isfinite(out[i, h]).any()
+                if which == 0:
+                    assert not math.isfinite(lse[i, h])
+                c.out[i, h] = ref[0][i, h].to(c.out.dtype).cuda()
+                c.lse[i, h] = ref[1][i, h].float().cuda()
+        assert sees > 0 or (block == 8 and new[0] == 7)
+        c.reference = lambda: ref
+        c.check()
 
 
 @pytest.mark.parametrize("io,cache", [("bf16", None), ("f16", None), ("f32", None),
