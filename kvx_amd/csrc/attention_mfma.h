@@ -116,18 +116,45 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t w) {
 // rows of a tile see whole, note that there were some, and call this after the
 // tile's outputs are written (and a barrier): it looks at those steps again and
 // adds what they hold to the rows that see it.  A thread has elements of its
-// own, so the additions need no order.  step: tokens of a step; [all_lo, all_hi):
-// tokens that all rows see.
-template <int IO, int C>
-__device__ __forceinline__ void add_infinities(const AttentionArgs &a, const QueryTile &t, int kvh,
-                                            int head0, int nheads, int z, int from, int to, int lo,
-                                            int all_lo, int all_hi, int step) {
+// own, so the additions need no order.  tile, z, y: the workgroup's tile, split,
+// and kv head and part of its group; STEP: tokens of a step; HOLES: they were
+// also taken out of steps some of whose tokens are not there.
+//
+// Not inlined, and with the address of its arguments instead of the caller's
+// copy: what this rare path uses must not wait in scalar registers through the
+// loops before it, which have too few of them.
+template <int IO, int C, int STEP, bool HOLES>
+__device__ __attribute__((noinline)) void add_infinities(uint64_t args, int tile, int z, int y) {
+  args = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)args) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(args >> 32)) << 32;
+  const AttentionArgs &a =
+      *(const AttentionArgs *)(const __attribute__((address_space(4))) AttentionArgs *)args;
+  QueryTile t;
+  if (!find_tile(a, __builtin_amdgcn_readfirstlane(tile), &t)) return;
+  z = __builtin_amdgcn_readfirstlane(z);
+  y = __builtin_amdgcn_readfirstlane(y);
+  const int kvh = y / a.head_tiles;
+  const int head0 = (y - kvh * a.head_tiles) * a.tile_heads;
+  const int nheads = min(a.tile_heads, a.group - head0);
+  int lo, hi, all_lo, all_hi, from, to;  // all rows see [all_lo, all_hi)
+  row_range(a, t, t.first, &lo, &all_hi);
+  row_range(a, t, t.first + t.count - 1, &all_lo, &hi);
+  split_range(a, lo, hi, z, &from, &to);
   for (int d = (int)threadIdx.x; d < a.head_dim; d += (int)blockDim.x) {
     const int64_t at_d = (d / a.gv.pack) * a.gv.s_piece + (d % a.gv.pack) * a.gv.s_inner;
     for (int at = from > lo ? from : lo; at < to; ++at) {
-      const int base = from + (at - from) / step * step;
-      if (base >= all_lo && base + step <= all_hi) continue;
+      const int base = from + (at - from) / STEP * STEP;
       TokenRows r;
+      if (base >= all_lo && base + STEP <= all_hi) {
+        bool whole = true;
+        if constexpr (HOLES)
+          for (int i = base; i < base + STEP; ++i)
+            whole &= token_rows(a, token_entry(a, t, i), i, &r);
+        if (whole) {
+          at = base + STEP - 1;
+          continue;
+        }
+      }
       if (!token_rows(a, token_entry(a, t, at), at, &r)) continue;
       float x = value_at<C>(r.v + kvh * a.gv.s_head + at_d);
       if (fabsf(x) < INFINITY) continue;
@@ -149,6 +176,11 @@ __device__ __forceinline__ void add_infinities(const AttentionArgs &a, const Que
       }
     }
   }
+}
+
+// The address of a kernel's arguments, `offset` bytes into them.
+__device__ __forceinline__ uint64_t args_address(size_t offset) {
+  return reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr()) + offset;
 }
 
 // scale * q.k in units of log2, the scale of an FP8 key included in the

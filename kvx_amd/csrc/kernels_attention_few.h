@@ -66,12 +66,12 @@ struct FewShared {
   int infinities;  // see add_infinities
 };
 
-// Workgroup `id` of its grid.  IO: type of queries and of the products; C: the
+// Workgroup `id` of its grid, whose arguments start at args_at.  IO: type of queries and of the products; C: the
 // cache's type; DP: head_dim rounded up to 64, 128 or 256; VT: values with the
 // token axis innermost; INDEXED: scales by block; GROUPED: blocks hold whole
 // groups of 16 tokens; STREAM: keys and values are read past the caches.
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED, bool STREAM>
-__device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t id,
+__device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t args_at, uint32_t id,
                                               FewShared<DP> &shared) {
   constexpr bool kFp8 = C != IO, kF32 = IO == KVX_DTYPE_F32;
   constexpr int E = bytes_of_type<C>();
@@ -635,14 +635,14 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, uint32_t i
   }
   if (infinities == 0) return;
   __syncthreads();
-  add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kFewStep);
+  add_infinities<IO, C, kFewStep, false>(args_address(args_at), tile, z, y);
 }
 
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED, bool STREAM>
 __global__ void __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2)
     attention_few_kernel(AttentionArgs a) {
   __shared__ FewShared<DP> shared;
-  attention_few<IO, C, DP, VT, INDEXED, GROUPED, STREAM>(a, blockIdx.x, shared);
+  attention_few<IO, C, DP, VT, INDEXED, GROUPED, STREAM>(a, 0, blockIdx.x, shared);
 }
 
 // go(DP, VT, INDEXED, GROUPED) with the constants that a call needs.

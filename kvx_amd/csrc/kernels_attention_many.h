@@ -92,9 +92,10 @@ __device__ __forceinline__ u32x2 lds_transposed(const lds_char *at) {
                                        (__attribute__((address_space(3))) s16x4 *)(at)));
 }
 
-// Workgroup `id` of its grid.
+// Workgroup `id` of its grid, whose arguments start at args_at.
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED>
-__device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t id, char *lds) {
+__device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t args_at, uint32_t id,
+                                               char *lds) {
   constexpr bool kFp8 = C != IO;
   constexpr bool kRelative = INDEXED && IO == KVX_DTYPE_F16;  // see kLeastScale
   constexpr int E = kFp8 ? 1 : 2;
@@ -117,8 +118,9 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
   const int y = (int)(id % (uint32_t)hh);
   id /= (uint32_t)hh;
   const int z = (int)(id % (uint32_t)a.splits);
+  const int tile = a.tiles - 1 - (int)(id / (uint32_t)a.splits);
   QueryTile t;
-  if (!find_tile(a, a.tiles - 1 - (int)(id / (uint32_t)a.splits), &t)) return;
+  if (!find_tile(a, tile, &t)) return;
   const int tid = (int)threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int c = lane % 32, h = lane / 32;
@@ -285,8 +287,8 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
     return s.there == ~0ull && base >= last_lo && base + kManyStep <= first_hi;
   };
   // From registers: FP8 codes become elements, values of tokens that are not
-  // there, NaN and infinities of tokens that some rows do not see, and what is
-  // past a key's end become 0.
+  // there, NaN and infinities of steps that are not plain, and what is past a
+  // key's end become 0.
   auto put = [&](char *line, int swap, const Raw<16> &x) {
     if constexpr (kFp8) {
 #pragma unroll
@@ -303,9 +305,6 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
   auto store = [&](const Step &s, Staged &staged, int base, int buffer) {
     char *kb = lds + buffer * BUFFER, *vb = kb + TENSOR;
     if (!plain(s, base)) {
-      // the steps that add_infinities looks at again: missing tokens alone are no
-      // reason to take anything out of the others
-      const bool partly = base < last_lo || base + kManyStep > first_hi;
       uint32_t odd = 0;
 #pragma unroll
       for (int l = 0; l < NVL; ++l) {
@@ -324,8 +323,8 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
                    ((have >> (4 * w)) & 4 ? 0xFF0000u : 0u) |
                    ((have >> (4 * w)) & 8 ? 0xFF000000u : 0u);
           const uint32_t x = staged.v[l].w[w] & keep;
-          odd |= partly ? not_finite<C>(x) : 0u;
-          staged.v[l].w[w] = partly ? only_finite<C>(x) : x;
+          odd |= not_finite<C>(x);
+          staged.v[l].w[w] = only_finite<C>(x);
         }
       }
       if (odd != 0) *infinities = 1;
@@ -627,7 +626,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, uint32_t 
   }
   __syncthreads();
   if (*infinities != 0)
-    add_infinities<IO, C>(a, t, kvh, head0, nheads, z, from, to, lo, last_lo, first_hi, kManyStep);
+    add_infinities<IO, C, kManyStep, true>(args_address(args_at), tile, z, y);
 }
 
 // A batch's sequences of few new tokens, beside the ones of many: their
@@ -649,9 +648,11 @@ __global__ void __launch_bounds__(kManyThreads, DP == 256 ? 1 : DP == 128 ? 2 : 
   static_assert(sizeof(FewShared<DP>) <= many_lds<DP, INDEXED>() && kFewThreads == kManyThreads);
   if (blockIdx.x < x.few_grid)
     attention_few<IO, C, DP, VT, INDEXED, GROUPED, false>(
-        x.few, blockIdx.x, *reinterpret_cast<FewShared<DP> *>(lds));
+        x.few, offsetof(MixedArgs, few), blockIdx.x,
+        *reinterpret_cast<FewShared<DP> *>(lds));
   else
-    attention_many<IO, C, DP, VT, INDEXED, GROUPED>(x.many, blockIdx.x - x.few_grid, lds);
+    attention_many<IO, C, DP, VT, INDEXED, GROUPED>(x.many, offsetof(MixedArgs, many),
+                                                     blockIdx.x - x.few_grid, lds);
 }
 
 // few: null where no sequence can have few new tokens; p.grid: 0 where none can
