@@ -49,10 +49,20 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
 }
 
 // Block-indexed scales of values multiply the weights, which the products take in
-// the queries' type.  BF16 and F32 have the range for that; F16 weights carry
-// them relative to a reference, from this one on (values of so small a scale are
-// 0 in an F16 output: 2^-64 * 57344).
+// the queries' type.  BF16 and F32 have the range for that.  F16 has not: a row's
+// weights are taken relative to a reference near the largest product of weight
+// and scale so far (not of the scale alone: a page of a large one may have next
+// to no weight), and its sums count in units of it.
+//
+// kLeastScale: the smallest reference; a sum of so small a scale is 0 in an F16
+// output (2^-64 * 57344).
 constexpr float kLeastScale = 0x1p-64f;
+
+// The reference of a row, `was` until now, for a step whose largest weight is
+// `most`: weights may grow to 2^14 before a new one is taken, 2^-7 of the largest.
+__device__ __forceinline__ float reference_of(float was, float most) {
+  return most > was * 0x1p14f || was < kLeastScale ? fmaxf(most * 0x1p-7f, kLeastScale) : was;
+}
 
 // Two f32 to two 16-bit elements, to nearest even.
 template <int IO>

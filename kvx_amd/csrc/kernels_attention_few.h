@@ -180,7 +180,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
       scale_rest = product < 0.0f ? -scale_rest : scale_rest;
     }
   }
-  float m = -INFINITY, l = 0.0f, vref = kLeastScale;
+  float m = -INFINITY, l = 0.0f, unit = kLeastScale;
   f32x4 acc[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -425,8 +425,12 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
       if (__any(top > m)) {
         const float alpha = __builtin_amdgcn_exp2f(m - shift);
         l *= alpha;
+        if constexpr (kRelative) {
+          unit *= alpha;
+        } else {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) acc[j] *= alpha;
+          for (int j = 0; j < NV; ++j) acc[j] *= alpha;
+        }
       }
       m = top;
 #pragma unroll
@@ -439,33 +443,29 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
       if constexpr (INDEXED) {
         // Values stay codes; weights carry the tokens' scales.  A page in front of
         // the window may have slid out of it and its scale be anything: one that
-        // the row does not see counts as 0, by selection.  F16 weights carry them
-        // relative to the largest that the row saw, so that they stay in the
-        // type's range.
-        float by[4 * HALVES];
+        // the row does not see counts as 0, by selection.
 #pragma unroll
         for (int e = 0; e < 4 * HALVES; ++e) {
-          by[e] = token_scale(now, now.rows.vs, e);
-          by[e] = (hidden >> e) & 1 ? 0.0f : by[e];
+          const float by = token_scale(now, now.rows.vs, e);
+          p[e] *= (hidden >> e) & 1 ? 0.0f : by;
         }
         if constexpr (kRelative) {
-          float most = vref;
+          float most = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4 * HALVES; ++e) most = fmaxf(most, fabsf(by[e]));
+          for (int e = 0; e < 4 * HALVES; ++e) most = fmaxf(most, fabsf(p[e]));
           most = fmaxf(most, __shfl_xor(most, 16));
           most = fmaxf(most, __shfl_xor(most, 32));
-          if (__any(most > vref)) {
-            const float ratio = vref / most;
+          const float fresh = reference_of(unit, most);
+          if (__any(fresh != unit)) {
+            const float ratio = unit / fresh;
 #pragma unroll
             for (int j = 0; j < NV; ++j) acc[j] *= ratio;
-            vref = most;
+            unit = fresh;
           }
-          const float inv = 1.0f / vref;
+          const float inv = __builtin_amdgcn_rcpf(unit);
 #pragma unroll
-          for (int e = 0; e < 4 * HALVES; ++e) by[e] *= inv;
+          for (int e = 0; e < 4 * HALVES; ++e) p[e] *= inv;
         }
-#pragma unroll
-        for (int e = 0; e < 4 * HALVES; ++e) p[e] *= by[e];
       }
       if (now.there != kAll) clear_values(now.there);
       if (t.count > 1 && (base < last_lo || base + kFewStep > first_hi)) {
@@ -539,7 +539,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
   l += __shfl_xor(l, 32);
   if constexpr (kRelative) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) acc[j] *= vref;
+    for (int j = 0; j < NV; ++j) acc[j] *= unit;
   }
 
   // Join the waves: every wave brings its sums to the common maximum, then two

@@ -360,7 +360,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
     }
   };
 
-  float m = -INFINITY, l = 0.0f, vref = kLeastScale;
+  float m = -INFINITY, l = 0.0f, unit = kLeastScale;
   f32x16 acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x16{};
@@ -438,37 +438,14 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
       const float alpha = __builtin_amdgcn_exp2f(m - (now_m == -INFINITY ? 0.0f : now_m));
       m = now_m;
       l *= alpha;
+      if constexpr (kRelative) {
+        unit *= alpha;
+      } else {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[j] *= alpha;
+        for (int j = 0; j < NJ; ++j) acc[j] *= alpha;
+      }
     }
     const float shift = m == -INFINITY ? 0.0f : m;
-    // Scales of values by block: see the few-row kernel.
-    auto value_scale = [&](int b, int i) -> f32x4 {
-      f32x4 x = token_scales(now, now.rows.vs, buffer, 1, b, i);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = (hidden >> (16 * b + 4 * i + k)) & 1 ? 0.0f : x[k];
-      return x;
-    };
-    float inv = 1.0f;
-    if constexpr (kRelative) {
-      float most = vref;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = value_scale(b, i);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[k]));
-        }
-      most = fmaxf(most, __shfl_xor(most, 32));
-      if (__any(most > vref)) {
-        const float ratio = vref / most;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] *= ratio;
-        vref = most;
-      }
-      inv = 1.0f / vref;
-    }
     Frag w[4];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
@@ -483,15 +460,37 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
       if constexpr (INDEXED) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = value_scale(b, i);
+          // by selection: see the few-row kernel
+          const f32x4 x = token_scales(now, now.rows.vs, buffer, 1, b, i);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[b][4 * i + k] *= kRelative ? x[k] * inv : x[k];
+          for (int k = 0; k < 4; ++k)
+            s[b][4 * i + k] *= (hidden >> (16 * b + 4 * i + k)) & 1 ? 0.0f : x[k];
         }
       }
+    }
+    if constexpr (kRelative) {
+      float most = 0.0f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(s[b][i]));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const float fresh = reference_of(unit, most);
+      if (__any(fresh != unit)) {
+        const float ratio = unit / fresh;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] *= ratio;
+        unit = fresh;
+      }
+      const float inv = __builtin_amdgcn_rcpf(unit);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] *= inv;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         w[2 * b + i / 4].w[i % 4] = pair_of<IO>(s[b][2 * i], s[b][2 * i + 1]);
-    }
     // Values of 16 tokens (in the weights' order) of element 32 j + c.
     const int li = lane % 16;
     const lds_char *values_at = cur + TENSOR;
@@ -582,7 +581,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
   l += __shfl_xor(l, 32);
   if constexpr (kRelative) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[j] *= vref;
+    for (int j = 0; j < NJ; ++j) acc[j] *= unit;
   }
   const bool none = m == -INFINITY && l == 0.0f;
   const int64_t line = t.begin + t.first + tok;

@@ -8,7 +8,7 @@ import torch
 
 from kvx_amd.abi import Status
 
-from operator_helpers import AttentionCase, set_rows
+from operator_helpers import AttentionCase, scale_rows, set_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,33 @@ def test_infinities_beside_missing_blocks(io, cache, layout, table, new, window)
     half = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}[io]
     over = (got - want).abs()[fine] - (tol + half * (want.abs() + tol) + 2.0 ** -25)[fine]
     assert (over <= 0).all()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("cache", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("new", [None, [30, 1, 60]])
+@pytest.mark.parametrize("table", ["packed", "ragged"])
+def test_pages_of_very_different_scales(io, cache, new, table):
+    """A page whose values have a scale 10^8 times the others', but whose tokens
+    have weights near e^-28: its part is small, and the others keep their
+    digits."""
+    c = AttentionCase(io=io, cache=cache, scales="block", H=2, G=2, D=64, lens=[96, 40, 150],
+                      new=new, table=table)
+    ks = torch.ones(c.nb)
+    vs = torch.full((c.nb,), 0.01)
+    k = 0.5 * torch.randn(c.rows[0].shape, generator=torch.Generator().manual_seed(3))
+    k[..., 0] = 0
+    for s, j in ((0, 1), (1, 0), (2, 4)):
+        b = int(c.tb[s, j])
+        vs[b] = 1e6
+        k[b, ..., 0] = -28.0
+    c.q[..., 0] = 8.0
+    c.q_dev.copy_(c.q)
+    c.rows[0] = k.to(c.rows[0].dtype)
+    set_rows(c.cache.key_cache, c.cache.k_layout, c.rows[0])
+    for w, x in enumerate((ks, vs)):
+        c.kv_scales[w].values.copy_(x)
+        c.exact[w] = c.rows[w].double() * scale_rows(x, "block", c.nb, c.H)[:, None, :, None]
+    assert c.run() == Status.OK
+    torch.cuda.synchronize()
+    c.check()
