@@ -48,6 +48,16 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+// Weights are 2^(x - m), m the maximum of the logits x less this.  An F16 weight
+// has 11 digits down to 2^-14 and none below 2^-25: with a maximum of 1 a long
+// context would lose the many tokens of small weights (32768 tokens of e^-17.75
+// beside one of 1: all of them).  `room`: how far the maximum may grow, in powers
+// of two, before m follows it; the largest weight is 2^14 or 2^15.
+template <int IO>
+__device__ __forceinline__ constexpr float less_of_maximum(int room) {
+  return IO == KVX_DTYPE_F16 ? (room > 0 ? 15.0f - (float)room : 14.0f) : 0.0f;
+}
+
 // Block-indexed scales of values multiply the weights, which the products take in
 // the queries' type.  BF16 and F32 have the range for that.  F16 has not: a row's
 // weights are taken relative to a reference near the largest product of weight

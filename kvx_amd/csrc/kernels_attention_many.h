@@ -22,7 +22,8 @@
 //                 they are and read plainly).
 //   The sums of a row are a lane's own, so rescaling them is one multiplication
 //   each; it is put off until a maximum has grown by more than 8 (weights then
-//   reach 2^8, which changes neither their relative rounding nor the F32 sums).
+//   are 2^8 times as large, which changes neither their relative rounding nor the
+//   F32 sums).
 //
 // Measured: a chunk of 8192 tokens, 8 kv heads of 128, groups of 4, BF16: 583 us
 // (940 TFLOP/s); chunks of 2048 tokens at 4096 to 8192: 323 us (805 TFLOP/s).
@@ -44,6 +45,7 @@ constexpr int kManyWaves = 4;
 constexpr int kManyThreads = kManyWaves * kWave;
 static_assert(kManyRowTile == 32 * kManyWaves, "32 rows a wave");
 constexpr int kManyStep = 64;
+constexpr int kRoom = 8;  // see less_of_maximum
 
 // Operands are read from LDS this many products before they are used (about 128
 // cycles of 32 each); scheduling barriers, which vector and scalar operations
@@ -432,8 +434,8 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);  // NaN does not move it
     }
-    top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-    if (__any(top > m + 8.0f)) {
+    top = fmaf(fmaxf(top, __shfl_xor(top, 32)), scale, -less_of_maximum<IO>(kRoom));
+    if (__any(top > m + (float)kRoom)) {
       const float now_m = fmaxf(top, m);
       const float alpha = __builtin_amdgcn_exp2f(m - (now_m == -INFINITY ? 0.0f : now_m));
       m = now_m;
