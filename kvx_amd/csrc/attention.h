@@ -35,6 +35,7 @@ namespace dev {
 
 constexpr int kRowTile = 16;       // rows of a tile of the kernels for few rows
 constexpr int kManyRowTile = 128;  // and of the one for many
+constexpr float near_cap(int io) { return io == KVX_DTYPE_BF16 ? 512.0f : 64.0f; }  // see cap_logits
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
@@ -63,8 +64,9 @@ struct AttentionArgs {
   int32_t qptr64;
   int32_t seqs, tokens, heads, group, head_dim;
   int32_t causal, window;
+  float scale, softcap;  // as given; softcap 0: none
   float scale_log2;  // scale * log2 e
-  float cap, cap_in; // softcap * log2 e and scale / softcap; cap 0: none
+  float cap, cap_in; // softcap / 4 * log2 e (finite for any softcap), scale / softcap
   float scale_rest, cap_rest;  // what rounding left of scale_log2 and cap
   // tiles
   int32_t tile_heads, head_tiles, tile_tokens, tiles;
@@ -289,9 +291,16 @@ __device__ __forceinline__ float scale_of(const ScaleRef &s, int32_t block, int3
   return s.p[s.indexed ? block * s.s_block + head * s.s_head : 0];
 }
 
+// Four times tanh of a raw product's logit over the softcap, to be multiplied by
+// a.cap: good to a few units of F32 for every softcap.  A quotient, as scale /
+// softcap may be subnormal or infinite.
+__device__ __forceinline__ float capped_part(const AttentionArgs &a, float dot) {
+  return 4.0f * tanhf(dot * a.scale / a.softcap);
+}
+
 // x = scale * q.k (in log2 units) of a raw product.
 __device__ __forceinline__ float logit(const AttentionArgs &a, float dot) {
-  if (a.cap != 0.0f) return a.cap * tanhf(dot * a.cap_in);
+  if (a.softcap != 0.0f) return a.cap * capped_part(a, dot);
   return dot * a.scale_log2;
 }
 

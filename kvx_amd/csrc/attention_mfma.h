@@ -203,11 +203,43 @@ __device__ __forceinline__ uint64_t args_address(size_t offset) {
   return reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr()) + offset;
 }
 
-// scale * q.k in units of log2, the scale of an FP8 key included in the
-// arguments; tanh(y) = 1 - 2 / (1 + e^2y).
-__device__ __forceinline__ float capped(const AttentionArgs &a, float x) {
-  const float e = __builtin_amdgcn_exp2f(x * a.cap_in * (2.0f * kLog2e));
-  return a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + e);
+// The capped logits in units of log2 of raw products x (by: the scale of an FP8
+// key), for 16-bit products.  With y = scale x / softcap:
+//
+// - softcap to near_cap: softcap * (1 - 2 / (1 + e^2y)), off by up to 2^-21 of the
+//   softcap and so a sixteenth of a weight's rounding, 2^-15 of F16, 2^-12 of BF16;
+// - larger ones, for which that grows: right to about 2^-20 of the logit, by
+//   scale x * tanh(y) / y for |y| < 1/2, a polynomial in y^2 (least maximum error
+//   on [0, 1/4], 1.5e-8), so that a cap far away leaves logits as they are.
+//
+// FAR: the second form too.  Only the streaming kernel for few rows has it, and
+// takes chunks of any length with such a cap: in the kernel for many rows it costs
+// chunks with near caps 27 to 43 % where it is the only form, and registers that
+// other calls miss beside the first (a mixed batch without a cap: 62 us for 54).
+// Two chunks of 2048 tokens at 4096 to 8192, BF16 heads of 128: 400 us with a cap
+// of 30, 1763 with one of 10^5.
+template <int IO, bool FAR, typename V, int N>
+__device__ __forceinline__ void cap_logits(const AttentionArgs &a, float by, V &x) {
+  if (!FAR || a.softcap <= near_cap(IO)) {
+    const float cap = 4.0f * a.cap;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = __builtin_amdgcn_exp2f(x[i] * by * a.cap_in * (2.0f * kLog2e));
+      x[i] = fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + e), cap);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = x[i] * by * a.cap_in, u = y * y;
+    const float e = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e));
+    const float far = a.cap * fmaf(__builtin_amdgcn_rcpf(1.0f + e), -8.0f, 4.0f);
+    float r = fmaf(u, 0.01724149f, -0.05304549f);
+    r = fmaf(u, r, 0.13325879f);
+    r = fmaf(u, r, -0.33333144f);
+    r = fmaf(u, r, 1.0f);
+    x[i] = fabsf(y) < 0.5f ? x[i] * by * a.scale_log2 * r : far;
+  }
 }
 
 // The factor from products to logits in units of log2 (1 where a softcap has
@@ -216,7 +248,7 @@ __device__ __forceinline__ float capped(const AttentionArgs &a, float x) {
 // the queries 0.
 template <int IO, int N>
 __device__ __forceinline__ float positive_scale(const AttentionArgs &a, float ks, Frag (&q)[N]) {
-  if (a.cap != 0.0f) return 1.0f;
+  if (a.softcap != 0.0f) return 1.0f;
   const float scale = a.scale_log2 * ks;
   const uint32_t keep = scale == 0.0f ? 0u : ~0u, flip = scale >= 0.0f             ? 0u
                                                             : IO == KVX_DTYPE_F32 ? 0x80000000u

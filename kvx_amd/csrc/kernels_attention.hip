@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.h"
 #include "kvx_internal.h"
@@ -290,10 +291,14 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
   a.causal = p.causal;
   a.window = p.window;
   a.scale_log2 = p.scale * kLog2e;
-  a.cap = p.softcap * kLog2e;
+  a.scale = p.scale;
+  a.softcap = p.softcap;
+  // a quarter, so that no softcap is infinite; positive for every one
+  a.cap = p.softcap > 0.0f ? std::max(p.softcap * (0.25f * kLog2e), FLT_MIN) : 0.0f;
   a.scale_rest = (float)((double)p.scale * kLog2eWide - (double)a.scale_log2);
-  a.cap_rest = (float)((double)p.softcap * kLog2eWide - (double)a.cap);
-  a.cap_in = p.softcap > 0.0f ? p.scale / p.softcap : 0.0f;
+  a.cap_rest = a.cap > FLT_MIN ? (float)((double)p.softcap * (0.25 * kLog2eWide) - (double)a.cap) : 0.0f;
+  // infinite for the smallest softcaps: 0 * infinity would be NaN
+  a.cap_in = p.softcap > 0.0f ? std::clamp(p.scale / p.softcap, -FLT_MAX, FLT_MAX) : 0.0f;
   a.least_rows = 0;
   a.most_rows = 0x7FFFFFFF;
   Plan r{};
@@ -320,8 +325,8 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
               steps_fit(g.gv);
   const bool few_ok = most != kRows && cores && values_fit(p, kFew, &r.vt);
   bool vt_many = false;
-  r.many = most == kMany && few_ok && g.io_dtype != KVX_DTYPE_F32 && values_fit(p, kMany, &vt_many) &&
-           vt_many == r.vt;
+  r.many = most == kMany && few_ok && g.io_dtype != KVX_DTYPE_F32 && p.softcap <= near_cap(g.io_dtype) &&
+           values_fit(p, kMany, &vt_many) && vt_many == r.vt;
   if (!few_ok) {
     AttentionArgs &x = add(kRows, a);
     tile_rows(&x, kRowTile);

@@ -66,10 +66,11 @@ struct FewShared {
   int infinities;  // see add_infinities
 };
 
-// Workgroup `id` of its grid, whose arguments start at args_at.  IO: type of queries and of the products; C: the
-// cache's type; DP: head_dim rounded up to 64, 128 or 256; VT: values with the
-// token axis innermost; INDEXED: scales by block; GROUPED: blocks hold whole
-// groups of 16 tokens; STREAM: keys and values are read past the caches.
+// Workgroup `id` of its grid, whose arguments start at args_at.  IO: type of
+// queries and of the products; C: the cache's type; DP: head_dim rounded up to 64,
+// 128 or 256; VT: values with the token axis innermost; INDEXED: scales by block;
+// GROUPED: blocks hold whole groups of 16 tokens; STREAM: keys and values are read
+// past the caches (and 16-bit queries may have a softcap past near_cap).
 template <int IO, int C, int DP, bool VT, bool INDEXED, bool GROUPED, bool STREAM>
 __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t args_at, uint32_t id,
                                               FewShared<DP> &shared) {
@@ -172,11 +173,11 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
   // F32: the factor's rest too, or all logits would be off by its rounding.
   float scale = positive_scale<IO>(a, ks, q), scale_rest = 0.0f;
   if constexpr (kF32) {
-    const float hi = a.cap != 0.0f ? a.cap : a.scale_log2, by = a.cap != 0.0f ? 1.0f : ks;
+    const float hi = a.softcap != 0.0f ? a.cap : a.scale_log2, by = a.softcap != 0.0f ? 1.0f : ks;
     const float product = hi * by;
     if (product != 0.0f) {
       scale = fabsf(product);
-      scale_rest = fmaf(hi, by, -product) + (a.cap != 0.0f ? a.cap_rest : a.scale_rest) * by;
+      scale_rest = fmaf(hi, by, -product) + (a.softcap != 0.0f ? a.cap_rest : a.scale_rest) * by;
       scale_rest = product < 0.0f ? -scale_rest : scale_rest;
     }
   }
@@ -399,10 +400,13 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
         x[e] = s[e / 4][e % 4];
         if constexpr (INDEXED) x[e] *= token_scale(now, now.rows.ks, e);
       }
-      if (a.cap != 0.0f) {
+      if (a.softcap != 0.0f) {
+        if constexpr (kF32) {
 #pragma unroll
-        for (int e = 0; e < 4 * HALVES; ++e)
-          x[e] = kF32 ? tanhf(x[e] * ks * a.cap_in) : capped(a, x[e] * ks);
+          for (int e = 0; e < 4 * HALVES; ++e) x[e] = capped_part(a, x[e] * ks);
+        } else {
+          cap_logits<IO, STREAM, decltype(x), 4 * HALVES>(a, ks, x);
+        }
       }
       uint32_t hidden = 0;  // bit e: this lane's row does not see its token e
       if (!whole) {

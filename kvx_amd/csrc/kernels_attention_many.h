@@ -416,10 +416,7 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
           for (int w = 0; w < 4; ++w) s[b][4 * i + w] *= x[w];
         }
       }
-      if (a.cap != 0.0f) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = capped(a, s[b][i] * ks);
-      }
+      if (a.softcap != 0.0f) cap_logits<IO, false, f32x16, 16>(a, ks, s[b]);
       if (!whole) {
         const uint32_t there = (uint32_t)(now.there >> (32 * b)) >> (4 * h);
         const int start = base + 32 * b + 4 * h;

@@ -86,13 +86,14 @@ def scale_rows(values, kind, nb, H):
 
 
 def attention_reference(q, rows_of, lens, new, G, *, causal=True, scale, window=0, softcap=0.0,
-                        u_p=0.0):
+                        u_p=0.0, cap_rel=None):
     """out, lse in float64 and how far 32-bit kernels may be from them.
 
     rows_of(s) -> (k, v [n, H, D] float64, there [n] bool): the sequence's
     tokens that the table holds.  With c = (D + 8) 2^-24 times the sum of the
     absolute products, a logit is off by at most d = c (+ cap 2^-21 for the
-    softcap's tanh), every weight by a relative 2 d + u_p (u_p: its rounding
+    softcap's tanh; with `cap_rel` that part of the capped logit, and cap 2^-149
+    where tanh's argument is subnormal), every weight by a relative 2 d + u_p (u_p: its rounding
     for the matrix cores), and sums over n weights by n 2^-24."""
     T, Hq, D = q.shape
     out = torch.zeros((T, Hq, D), dtype=torch.float64)
@@ -119,7 +120,10 @@ def attention_reference(q, rows_of, lens, new, G, *, causal=True, scale, window=
                 d = (D + 8) * U32 * size.amax(-1)
                 if softcap:
                     x = softcap * torch.tanh(x / softcap)
-                    d = d + softcap * 2.0 ** -21
+                    if cap_rel is None:
+                        d = d + softcap * 2.0 ** -21
+                    else:
+                        d = d + cap_rel * x.abs().amax(-1) + softcap * 2.0 ** -149
                 l = torch.logsumexp(x, -1)
                 p = torch.exp(x - l[..., None])
                 o = torch.einsum("hgn,nhd->hgd", p, vv)
@@ -137,6 +141,8 @@ def attention_reference(q, rows_of, lens, new, G, *, causal=True, scale, window=
 class AttentionCase:
     """A batch for paged.attention: cache, table, queries, and its result in
     64 bits."""
+
+    cap_rel = None  # see attention_reference
 
     def __init__(self, *, io="bf16", cache=None, layout="nhd", table="packed", bs=16, H=2, G=4,
                  D=64, lens=(37,), new=None, index=torch.int32, scales="tensor", seed=0,
@@ -241,7 +247,7 @@ class AttentionCase:
     def reference(self):
         u_p = 0.0 if self.io == "f32" else HALF[self.io]
         return attention_reference(self.q[: self.total], self.rows_of, self.lens, self.new, self.G,
-                                   scale=self.scale, u_p=u_p, **self.args)
+                                   scale=self.scale, u_p=u_p, cap_rel=self.cap_rel, **self.args)
 
     def run(self, **more):
         kw = dict(scale=self.scale, lse=self.lse, max_seq_len=max(self.lens + [0]),

@@ -1,6 +1,17 @@
-"""Long contexts whose weights are small beside one, against the definition in
-64 bits: an F16 weight below 2^-14 of the largest would lose digits, and one below
-2^-25 all of them."""
+"""Softcaps of any size, and long contexts whose weights are small beside one:
+against the definition in 64 bits.
+
+Softcap.  With x the logit and c the cap, c tanh(x / c) is computed relative to
+itself: in F32 and on the vector unit from tanhf (a few units of 2^-24); in 16 bits
+with caps past 64 (F16) or 512 (BF16) by a polynomial for |x| < c / 2 (2^-26 and about eight
+roundings), else as c (1 - 2 / (1 + e)) with e = exp(2 x / c): exp2 and the
+reciprocal are good to 2^-23, the argument's rounding is worth |y| (1 - tanh^2 y)
+2^-23 < 0.45 * 2^-23, in all less than 2^-22 of 1 and so 2^-21 of tanh(1/2).  Twice
+that, 2^-20, is allowed.  Smaller caps in 16 bits take the latter form for all x
+and are allowed 2^-21 of the cap, as in the other tests.
+
+Weights.  An F16 weight below 2^-14 of the largest would lose digits, and one
+below 2^-25 all of them; a long context has many."""
 import math
 
 import pytest
@@ -9,9 +20,49 @@ import torch
 from kvx_amd import paged
 from kvx_amd.abi import Layout, Status
 
-from operator_helpers import DT, scale_arg
+from operator_helpers import AttentionCase, DT, scale_arg
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("softcap", [1e-3, 2.0, 50.0, 64.0, 65.0, 512.0, 513.0, 1e3, 1e5, 1e6, 1e20, 3e38])
+@pytest.mark.parametrize("io,cache,D", [("bf16", None, 64), ("f16", None, 64), ("f32", None, 64),
+                                        ("f16", "e4m3", 128), ("f32", "e5m2", 64),
+                                        ("bf16", None, 20), ("f32", None, 20)])
+@pytest.mark.parametrize("new", [None, [80, 3]])
+@pytest.mark.parametrize("scale", [0.2, -3.0])
+def test_softcaps(softcap, io, cache, D, new, scale):
+    c = AttentionCase(io=io, cache=cache, lens=[100, 64], new=new, D=D, softcap=softcap, scale=scale)
+    if softcap > (512 if io == "bf16" else 64) or io == "f32" or D == 20:
+        c.cap_rel = 2.0 ** -20
+    assert c.run() == Status.OK
+    c.check()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 20])
+def test_smallest_softcap(io, D):
+    """A cap that is subnormal: all logits are as good as 0."""
+    c = AttentionCase(io=io, lens=[40, 90], new=[1, 60], D=D, softcap=1e-44)
+    assert c.run() == Status.OK
+    c.check()
+
+
+def test_far_softcaps_of_chunks():
+    """Far caps take the kernel for few rows, also for many tiles a sequence."""
+    for kw in (dict(io="bf16", lens=[700, 40, 300], new=[500, 1, 129]),
+               dict(io="f16", cache="e4m3", lens=[2500], new=[40], window=300),
+               dict(io="f16", layout="vllm", lens=[90, 400], new=[90, 200])):
+        c = AttentionCase(D=64, softcap=1e4, H=2, G=4, **kw)
+        c.cap_rel = 2.0 ** -20
+        assert c.run() == Status.OK
+        c.check()
+        size = paged.attention_workspace_size(c.cache, c.q_dev, c.table, c.lens_t, c.indptr,
+                                              max_seq_len=max(c.lens), max_query_len=max(c.new),
+                                              k_scale=c.kv_scales[0], v_scale=c.kv_scales[1])
+        w = torch.empty(size, dtype=torch.uint8, device="cuda")
+        assert c.run(workspace=w) == Status.OK
+        c.check()
 
 
 @pytest.mark.parametrize("io,cache,scales", [("f16", None, "tensor"), ("f16", "e4m3", "tensor"),
