@@ -6,7 +6,7 @@
 #include <cfloat>
 
 #include "attention.h"
-#include "kvx_internal.h"
+#include "operators_internal.h"
 
 namespace kvx {
 namespace dev {

@@ -14,7 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"
-#include "kvx_internal.h"
+#include "operators_internal.h"
 
 namespace kvx {
 namespace dev {

@@ -103,57 +103,6 @@ struct GatherPlan {
   int32_t cache_dtype;
 };
 
-// Everything the rotary write needs, already validated on the host.  `w`
-// describes keys, values and their cache rows; strides are in elements.
-struct RopePlan {
-  WritePlan w;
-  const void *query;
-  void *query_out;
-  const void *positions;
-  const float *inv_freq;
-  int64_t k_tok, k_head, v_tok, v_head;
-  int64_t q_tok, q_head, o_tok, o_head;
-  float magnitude;
-  int32_t position_is64;
-  int32_t query_heads;  // 0: no queries
-  int32_t rot_dim;
-  int32_t interleaved;
-};
-
-// Everything the attention needs, already validated on the host.  The cache
-// and its table are described as a gather's (`g`: its dst, max_seq_len, conv
-// and scales are not used); strides are in elements.
-struct AttentionPlan {
-  GatherPlan g;
-  const void *query;
-  void *out;
-  float *lse;
-  const void *query_indptr;
-  void *workspace;
-  int64_t q_tok, q_head, o_tok, o_head;
-  float scale;
-  float softcap;
-  int32_t indptr_is64;
-  int32_t tokens;
-  int32_t query_heads;
-  int32_t causal;
-  int32_t window;         // 0: none
-  int32_t max_seq_len;    // hints, 0: not known
-  int32_t max_query_len;
-  int32_t scaled;         // FP8 cache
-};
-
-// One K or V tensor of a block copy.
-struct CopyTensor {
-  char *data;
-  int64_t num_blocks;
-  Geom g;
-  int32_t block_size;
-  int32_t heads;
-  int32_t head_dim;
-  int32_t esize;
-};
-
 // Element size in bytes of a payload dtype, 0 for non-payload dtypes.
 int dtype_size(kvx_dtype_t dt);
 
@@ -161,26 +110,6 @@ int dtype_size(kvx_dtype_t dt);
 // KVX_STATUS_INTERNAL_ERROR when the launch itself fails.
 kvx_status_t enqueue_write(const WritePlan &plan, void *stream);
 kvx_status_t enqueue_gather(const GatherPlan &plan, void *stream);
-kvx_status_t enqueue_rope_write(const RopePlan &plan, void *stream);
-kvx_status_t enqueue_attention(const AttentionPlan &plan, void *stream);
-kvx_status_t enqueue_copy_blocks(const CopyTensor *tensors, int64_t count, const void *pairs,
-                                 bool index_is64, int64_t pair_count, void *stream);
-
-// Bytes of workspace that enqueue_attention uses for the plan (its pointers
-// are not read).
-uint64_t attention_workspace(const AttentionPlan &plan);
-uint64_t attention_workspace_bound(const AttentionPlan &p);  // for any alignment
-
-// Checks and conversions that the entry points share (launch.cpp).
-bool is_io_float(kvx_dtype_t dt);
-bool is_fp8(kvx_dtype_t dt);
-kvx_status_t fill_geom(const kvx_cache_desc_t *cache, const kvx_tensor_desc_t *t, Geom *g);
-bool block_fits(const Geom &g, int64_t bs, int64_t heads, int64_t head_dim, int esize,
-                int64_t pitch);
-kvx_status_t resolve_scale_desc(const kvx_scale_desc_t *d, const kvx_cache_desc_t *cache,
-                                bool block_ok, ScaleRef *out);
-kvx_status_t resolve_write_scale(const kvx_scale_desc_t *desc, const void *raw,
-                                 const kvx_cache_desc_t *cache, ScaleRef *out);
 
 // Shared launch-path implementations behind the exported entry points.
 // `expected` is the dtype the per-dtype helper requires of cache and io

@@ -16,7 +16,7 @@
 #include <hip/hip_runtime.h>
 
 #include "kvx_ext.h"
-#include "kvx_internal.h"
+#include "operators_internal.h"
 #include "kvx_paged_kv.h"
 
 namespace kvx {

@@ -8,7 +8,7 @@
 #include <vector>
 
 #include "kvx_ext.h"
-#include "kvx_internal.h"
+#include "operators_internal.h"
 
 namespace kvx {
 namespace {
