@@ -78,7 +78,7 @@ struct AttentionArgs {
   int32_t part_rows;  // partial row of (s, i): s * part_rows + i; 0: the row number
   float *part_o;      // [partial row, query head, split, head_dim]
   float *part_ml;     // the same without head_dim: (maximum, sum of weights)
-  int32_t chunk_k, chunk_v;  // elements of a head that load together (rows kernel)
+  int32_t chunk_k;    // keys' elements load four at a time (rows kernel)
 };
 
 struct QueryTile {
@@ -219,8 +219,8 @@ __device__ __forceinline__ void row_range(const AttentionArgs &a, const QueryTil
     *lo = (int)min(pos - a.window + 1, (int64_t)t.usable);
 }
 
-// Tokens of split z of a tile that sees [lo, hi): split_tokens each, or more
-// where the sequence is longer than the host knew; from a multiple of 64 on.
+// Tokens of split z of a tile that sees [lo, hi): split_steps steps of 64 each, or
+// more where the sequence is longer than the host knew; from a multiple of 64 on.
 __device__ __forceinline__ void split_range(const AttentionArgs &a, int lo, int hi, int z,
                                             int *from, int *to) {
   const int start = lo & ~63;

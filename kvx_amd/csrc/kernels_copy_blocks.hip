@@ -31,7 +31,6 @@ struct CopyArgs {
     int64_t num_blocks;
   } t[kCopyTensors];
   const void *pairs;
-  int64_t pair_count;
   int64_t block_bytes;
   int32_t tensors;
   int32_t parts;  // workgroups per block
@@ -162,9 +161,9 @@ kvx_status_t enqueue_copy_blocks(const CopyTensor *tensors, int64_t count, const
     const int64_t per_pair = parts * a.tensors, batch = pairs_per_launch(per_pair);
     if (batch == 0) return false;
     for (int64_t at = 0; at < pair_count; at += batch) {
-      a.pair_count = pair_count - at < batch ? pair_count - at : batch;
+      const int64_t n = pair_count - at < batch ? pair_count - at : batch;
       a.pairs = static_cast<const char *>(pairs) + at * pair_bytes;
-      const int64_t grid = a.pair_count * per_pair;
+      const int64_t grid = n * per_pair;
       if (width == 16) launch_copy<16>(a, index_is64, grid, s);
       else if (width == 4) launch_copy<4>(a, index_is64, grid, s);
       else if (width == 2) launch_copy<2>(a, index_is64, grid, s);

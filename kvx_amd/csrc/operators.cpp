@@ -277,7 +277,6 @@ static kvx_status_t plan_attention(const kvx_cache_desc_t *cache, const kvx_atte
   p->window = (int32_t)a->window;
   p->max_seq_len = (int32_t)a->max_seq_len;
   p->max_query_len = (int32_t)(a->query_indptr == nullptr ? 1 : a->max_query_len);
-  p->scaled = is_fp8(cdt);
   return KVX_STATUS_OK;
 }
 

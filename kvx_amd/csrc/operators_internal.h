@@ -26,8 +26,8 @@ struct RopePlan {
 };
 
 // Everything the attention needs, already validated on the host.  The cache
-// and its table are described as a gather's (`g`: its dst, max_seq_len, conv
-// and scales are not used); strides are in elements.
+// and its table are described as a gather's (`g`: its dst, max_seq_len and conv
+// are not used); strides are in elements.
 struct AttentionPlan {
   GatherPlan g;
   const void *query;
@@ -45,7 +45,6 @@ struct AttentionPlan {
   int32_t window;         // 0: none
   int32_t max_seq_len;    // hints, 0: not known
   int32_t max_query_len;
-  int32_t scaled;         // FP8 cache
 };
 
 // One K or V tensor of a block copy.
@@ -65,10 +64,11 @@ kvx_status_t enqueue_attention(const AttentionPlan &plan, void *stream);
 kvx_status_t enqueue_copy_blocks(const CopyTensor *tensors, int64_t count, const void *pairs,
                                  bool index_is64, int64_t pair_count, void *stream);
 
-// Bytes of workspace that enqueue_attention uses for the plan (its pointers
-// are not read).
+// Bytes of workspace that enqueue_attention uses for the plan, whose pointers'
+// alignment takes part in the choice of the kernel, and the most that it uses
+// whatever that alignment is.  Neither reads through a pointer.
 uint64_t attention_workspace(const AttentionPlan &plan);
-uint64_t attention_workspace_bound(const AttentionPlan &p);  // for any alignment
+uint64_t attention_workspace_bound(const AttentionPlan &plan);
 
 // Checks and conversions that the entry points share (launch.cpp).
 bool is_io_float(kvx_dtype_t dt);
