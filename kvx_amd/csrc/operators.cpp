@@ -230,6 +230,8 @@ static kvx_status_t plan_attention(const kvx_cache_desc_t *cache, const kvx_atte
   }
   if (a->query_indptr != nullptr ? !is_index(a->query_indptr_dtype) : T != S)
     return KVX_STATUS_INVALID_ARGUMENT;
+  if (a->query_indptr != nullptr && T + S > kMost32)
+    return KVX_STATUS_UNSUPPORTED;  // tile numbers are 32-bit
   if (pointers &&
       (a->query.data == nullptr || a->out.data == nullptr || a->seq_lens.lengths == nullptr ||
        (fmt != KVX_BLOCK_TABLE_KV_OFFSETS &&
