@@ -165,3 +165,21 @@ def test_pages_of_very_different_scales(io, cache, new, table):
     assert c.run() == Status.OK
     torch.cuda.synchronize()
     c.check()
+
+
+@pytest.mark.parametrize("table,bs,layout", [("packed", 16, "nhd"), ("packed", 8, "vllm"),
+                                             ("ragged", 16, "nhd"), ("ragged", 8, "vllm")])
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("new", [None, [40, 3]])
+@pytest.mark.parametrize("window", [0, 2000])
+def test_block_scales_of_split_sequences(window, new, io, table, bs, layout):
+    """Contexts whose tokens are divided among workgroups; pages of nobody, and
+    those in front of the window, have scales that were never written."""
+    for kind in ("block", "block_head"):
+        c = AttentionCase(io=io, cache="e4m3", scales=kind, layout=layout, table=table, bs=bs, H=1,
+                          G=4, D=64, lens=[5000, 70], new=new, window=window)
+        for s in c.kv_scales:
+            for i, b in enumerate((~seen_blocks(c, window)).nonzero()[:, 0].tolist()):
+                s.values[b] = POISON[(i + b) % 4]
+        assert c.run() == Status.OK
+        c.check()
