@@ -376,8 +376,10 @@ Plan make_plan(const AttentionPlan &p, Kind most) {
     AttentionArgs &x = r.part[i].a;
     if (x.splits == 1) continue;
     const int64_t sums = join_rows(x) * p.query_heads * x.splits;
-    x.part_o = reinterpret_cast<float *>(static_cast<char *>(p.workspace) + r.workspace);
-    x.part_ml = x.part_o + sums * x.head_dim;
+    // as numbers: the workspace is null where only its size is asked for
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.workspace) + r.workspace;
+    x.part_o = reinterpret_cast<float *>(at);
+    x.part_ml = reinterpret_cast<float *>(at + (uint64_t)sums * x.head_dim * 4);
     r.workspace += ((uint64_t)sums * (x.head_dim + 2) * 4 + 15) & ~(uint64_t)15;
   }
   return r;

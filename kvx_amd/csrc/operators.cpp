@@ -19,6 +19,31 @@ bool on_device(const kvx_tensor_desc_t &t) {
   return t.memory == KVX_MEMORY_DEVICE || t.memory == KVX_MEMORY_UNIFIED;
 }
 
+// An axis of n elements spans less than 2^56 of them: no offset on the host or the
+// device overflows.
+bool spans(int64_t n, int64_t stride) {
+  const int64_t most = ((int64_t)1 << 56) / (n > 1 ? n : 1);
+  return stride >= -most && stride <= most;
+}
+
+// fill_geom, with strides of axes of one element as 0 (they are never used) and
+// the others' spans checked.
+kvx_status_t cache_geom(const kvx_cache_desc_t *c, const kvx_tensor_desc_t *t, Geom *g) {
+  const kvx_status_t st = fill_geom(c, t, g);
+  if (st != KVX_STATUS_OK) return st;
+  const int64_t pack = g->pack > 0 ? g->pack : 1;
+  struct {
+    int64_t n, *stride;
+  } const axes[5] = {{(int64_t)c->num_blocks, &g->s_block}, {(int64_t)c->block_size, &g->s_off},
+                     {(int64_t)c->num_kv_heads, &g->s_head},
+                     {(int64_t)c->head_dim / pack, &g->s_piece}, {pack, &g->s_inner}};
+  for (const auto &x : axes) {
+    if (x.n <= 1) *x.stride = 0;
+    else if (!spans(x.n, *x.stride)) return KVX_STATUS_INVALID_ARGUMENT;
+  }
+  return KVX_STATUS_OK;
+}
+
 bool is_index(kvx_dtype_t dt) { return dt == KVX_DTYPE_S32 || dt == KVX_DTYPE_S64; }
 
 // A [tokens, heads, head_dim] tensor of rows with adjacent head elements and
@@ -32,7 +57,7 @@ kvx_status_t check_rows(const kvx_tensor_desc_t &t, int64_t tokens, int64_t head
   if (t.stride[2] != 1 && head_dim > 1) return KVX_STATUS_UNSUPPORTED;
   *tok = tokens > 1 ? t.stride[0] : 0;
   *head = heads > 1 ? t.stride[1] : 0;
-  return KVX_STATUS_OK;
+  return spans(tokens, *tok) && spans(heads, *head) ? KVX_STATUS_OK : KVX_STATUS_INVALID_ARGUMENT;
 }
 
 // A written tensor: no two of its elements may share an address.
@@ -97,9 +122,9 @@ static kvx_status_t plan_rope(const kvx_cache_desc_t *cache, const kvx_write_des
     if (rows_overlap(T, Hq, D, p->o_tok, p->o_head)) return KVX_STATUS_UNSUPPORTED;
   }
   WritePlan &w = p->w;
-  st = fill_geom(cache, &cache->k, &w.gk);
+  st = cache_geom(cache, &cache->k, &w.gk);
   if (st != KVX_STATUS_OK) return st;
-  st = fill_geom(cache, &cache->v, &w.gv);
+  st = cache_geom(cache, &cache->v, &w.gv);
   if (st != KVX_STATUS_OK) return st;
   if (is_fp8(cdt)) {
     st = resolve_write_scale(&write->k_scale_desc, write->k_scale, cache, &w.k_scale);
@@ -180,9 +205,9 @@ static kvx_status_t plan_attention(const kvx_cache_desc_t *cache, const kvx_atte
     return KVX_STATUS_INVALID_ARGUMENT;
   if (D > 512) return KVX_STATUS_UNSUPPORTED;
   GatherPlan &g = p->g;
-  st = fill_geom(cache, &cache->k, &g.gk);
+  st = cache_geom(cache, &cache->k, &g.gk);
   if (st != KVX_STATUS_OK) return st;
-  st = fill_geom(cache, &cache->v, &g.gv);
+  st = cache_geom(cache, &cache->v, &g.gv);
   if (st != KVX_STATUS_OK) return st;
   if (is_fp8(cdt)) {
     // Without pointers a descriptor's data may be NULL: anything stands for it.
@@ -347,7 +372,7 @@ KVX_API kvx_status_t kvx_launch_copy_blocks(const kvx_cache_desc_t *const *cache
       if (st != KVX_STATUS_OK) return st;
       for (const kvx_tensor_desc_t *t : {&c->k, &c->v}) {
         kvx::CopyTensor x{};
-        st = kvx::fill_geom(c, t, &x.g);
+        st = kvx::cache_geom(c, t, &x.g);
         if (st != KVX_STATUS_OK) return st;
         if (c->block_size == 0) return KVX_STATUS_INVALID_ARGUMENT;
         if (c->num_blocks == 0 || c->num_kv_heads == 0 || c->head_dim == 0) continue;
