@@ -127,7 +127,7 @@ typedef struct kvx_rope_desc {
   const void *positions;   /* [num_tokens] */
   const float *inv_freq;   /* F32 [rot_dim / 2] */
   kvx_tensor_desc_t query; /* [num_tokens, query_heads, head_dim]; ndim 0: none */
-  kvx_tensor_desc_t query_out; /* same shape; may be the query itself */
+  kvx_tensor_desc_t query_out; /* same shape; the query itself or apart from it */
 } kvx_rope_desc_t;
 
 /* Rotates query rows into query_out and key rows into the paged cache, and
@@ -157,7 +157,8 @@ typedef enum kvx_attention_flags KVX_ENUM_BASE {
  * Query head h reads kv head h / (query heads / num_kv_heads).  Tokens that a
  * gather would skip (a block id out of range, no table entry, past the RAGGED
  * count) are not attended to.  A row that attends to nothing is 0 with lse
- * -infinity.  Rows behind the last sequence are left as they were.
+ * -infinity.  Rows behind the last sequence are left as they were.  Scales of
+ * blocks that a row attends to nothing of may be anything, as their tokens may.
  * Sums and softmax statistics are F32. */
 typedef struct kvx_attention_desc {
   uint32_t size;  /* sizeof(kvx_attention_desc_t) */
@@ -165,13 +166,14 @@ typedef struct kvx_attention_desc {
   kvx_tensor_desc_t query; /* [num_tokens, query_heads, head_dim], F16/BF16/F32, the
                               cache's dtype unless that is FP8; elements of a head
                               adjacent, any other strides */
-  kvx_tensor_desc_t out;   /* same shape and dtype; may be the query itself */
+  kvx_tensor_desc_t out;   /* same shape and dtype; the query itself or apart from it */
   float *lse;              /* F32 [num_tokens, query_heads], or NULL */
   const void *query_indptr; /* [seq_count + 1] row numbers, or NULL */
   kvx_dtype_t query_indptr_dtype; /* S32 or S64 */
   uint32_t window;         /* tokens seen, its own included; 0: all.  Causal only */
   float scale;
-  float softcap;           /* 0: none */
+  float softcap;           /* 0: none; any finite one.  Past 64 (F16; BF16: 512) chunks take
+                              longer */
   uint32_t max_seq_len;    /* largest sequence and most query rows of one, as far as */
   uint32_t max_query_len;  /* known (0: not): they steer the split, not the result */
   kvx_block_table_t block_table; /* PACKED, RAGGED or KV_OFFSETS, as a gather's */

@@ -28,14 +28,14 @@
 // 16 i + 4 g + w of a key is the w-th of the lane's i-th load, and takes part in
 // the product 4 i + w with the query's element of that place; values need no
 // transposition, a product takes tokens 4 g + i of the four groups.  Wide F32
-// rows take steps of 16 tokens, so that two waves a SIMD have registers (heads
-// of 128, 16 sequences of 4096 tokens: 107 us, 111 with 32 tokens and one wave;
-// of 256: 242, and 584 with 32 tokens, for which there are no registers).
+// rows take steps of 16 tokens for two waves a SIMD, which at heads of 128 still
+// move 8 to 20 registers through scratch memory (16 sequences of 4096 tokens: 107 us,
+// 111 with 32 tokens and one wave; heads of 256: 242, and 584 with 32 tokens).
 //
-// Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16
-// 97 us (5.5 TB/s), FP8 60 us (4.5 TB/s), F32 196 us (5.5 TB/s); 200 of 4000
-// tokens, FP8: 320 us (5.1 TB/s).  More waves a
-// SIMD in fewer registers spill: BF16 at three 142 us.
+// Measured, 64 sequences of 2048 tokens, 8 kv heads of 128, groups of 4: BF16 97 us
+// (5.5 TB/s), FP8 62 us (4.3 TB/s; with block scales 63), F32 195 us (5.5 TB/s);
+// heads of 256, BF16 193 us (5.6 TB/s), FP8 104 (5.2); 200 of 4000 tokens, FP8: 320 us
+// (5.1 TB/s).  More waves a SIMD in fewer registers spill: BF16 at three 142 us.
 //
 // Keys and values that one tile reads are streamed past the caches (5 sequences
 // of 16384 to 32768 tokens: 85 us, 94 without), unless a sequence may have two

@@ -25,8 +25,10 @@
 //   are 2^8 times as large, which changes neither their relative rounding nor the
 //   F32 sums).
 //
-// Measured: a chunk of 8192 tokens, 8 kv heads of 128, groups of 4, BF16: 583 us
-// (940 TFLOP/s); chunks of 2048 tokens at 4096 to 8192: 323 us (805 TFLOP/s).
+// Measured, 8 kv heads of 128, groups of 4, BF16 (from card to card): a chunk of
+// 8192 tokens 583 to 645 us (850 to 940 TFLOP/s), two chunks of 2048 at 4096 to 8192
+// 323 to 340 us (765 to 805); those from FP8 320 to 332, with block scales 380 to 395
+// (F16 405 to 418: its weights need a reference), heads of 256 760 to 775 (680).
 // Matrix and vector instructions of a SIMD's two waves add up to nearly all of
 // it: they overlap little.  The next step's products written between the weights
 // of this one ran slower (402 us for 340), and the products' priority gives 2 %.
@@ -629,11 +631,17 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
 
 // A batch's sequences of few new tokens, beside the ones of many: their
 // workgroups start first, and wait for memory while the others compute (12
-// sequences, 8 of 100 to 500 new tokens with a window of 1024, 4 kv heads of 64:
-// 55 us with the join, 64 as two launches; a chunk that is alone takes 1 to 4 %
-// longer for the code that it does not run).
-// Heads of 64: three waves a SIMD (10 chunks of 256 tokens at 2048, FP8: 90 us,
-// 126 with two).
+// sequences, 4 of them chunks of 100 to 500 new tokens, with a window of 1024, 4 kv
+// heads of 64: 53 us with the join, 9 more as two launches; a chunk that is alone
+// takes 1 to 4 % longer for the code that it does not run).
+//
+// Heads of 64: three waves a SIMD, for which the FP8 forms move 3 to 25 registers
+// through scratch memory (with block scales 15 to 45, those of 128 and 256 up to 20)
+// and the BF16 ones with the token axis innermost 3 to 7.  Short chunks gain by the
+// third wave, long ones lose: 10 chunks of 256 tokens at 2048, FP8, three and two
+// waves: 91 and 109 us, with block scales 119 and 128; 2 of 2048 at 4096 to 8192: 233
+// and 227, with block scales 329 and 295, token axis innermost 257 and 234; BF16 240
+// and 238, token axis innermost 240 and 231.
 struct MixedArgs {
   AttentionArgs many, few;
   uint32_t few_grid;

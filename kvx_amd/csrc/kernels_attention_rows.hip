@@ -1,6 +1,6 @@
 // Attention over a paged cache for everything the matrix-core kernels do not
-// take: head dims that are not multiples of 8 or past 256, strides without
-// 16-byte chunks.
+// take: head dims that are not multiples of 8 (from an FP8 cache of 16) or past 256,
+// strides without 16-byte chunks.
 //
 // A workgroup of four waves has 16 query rows of one kv head; each wave takes
 // every fourth step of 64 tokens.  Products: lane = token, so that its key
@@ -8,8 +8,9 @@
 // queries come from LDS as broadcasts.  Sums: lane = element of the head, 16
 // weights a token from LDS, again broadcasts.  Each key or value element is
 // used 16 times per load, in F32 throughout; LDS and the vector unit bound it
-// (16 sequences of 4096 tokens, 8 kv heads of 100 F32: 336 us, 1.2 TB/s; where
-// the matrix cores can be used, heads of 128 take 107).
+// (16 sequences of 4096 tokens, 8 kv heads of 100 F32: 335 us, 1.2 TB/s; where
+// the matrix cores can be used, heads of 128 take 107; 64 of 2048, FP8 heads of 72:
+// 534 us, 0.3 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "attention.h"

@@ -10,7 +10,8 @@
 //
 // Measured, 64 tensors (32 layers) of 32 KiB blocks: 400 pairs 318 us (5.3 TB/s;
 // a library copy of 2 GiB reaches 4.9), 2 pairs 3.4 us in the kernel and 10.7 us
-// a call, which the host's walk over the layers takes.
+// a call, which the host's walk over the layers takes; element by element (16
+// padded tensors, 400 pairs) 346 us, 1.2 TB/s, where dense blocks take 80.
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"

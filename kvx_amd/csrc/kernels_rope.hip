@@ -19,8 +19,9 @@
 //
 // Measured: 32768 tokens of 32 + 8 + 8 heads of 128, BF16, 163 us (4.9 TB/s);
 // 4 tokens 5.2 us, 251 into an FP8 cache 7.2 us, where a launch's latency is
-// nearly all.  With one query and one key head a token's angles cost more than
-// its bytes (90000 tokens into FP8: 82 us, 1.4 TB/s).
+// nearly all; prefill into an FP8 cache 165 us (4.5 TB/s), in F32 313 (5.1).  With
+// one query and one key head a token's angles cost more than its bytes (90000 tokens
+// into FP8: 75 to 82 us, 1.4 to 1.6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include "kernels.h"

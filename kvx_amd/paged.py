@@ -584,8 +584,9 @@ def rope_write_kv(cache: PagedCache, query: torch.Tensor | None, key: torch.Tens
                   value: torch.Tensor, positions: torch.Tensor, rope: Rope,
                   slot_mapping: torch.Tensor, *, query_out: torch.Tensor | None = None,
                   k_scale=None, v_scale=None, stream=None) -> Status:
-    """Rotates [T, Hq, D] queries into `query_out` (None: in place) and
-    [T, H, D] keys into the paged cache, and writes the values beside them:
+    """Rotates [T, Hq, D] queries into `query_out` (None: in place; else apart
+    from the query) and [T, H, D] keys into the paged cache, and writes the
+    values beside them:
     ``write_kv`` of the rotated keys, each element rounded once.  Tensors may
     have any token and head strides (views of one projection's output).  A
     slot of -1 skips a row's key and value; its query is rotated.  `query`
@@ -668,7 +669,7 @@ def attention(cache: PagedCache, query: torch.Tensor, out: torch.Tensor, block_t
     seq_lens[s] cached tokens, the new ones last.  A row at position p attends
     to the tokens up to p (`causal`; else to all), with a `window` only to the
     last `window` of them.  softmax(scale * q.k) v goes to `out` (like
-    `query`, or the query itself), the natural logarithm of the weights' sum to `lse` (float32 [T,
+    `query` and apart from it, or the query itself), the natural logarithm of the weights' sum to `lse` (float32 [T,
     Hq], or None); `scale` is 1 / sqrt(D) unless given; `softcap` > 0 turns a
     logit x into softcap * tanh(x / softcap).  Hq is a multiple of the cache's
     heads.  Rows that attend to nothing are 0 with lse -inf; rows behind the
@@ -766,7 +767,7 @@ def copy_blocks(caches, pairs: torch.Tensor, *, stream=None) -> Status:
     dst) of `pairs` (int32 / int64 [n, 2]) block src of K and V to block dst,
     in every PagedCache of `caches`.  Rows with an id outside the pool (such
     as -1 padding) are skipped; no dst may be the src or dst of another row.
-    Block-indexed FP8 scales are the caller's to copy.
+    Block-indexed FP8 scales are the caller's to copy with their blocks.
     kvx_launch_copy_blocks."""
     lib = abi.load()
     caches = caches if isinstance(caches, list) else list(caches)
