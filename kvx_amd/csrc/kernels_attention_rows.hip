@@ -139,8 +139,11 @@ __global__ void __launch_bounds__(kRowsThreads) attention_rows_kernel(AttentionA
       l[r] = l[r] * alpha + wave_sum(p);
 #pragma unroll
       for (int j = 0; j < DJ; ++j) acc[r][j] *= alpha;
-      // a page that the row does not see may have any scale
-      pw[lane * kRowTile + r] = seen ? p * vs : 0.0f;
+      // 0: the row does not see the token, whose page may have any scale.  A weight
+      // that vanished is the smallest number instead, so that a value that is not
+      // finite still reaches the row.
+      const float w = p * vs;
+      pw[lane * kRowTile + r] = !seen ? 0.0f : w == 0.0f ? 0x1p-149f : w;
     }
     wave_sync();
     const int count = min(kWave, to - base);

@@ -183,3 +183,30 @@ def test_block_scales_of_split_sequences(window, new, io, table, bs, layout):
                 s.values[b] = POISON[(i + b) % 4]
         assert c.run() == Status.OK
         c.check()
+
+
+@pytest.mark.parametrize("io,cache,D", [("bf16", None, 64), ("f16", None, 64), ("f32", None, 64),
+                                        ("bf16", None, 20), ("f32", None, 20), ("f16", "e5m2", 20)])
+@pytest.mark.parametrize("new", [[1], [40]])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_values_of_tokens_of_next_to_no_weight(io, cache, D, new, bad):
+    """A token whose weight is e^-200 of the others' is attended to all the same:
+    a value that is not finite reaches every row that sees it."""
+    c = AttentionCase(io=io, cache=cache, D=D, lens=[130], new=new, H=1, G=2, scale=0.125)
+    k = torch.zeros(c.rows[0].shape)
+    t = 70
+    page = int(c.tb[0, t // 16])
+    one = 1.0 if cache is None else 1.0 / float(c.kv_scales[0].values[0])
+    k[page, t % 16, :, 0] = -40.0 * one
+    c.q[..., 0] = 40.0
+    c.q_dev.copy_(c.q)
+    c.rows[0] = k.to(c.rows[0].dtype)
+    set_rows(c.cache.key_cache, c.cache.k_layout, c.rows[0])
+    c.rows[1][page, t % 16, 0, 3] = bad
+    set_rows(c.cache.value_cache, c.cache.v_layout, c.rows[1])
+    assert c.run() == Status.OK
+    torch.cuda.synchronize()
+    out = c.out.cpu().double()
+    assert not torch.isfinite(out[..., 3]).any()
+    out[..., 3] = 0
+    assert torch.isfinite(out).all() and torch.isfinite(c.lse).all()
