@@ -159,7 +159,9 @@ typedef enum kvx_attention_flags KVX_ENUM_BASE {
  * count) are not attended to.  A row that attends to nothing is 0 with lse
  * -infinity.  Rows behind the last sequence are left as they were.  Scales of
  * blocks that a row attends to nothing of may be anything, as their tokens may.
- * Sums and softmax statistics are F32. */
+ * Sums and softmax statistics are F32, and so are logits: past 9e7 (F16 queries;
+ * else 1e9) in size their rounding alone leaves the weights' range, and a row may
+ * turn NaN. */
 typedef struct kvx_attention_desc {
   uint32_t size;  /* sizeof(kvx_attention_desc_t) */
   uint32_t flags; /* kvx_attention_flags_t */

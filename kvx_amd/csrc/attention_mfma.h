@@ -52,10 +52,15 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
 // has 11 digits down to 2^-14 and none below 2^-25: with a maximum of 1 a long
 // context would lose the many tokens of small weights (32768 tokens of e^-17.75
 // beside one of 1: all of them).  `room`: how far the maximum may grow, in powers
-// of two, before m follows it; the largest weight is 2^14 or 2^15.
+// of two, before m follows it; the largest weight is 2^14 or 2^15.  Past 2^20 a
+// maximum has few digits behind the point, which are all of its weight's (2^e, e the
+// rounding of m): m is the maximum itself then, so that F16 weights hold out to
+// logits of 2^27, as others to 2^31.
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > 0x1p20f; }
 template <int IO>
-__device__ __forceinline__ constexpr float less_of_maximum(int room) {
-  return IO == KVX_DTYPE_F16 ? (room > 0 ? 15.0f - (float)room : 14.0f) : 0.0f;
+__device__ __forceinline__ float reference_maximum(float top, int room) {
+  if constexpr (IO != KVX_DTYPE_F16) return top;
+  return is_far(top) ? top : top - (room > 0 ? 15.0f - (float)room : 14.0f);
 }
 
 // Block-indexed scales of values multiply the weights, which the products take in

@@ -423,7 +423,7 @@ __device__ __forceinline__ void attention_few(const AttentionArgs &a, size_t arg
 #pragma unroll
       for (int e = 0; e < 4 * HALVES; ++e) top = fmaxf(top, x[e]);  // NaN does not move it
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaf(fmaxf(top, __shfl_xor(top, 32)), scale, -less_of_maximum<IO>(0));
+      top = reference_maximum<IO>(fmaxf(top, __shfl_xor(top, 32)) * scale, 0);
       top = fmaxf(top, m);
       const float shift = top == -INFINITY ? 0.0f : top;
       if (__any(top > m)) {

@@ -47,7 +47,7 @@ constexpr int kManyWaves = 4;
 constexpr int kManyThreads = kManyWaves * kWave;
 static_assert(kManyRowTile == 32 * kManyWaves, "32 rows a wave");
 constexpr int kManyStep = 64;
-constexpr int kRoom = 8;  // see less_of_maximum
+constexpr int kRoom = 8;  // see reference_maximum
 
 // Operands are read from LDS this many products before they are used (about 128
 // cycles of 32 each); scheduling barriers, which vector and scalar operations
@@ -433,8 +433,8 @@ __device__ __forceinline__ void attention_many(const AttentionArgs &a, size_t ar
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);  // NaN does not move it
     }
-    top = fmaf(fmaxf(top, __shfl_xor(top, 32)), scale, -less_of_maximum<IO>(kRoom));
-    if (__any(top > m + (float)kRoom)) {
+    top = reference_maximum<IO>(fmaxf(top, __shfl_xor(top, 32)) * scale, kRoom);
+    if (__any(top > m + (IO == KVX_DTYPE_F16 && is_far(top) ? 0.0f : (float)kRoom))) {
       const float now_m = fmaxf(top, m);
       const float alpha = __builtin_amdgcn_exp2f(m - (now_m == -INFINITY ? 0.0f : now_m));
       m = now_m;

@@ -20,7 +20,7 @@ import torch
 from kvx_amd import paged
 from kvx_amd.abi import Layout, Status
 
-from operator_helpers import AttentionCase, DT, scale_arg
+from operator_helpers import AttentionCase, DT, scale_arg, set_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,43 @@ def test_many_small_weights_beside_one(io, cache, scales, kind):
     assert ((out.cpu().double() - want).abs() <= tol).all()
     want_l = 17.75 + torch.log1p(others * w)[:, None]
     assert ((lse.cpu().double() - want_l).abs() <= (n + 100) * 2.0 ** -24 + 4 * 17.75 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("io,cache,D", [("f16", None, 64), ("f16", "e4m3", 64), ("bf16", None, 128),
+                                        ("f32", None, 64), ("f16", None, 20)])
+@pytest.mark.parametrize("new", [None, [60, 3]])
+@pytest.mark.parametrize("scale", [1e3, 5e4, 3e5])
+def test_logits_past_the_digits_of_f32(io, cache, D, new, scale):
+    """Logits so large that F32 does not tell neighbours apart: the weights stay
+    in their type's range.  One token's logit is far above the others': every row
+    that sees it has its value, the rounding of weight and output aside.  F16
+    weights hold out to logits of 9e7 (2^27 in units of log2, whose rounding is 2^3),
+    others to 1e9 (2^31)."""
+    if io == "f16" and D != 20:
+        scale = min(scale, 5e4)
+    c = AttentionCase(io=io, cache=cache, lens=[130, 90], new=new, H=2, G=4, D=D, scale=scale)
+    assert c.run() == Status.OK
+    torch.cuda.synchronize()
+    assert torch.isfinite(c.out.double()).all() and torch.isfinite(c.lse).all()
+    for s in range(2):
+        b = int(c.tb[s, 1])
+        c.rows[0][b, 3, :, 0] = 400.0 if cache is None else 448.0
+    c.q[..., 0] = 3.0 + torch.rand(c.q.shape[:-1]).to(c.q.dtype)
+    c.q_dev.copy_(c.q)
+    set_rows(c.cache.key_cache, c.cache.k_layout, c.rows[0])
+    if cache:
+        c.kv_scales[0].values.fill_(0.9)
+        c.rows[0][...] = (c.rows[0].float() / 448).to(c.rows[0].dtype)
+        for s in range(2):
+            c.rows[0][int(c.tb[s, 1]), 3, :, 0] = 448.0
+        set_rows(c.cache.key_cache, c.cache.k_layout, c.rows[0])
+    assert c.run() == Status.OK
+    torch.cuda.synchronize()
+    out, row = c.out.cpu().double(), 0
+    half = torch.finfo(DT[io]).eps / 2
+    for s, (n, m) in enumerate(zip(c.lens, c.new)):
+        v = c.exact[1][int(c.tb[s, 1]), 3].repeat_interleave(c.G, 0)
+        for i in range(m):
+            if n - m + i >= 19:
+                assert ((out[row] - v).abs() <= 4 * half * v.abs() + 2.0 ** -24).all()
+            row += 1
